@@ -85,7 +85,7 @@ class StepPlan(C.Structure):
 # == FSGS_ABI_VERSION of include/fsgs.h as of the SIGNATURES table below: load() refuses any other library (a stale
 # build — the .so files are git-ignored and travel separately, A/B builds come in through FSGS_LIB — would read a stream
 # pointer as a flag or write past a buffer that has since grown)
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 SIGNATURES = {
     "fsgs_version": (_i, []),
@@ -207,6 +207,12 @@ SIGNATURES = {
     "fsgs_step_backward": (_i, [C.POINTER(StepPlan), _i64, C.POINTER(_i64), _p]),
     "fsgs_step_run": (_i, [C.POINTER(StepPlan), _i64, C.POINTER(_i64), _p]),
     "fsgs_step_plan_bytes": (_i64, []),
+    "fsgs_linear_fwd": (_i, [_i64, _i, _i, _i, _p, _i64, _p, _p, _i, _p, _i64, _p, _p]),
+    "fsgs_linear_bwd_scratch_bytes": (_i64, [_i64, _i, _i, _i, _i, _i, _i, _i]),
+    "fsgs_linear_bwd": (_i, [_i64, _i, _i, _i, _p, _i64, _p, _p, _i, _p, _i64, _p, _p, _p, _p, _i64, _p]),
+    "fsgs_distill_scratch_bytes": (_i64, []),
+    "fsgs_distill_fwd": (_i, [_i64, _i, _i, _i, _p, _i64, _i, _p, _i64, _i, _p, _i64, _p, _f, _i, _p, _p, _p, _p, _i64, _p]),
+    "fsgs_distill_bwd": (_i, [_i64, _i, _i, _i, _p, _i64, _i, _p, _i64, _i, _p, _i64, _p, _f, _p, _p, _p, _i, _p, _p]),
 }
 
 _lib: Optional[C.CDLL] = None

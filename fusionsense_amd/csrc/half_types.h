@@ -1,0 +1,62 @@
+// The three element types of the semantic-head operators (fp32 / bf16 / fp16) and their matrix instructions.
+#pragma once
+#include "common.h"
+
+namespace fsgs {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// A chunk is 16 bytes of a row: what a lane loads, stores and feeds to the matrix pipe at a time.
+struct alignas(16) Chunk {
+    uint32_t u[4];
+};
+
+template <typename T>
+constexpr int kChunk = 16 / (int)sizeof(T);
+
+// `p` is aligned to its element only (rows of odd length start anywhere): gfx950 takes vector accesses at any byte address,
+// so the compiler keeps these as one access.
+template <typename T>
+__device__ __forceinline__ Chunk load_chunk(const T *p) {
+    Chunk c;
+    __builtin_memcpy(&c, p, sizeof(Chunk));
+    return c;
+}
+
+// The first `n` elements (n <= 0: none), the others zero; nothing behind the n-th is touched.
+template <typename T>
+__device__ __forceinline__ Chunk load_chunk_n(const T *p, int n) {
+    if (n >= kChunk<T>) return load_chunk(p);
+    T v[kChunk<T>];
+#pragma unroll
+    for (int i = 0; i < kChunk<T>; ++i) v[i] = i < n ? p[i] : (T)0.f;
+    Chunk c;
+    __builtin_memcpy(&c, v, sizeof(Chunk));
+    return c;
+}
+
+// acc += A B for one 16x16 tile: lane l holds row (l & 15) of A and column (l & 15) of B; its 16 bytes cover the same part
+// of the summed axis in both, so their order along that axis does not matter.  Result: column l & 15, rows 4 (l >> 4) .. + 3.
+template <typename T>
+__device__ __forceinline__ void mma_chunk(f32x4 &acc, const Chunk &a, const Chunk &b);
+template <>
+__device__ __forceinline__ void mma_chunk<__bf16>(f32x4 &acc, const Chunk &a, const Chunk &b) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ void mma_chunk<_Float16>(f32x4 &acc, const Chunk &a, const Chunk &b) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ void mma_chunk<float>(f32x4 &acc, const Chunk &a, const Chunk &b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, a.u[i]), __builtin_bit_cast(float, b.u[i]), acc,
+                                                   0, 0, 0);
+}
+
+inline bool known_dtype(int d) { return d == FSGS_F32 || d == FSGS_BF16 || d == FSGS_F16; }
+
+}  // namespace fsgs

@@ -1,0 +1,389 @@
+// One layer of the semantic head: y = act(x W^T + b) + r and its backward pass.
+//
+//   forward    z = x W^T + b, y = act(z) + r                       x [M,K], W [N,K], y [M,N]
+//   backward   dz = dy * act'(z) (z formed again from x: M*K values are read instead of M*N kept), dx = dz W,
+//              dW = dz^T x, db = sum_m dz, dr = dy
+//
+// Products run on the matrix cores in the tensors' own type, sums are fp32 throughout (fp32 tensors use the fp32 matrix
+// instructions: no reduced-precision product).
+#include "half_types.h"
+
+namespace fsgs {
+
+namespace {
+
+constexpr int kBM = 128;      // rows of x per tile
+constexpr int kSlabBytes = 128;  // one step along the summed axis: 64 half-width or 32 fp32 values
+
+struct LinArgs {
+    const void *x, *w, *bias, *res, *dy;
+    void *y;
+    int64_t rows, xp, rp, dyp, yp;
+    int K, N, act;
+};
+
+__device__ __forceinline__ float act_fwd(float z, int act) {
+    switch (act) {
+        case FSGS_ACT_RELU: return z > 0.f ? z : (z == z ? 0.f : z);
+        case FSGS_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case FSGS_ACT_SILU: return z / (1.f + expf(-z));
+        default: return z;
+    }
+}
+
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case FSGS_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+        case FSGS_ACT_GELU:
+            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+        case FSGS_ACT_SILU: {
+            const float s = 1.f / (1.f + expf(-z));
+            return s * (1.f + z * (1.f - s));
+        }
+        default: return 1.f;
+    }
+}
+
+enum { kModeFwd = 0, kModeDz = 1 };
+
+// Tile of 128 rows x BN columns, four waves of 64 x BN/2.  Both operands go through LDS in 128-byte slabs of the summed
+// axis; W is the A operand, so that a lane ends with four neighbouring columns of one row and stores them together.
+template <typename T, int MODE, int BN>
+__global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
+    constexpr int CE = kChunk<T>, BK = kSlabBytes / (int)sizeof(T);
+    constexpr int NT = BN / 32, MT = 4;
+    constexpr int XL = kBM * 8 / 256, WL = BN * 8 / 256;  // chunks per thread and slab
+    __shared__ Chunk xs[kBM * 8], ws[BN * 8];
+    const T *x = (const T *)a.x, *w = (const T *)a.w;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int ntiles_n = (a.N + BN - 1) / BN;
+    const int64_t tile = blockIdx.x;
+    const int64_t m0 = (tile / ntiles_n) * kBM;
+    const int n0 = (int)(tile % ntiles_n) * BN;
+    const int wm = (wave & 1) * 64, wn = (wave >> 1) * (BN / 2);
+    const int li = lane & 15, lg = lane >> 4;
+
+    f32x4 acc[NT][MT] = {};
+    Chunk xr[XL], wr[WL];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const int c = tid + i * 256, r = c >> 3, k = k0 + (c & 7) * CE;
+            const int64_t m = m0 + r;
+            xr[i] = load_chunk_n(x + m * a.xp + k, m < a.rows ? a.K - k : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+            const int c = tid + i * 256, r = c >> 3, k = k0 + (c & 7) * CE;
+            const int n = n0 + r;
+            wr[i] = load_chunk_n(w + (int64_t)n * a.K + k, n < a.N ? a.K - k : 0);
+        }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < a.K; k0 += BK) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const int c = tid + i * 256, r = c >> 3;
+            xs[r * 8 + ((c & 7) ^ (r & 7))] = xr[i];
+        }
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+            const int c = tid + i * 256, r = c >> 3;
+            ws[r * 8 + ((c & 7) ^ (r & 7))] = wr[i];
+        }
+        __syncthreads();
+        if (k0 + BK < a.K) fetch(k0 + BK);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            Chunk xf[MT], wf[NT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int r = wm + i * 16 + li;
+                xf[i] = xs[r * 8 + ((s * 4 + lg) ^ (r & 7))];
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int r = wn + i * 16 + li;
+                wf[i] = ws[r * 8 + ((s * 4 + lg) ^ (r & 7))];
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) mma_chunk<T>(acc[i][j], wf[i], xf[j]);
+        }
+    }
+
+    const T *bias = (const T *)a.bias;
+    T *y = (T *)a.y;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int n = n0 + wn + i * 16 + lg * 4;
+        const int nv = min(4, a.N - n);
+        if (nv <= 0) continue;
+        float b[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) b[q] = bias && q < nv ? (float)bias[n + q] : 0.f;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int64_t m = m0 + wm + j * 16 + li;
+            if (m >= a.rows) continue;
+            const T *side = MODE == kModeDz ? (const T *)a.dy + m * a.dyp + n
+                            : a.res         ? (const T *)a.res + m * a.rp + n
+                                            : nullptr;
+            T sv[4], out[4];
+            if (side) {
+                if (nv == 4) __builtin_memcpy(sv, side, sizeof(sv));
+                else for (int q = 0; q < nv; ++q) sv[q] = side[q];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float z = acc[i][j][q] + b[q];
+                float v;
+                if constexpr (MODE == kModeDz) v = (float)sv[q] * act_slope(z, a.act);
+                else v = act_fwd(z, a.act) + (side ? (float)sv[q] : 0.f);
+                out[q] = (T)v;
+            }
+            T *dst = y + m * a.yp + n;
+            if (nv == 4) __builtin_memcpy(dst, out, sizeof(out));
+            else for (int q = 0; q < nv; ++q) dst[q] = out[q];
+        }
+    }
+}
+
+// W [N,K] -> W^T [K,N]: the operand of dx = dz W with its summed axis contiguous.
+template <typename T>
+__global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w, T *__restrict__ wt, int N, int K) {
+    __shared__ T t[32][33];
+    const int k0 = blockIdx.x * 32, n0 = blockIdx.y * 32;
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+    for (int i = r; i < 32; i += 8)
+        if (n0 + i < N && k0 + c < K) t[i][c] = w[(int64_t)(n0 + i) * K + k0 + c];
+    __syncthreads();
+    for (int i = r; i < 32; i += 8)
+        if (k0 + i < K && n0 + c < N) wt[(int64_t)(k0 + i) * N + n0 + c] = t[c][i];
+}
+
+struct DwArgs {
+    const void *dz, *x;
+    float *part_w, *part_b;  // [slices][N*K], [slices][N]
+    int64_t rows, dzp, xp, slice_rows;
+    int K, N;
+};
+
+// dW tile of 64 columns of dz x 64 columns of x over one slice of the rows, db beside it (tiles of k = 0: dz against ones).
+template <typename T>
+__global__ __launch_bounds__(256) void linear_dw_kernel(DwArgs a) {
+    constexpr int CE = kChunk<T>, MS = 32, CPR = 64 / CE, L = MS * CPR / 256 > 0 ? MS * CPR / 256 : 1;
+    __shared__ T ds[MS][64 + CE], xs[MS][64 + CE];
+    const T *dz = (const T *)a.dz, *x = (const T *)a.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int k0 = blockIdx.x * 64, n0 = blockIdx.y * 64, slice = blockIdx.z;
+    const int wn = (wave >> 1) * 32, wk = (wave & 1) * 32;
+    const int li = lane & 15, lg = lane >> 4;
+    const int64_t mb = slice * a.slice_rows, me = min(a.rows, mb + a.slice_rows);
+    const bool want_b = a.part_b && k0 == 0 && wk == 0;
+    f32x4 acc[2][2] = {}, accb[2] = {};
+    for (int64_t m0 = mb; m0 < me; m0 += MS) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int c = tid + i * 256, r = c / CPR, col = (c % CPR) * CE;
+            const int64_t m = m0 + r;
+            const Chunk cd = load_chunk_n(dz + m * a.dzp + n0 + col, m < me ? a.N - n0 - col : 0);
+            const Chunk cx = load_chunk_n(x + m * a.xp + k0 + col, m < me ? a.K - k0 - col : 0);
+            *(Chunk *)&ds[r][col] = cd;
+            *(Chunk *)&xs[r][col] = cx;
+        }
+        __syncthreads();
+        constexpr int STEPS = sizeof(T) == 2 ? 1 : 2;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            Chunk df[2], xf[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                T vd[CE], vx[CE];
+#pragma unroll
+                for (int e = 0; e < CE; ++e) {
+                    const int r = (s * 4 + lg) * CE + e;
+                    vd[e] = ds[r][wn + t * 16 + li];
+                    vx[e] = xs[r][wk + t * 16 + li];
+                }
+                __builtin_memcpy(&df[t], vd, 16);
+                __builtin_memcpy(&xf[t], vx, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], df[i], xf[j]);
+            if (want_b) {
+                T one[CE];
+#pragma unroll
+                for (int e = 0; e < CE; ++e) one[e] = (T)1.f;
+                Chunk of;
+                __builtin_memcpy(&of, one, 16);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mma_chunk<T>(accb[i], df[i], of);
+            }
+        }
+    }
+    float *pw = a.part_w ? a.part_w + (int64_t)slice * a.N * a.K : nullptr;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = n0 + wn + i * 16 + lg * 4 + q;
+            if (n >= a.N) continue;
+            if (pw)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int k = k0 + wk + j * 16 + li;
+                    if (k < a.K) pw[(int64_t)n * a.K + k] = acc[i][j][q];
+                }
+            if (want_b && li == 0) a.part_b[(int64_t)slice * a.N + n] = accb[i][q];
+        }
+}
+
+// Sum of the slices' partial gradients, in the slices' order.
+template <typename T>
+__global__ __launch_bounds__(256) void reduce_slices_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b,
+                                                            T *__restrict__ dw, T *__restrict__ db, int64_t nk, int N,
+                                                            int slices) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < nk) {
+        if (!dw) return;
+        float s = 0.f;
+        for (int t = 0; t < slices; ++t) s += part_w[t * nk + i];
+        dw[i] = (T)s;
+    } else if (db && i - nk < N) {
+        float s = 0.f;
+        for (int t = 0; t < slices; ++t) s += part_b[(int64_t)t * N + (i - nk)];
+        db[i - nk] = (T)s;
+    }
+}
+
+template <typename T, int MODE>
+int launch_tile(const LinArgs &a, hipStream_t s) {
+    const int64_t mt = (a.rows + kBM - 1) / kBM;
+    const int bn = a.N > 64 ? 128 : 64;
+    const int64_t tiles = mt * ((a.N + bn - 1) / bn);
+    if (tiles > (int64_t)UINT32_MAX / 256) return FSGS_EINVAL;  // (a grid holds at most 2^32 threads)
+    if (bn == 128) linear_tile_kernel<T, MODE, 128><<<(unsigned)tiles, 256, 0, s>>>(a);
+    else linear_tile_kernel<T, MODE, 64><<<(unsigned)tiles, 256, 0, s>>>(a);
+    return check_launch();
+}
+
+int dw_slices(int64_t rows, int K, int N) {
+    const int64_t tiles = (int64_t)((K + 63) / 64) * ((N + 63) / 64);
+    const int64_t want = (1024 + tiles - 1) / tiles, most = (rows + 255) / 256;
+    const int64_t s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : s);
+}
+
+struct BwdScratch {
+    size_t dz, wt, part_w, part_b, total;
+};
+
+BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bool dw, bool db) {
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    BwdScratch l;
+    const size_t s = (size_t)dw_slices(rows, K, N);
+    l.dz = 0;
+    l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
+    l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
+    l.part_b = l.part_w + (dw ? up(s * (size_t)K * N * 4) : 0);
+    l.total = l.part_b + (db ? up(s * (size_t)N * 4) : 0);
+    return l;
+}
+
+template <typename T>
+int run_bwd(LinArgs a, void *dx, void *dw, void *db, char *scratch, const BwdScratch &l, hipStream_t s) {
+    const void *dz = a.dy;
+    int64_t dzp = a.dyp;
+    if (a.act != FSGS_ACT_NONE) {
+        LinArgs z = a;
+        z.y = scratch + l.dz;
+        z.yp = a.N;
+        const int rc = launch_tile<T, kModeDz>(z, s);
+        if (rc != FSGS_OK) return rc;
+        dz = z.y;
+        dzp = a.N;
+    }
+    if (dx) {
+        T *wt = (T *)(scratch + l.wt);
+        transpose_kernel<T><<<dim3((a.K + 31) / 32, (a.N + 31) / 32), 256, 0, s>>>((const T *)a.w, wt, a.N, a.K);
+        int rc = check_launch();
+        if (rc != FSGS_OK) return rc;
+        LinArgs g = {};
+        g.x = dz, g.xp = dzp, g.w = wt, g.y = dx, g.yp = a.K, g.rows = a.rows, g.K = a.N, g.N = a.K;
+        rc = launch_tile<T, kModeFwd>(g, s);
+        if (rc != FSGS_OK) return rc;
+    }
+    if (dw || db) {
+        DwArgs d = {};
+        const int slices = dw_slices(a.rows, a.K, a.N);
+        d.dz = dz, d.dzp = dzp, d.x = a.x, d.xp = a.xp, d.rows = a.rows, d.K = a.K, d.N = a.N;
+        d.part_w = dw ? (float *)(scratch + l.part_w) : nullptr;
+        d.part_b = db ? (float *)(scratch + l.part_b) : nullptr;
+        d.slice_rows = (((a.rows + slices - 1) / slices) + 31) / 32 * 32;
+        const int kt = dw ? (a.K + 63) / 64 : 1;
+        linear_dw_kernel<T><<<dim3(kt, (a.N + 63) / 64, slices), 256, 0, s>>>(d);
+        int rc = check_launch();
+        if (rc != FSGS_OK) return rc;
+        const int64_t nk = (int64_t)a.N * a.K;
+        reduce_slices_kernel<T><<<(unsigned)((nk + a.N + 255) / 256), 256, 0, s>>>(d.part_w, d.part_b, (T *)dw, (T *)db, nk,
+                                                                                  a.N, slices);
+        return check_launch();
+    }
+    return FSGS_OK;
+}
+
+bool bad_sizes(int64_t rows, int K, int N, int dtype, int act) {
+    return rows < 0 || rows > INT32_MAX || K < 1 || N < 1 || K > FSGS_LINEAR_MAX_DIM || N > FSGS_LINEAR_MAX_DIM || !known_dtype(dtype) ||
+           act < FSGS_ACT_NONE || act > FSGS_ACT_SILU;
+}
+
+}  // namespace
+}  // namespace fsgs
+
+using namespace fsgs;
+
+extern "C" int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype, const void *x, int64_t x_pitch, const void *w,
+                               const void *bias, int act, const void *residual, int64_t res_pitch, void *y,
+                               fsgs_stream_t stream) {
+    if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
+    if (rows == 0) return FSGS_OK;
+    if (!x || !w || !y || x_pitch < 0 || res_pitch < 0) return FSGS_EINVAL;
+    LinArgs a = {};
+    a.x = x, a.xp = x_pitch, a.w = w, a.bias = bias, a.res = residual, a.rp = res_pitch, a.y = y, a.yp = out_dim;
+    a.rows = rows, a.K = in_dim, a.N = out_dim, a.act = act;
+    switch (dtype) {
+        case FSGS_F32: return launch_tile<float, kModeFwd>(a, as_stream(stream));
+        case FSGS_BF16: return launch_tile<__bf16, kModeFwd>(a, as_stream(stream));
+        default: return launch_tile<_Float16, kModeFwd>(a, as_stream(stream));
+    }
+}
+
+extern "C" int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int act, int want_dx,
+                                                 int want_dw, int want_db) {
+    if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
+    return (int64_t)bwd_layout(rows, in_dim, out_dim, dtype == FSGS_F32 ? 4 : 2, act, want_dx, want_dw, want_db).total;
+}
+
+extern "C" int fsgs_linear_bwd(int64_t rows, int in_dim, int out_dim, int dtype, const void *x, int64_t x_pitch, const void *w,
+                               const void *bias, int act, const void *dy, int64_t dy_pitch, void *dx, void *dw, void *db,
+                               void *scratch, int64_t scratch_bytes, fsgs_stream_t stream) {
+    if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
+    if (rows == 0 || (!dx && !dw && !db)) return FSGS_OK;
+    if (!x || !w || !dy || x_pitch < 0 || dy_pitch < 0) return FSGS_EINVAL;
+    const BwdScratch l = bwd_layout(rows, in_dim, out_dim, dtype == FSGS_F32 ? 4 : 2, act, dx, dw, db);
+    if (l.total > 0 && (!scratch || scratch_bytes < (int64_t)l.total)) return FSGS_ESCRATCH;
+    LinArgs a = {};
+    a.x = x, a.xp = x_pitch, a.w = w, a.bias = bias, a.dy = dy, a.dyp = dy_pitch;
+    a.rows = rows, a.K = in_dim, a.N = out_dim, a.act = act;
+    switch (dtype) {
+        case FSGS_F32: return run_bwd<float>(a, dx, dw, db, (char *)scratch, l, as_stream(stream));
+        case FSGS_BF16: return run_bwd<__bf16>(a, dx, dw, db, (char *)scratch, l, as_stream(stream));
+        default: return run_bwd<_Float16>(a, dx, dw, db, (char *)scratch, l, as_stream(stream));
+    }
+}

@@ -47,6 +47,7 @@ def render_fusionsense(
     crop_box=None,
     training: bool = True,
     binary_threshold: Optional[float] = None,
+    semantic_head=None,
 ) -> Dict[str, Tensor]:
     """One ``get_outputs`` call.  ``gauss_params`` uses the reference's stored parametrisation
     (dn_model.py:294-304): means, scales (log), quats, features_dc [N,3], features_rest [N,K-1,3],
@@ -54,8 +55,14 @@ def render_fusionsense(
     ``binary_threshold``: perform the binary-opacity write of :492-503 (the caller decides with
     ``splatfacto.binary_opacity_active``); ``crop_box`` (:class:`fusionsense_amd.crop.OrientedBox`) is used
     only when not ``training`` (:505-532); ``add_mask`` [N] bool marks the touch anchors whose means /
-    opacities / scales receive no gradient (:535-541)."""
+    opacities / scales receive no gradient (:535-541).
+
+    ``semantic_head`` (:class:`fusionsense_amd.semantics.SemanticHead`) with ``gauss_params["semantics"]`` [N,D] adds
+    "semantic_features" [H,W,D], the rows composited over zeros, and "semantic_logits" [H,W,V].  Their gradients reach the
+    rows and the head; the geometry is learned from the images alone, so they stop at it."""
     dev = device or gauss_params["means"].device
+    if semantic_head is not None and "semantics" not in gauss_params:
+        raise ValueError("semantic_head needs gauss_params['semantics'] [N,D]")
     if binary_threshold is not None:
         from .splatfacto import binary_opacity_write_
         binary_opacity_write_(gauss_params["opacities"], binary_threshold)
@@ -64,7 +71,11 @@ def render_fusionsense(
         crop_ids = crop_box.within(gauss_params["means"].detach())
         if crop_ids.sum() == 0:
             bg = background if background is not None else torch.ones(3, device=dev)
-            return get_empty_outputs(camera.width, camera.height, bg)
+            empty = get_empty_outputs(camera.width, camera.height, bg)
+            if semantic_head is not None:
+                plane = gauss_params["semantics"].new_zeros(camera.height, camera.width, gauss_params["semantics"].shape[1])
+                empty.update(semantic_features=plane, semantic_logits=semantic_head(plane))
+            return empty
         gauss_params = crop_params(gauss_params, crop_ids)
     means = gauss_params["means"]
     scales = gauss_params["scales"]
@@ -142,7 +153,16 @@ def render_fusionsense(
         )
         normals_im = normals_im / normals_im.norm(dim=-1, keepdim=True)
         normals_im = (normals_im + 1) / 2
+    semantic = {}
+    if semantic_head is not None:
+        plane, _, _ = rasterization(
+            means=means.detach(), quats=(quats / quats.norm(dim=-1, keepdim=True)).detach(), scales=torch.exp(scales.detach()),
+            opacities=torch.sigmoid(opacities.detach()).squeeze(-1), colors=gauss_params["semantics"], viewmats=viewmat, Ks=K,
+            width=W, height=H, tile_size=BLOCK_WIDTH, packed=False, near_plane=0.01, far_plane=1e10, render_mode="RGB",
+            sh_degree=None, rasterize_mode=rasterize_mode)
+        semantic = {"semantic_features": plane.squeeze(0), "semantic_logits": semantic_head(plane.squeeze(0))}
     return {
+        **semantic,
         "rgb": rgb.squeeze(0),
         "depth": depth_im,
         "normal": normals_im,

@@ -7,6 +7,7 @@ all arithmetic happens in libfsgs.so.  There is no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 import os
@@ -1787,3 +1788,202 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, lrs, step: int, beta1: floa
                               VP(*[m.data_ptr() for m in exp_avgs]), VP(*[v.data_ptr() for v in exp_avg_sqs]),
                               numel, lr, int(step), float(beta1), float(beta2), float(eps), stream_ptr(dev)),
          "fsgs_adam_step")
+
+
+# --------------------------------------------------------------------------------------
+# the semantic head: one layer (matrix product + bias + activation + residual), and the distillation loss that trains it
+# --------------------------------------------------------------------------------------
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+LINEAR_MAX_DIM = 65536
+DISTILL_MAX_K = 256
+DISTILL_T_RANGE = (1e-6, 1e6)
+
+
+def _on_device(dev: torch.device):
+    """The tensors' device as the current one: a launch on another device's stream is an error.  (No cost where it is.)"""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
+    """``t`` [..., width] -> (tensor whose storage the kernels read, elements between two rows).  A tensor whose rows lie at
+    one pitch (a slice of a wider plane, an expanded row) is read in place, any other is copied once."""
+    if t.numel() == 0:
+        return t, width
+    t2 = t.reshape(-1, width)
+    if width > 1 and t2.stride(1) != 1:
+        t2 = t2.contiguous()
+    return t2, (t2.stride(0) if t2.shape[0] > 1 else width)
+
+
+class _LinearAct(torch.autograd.Function):
+    """act(x W^T + b) + residual; the backward forms the pre-activation again instead of keeping it."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        lib = load()
+        dev = x.device
+        N, K = weight.shape
+        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
+        weight, bias = _c(weight), _c(bias)
+        if y.numel() > 0:
+            x2, xp = _rows(x, K)
+            r2, rp = _rows(residual, N) if residual is not None else (None, 0)
+            with _on_device(dev):
+                _run(lib.fsgs_linear_fwd, (x2.shape[0], K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), act,
+                                           r2.data_ptr() if r2 is not None else None, rp, ptr(y), stream_ptr(dev)),
+                     "fsgs_linear_fwd")
+        ctx.save_for_backward(x, weight, bias)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias = ctx.saved_tensors
+        lib = load()
+        dev = x.device
+        N, K = weight.shape
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        need_b = need_b and bias is not None
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        rows = x.numel() // K
+        new = torch.empty if rows > 0 else torch.zeros
+        dw = new(N, K, dtype=x.dtype, device=dev) if need_w else None
+        db = new(N, dtype=x.dtype, device=dev) if need_b else None
+        if rows > 0 and (need_x or need_w or need_b):
+            x2, xp = _rows(x, K)
+            g2, gp = _rows(dy, N)
+            with _on_device(dev):
+                nbytes = lib.fsgs_linear_bwd_scratch_bytes(rows, K, N, DTYPES[x.dtype], ctx.act, int(need_x), int(need_w),
+                                                           int(need_b))
+                scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+                _run(lib.fsgs_linear_bwd, (rows, K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), ctx.act,
+                                           g2.data_ptr(), gp, ptr(dx), ptr(dw), ptr(db), ptr(scratch), nbytes,
+                                           stream_ptr(dev)), "fsgs_linear_bwd")
+        return dx, dw, db, (dy if need_r else None), None
+
+
+def _require_float(t: Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a torch.Tensor")
+    if t.dtype not in DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must live on the GPU (there is no CPU path); got device {t.device}")
+
+
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: str = "none",
+               residual: Optional[Tensor] = None) -> Tensor:
+    """One layer of the semantic head in one launch: ``act(x @ weight.T + bias) + residual``.
+
+    ``x`` [..., in], ``weight`` [out, in], ``bias`` [out], ``residual`` [..., out]: one element type (float32, bfloat16,
+    float16) on one device; products in that type, sums in float32, one rounding at the end.  ``act`` is "none", "relu",
+    "gelu" (the erf form) or "silu".  Rows of ``x`` and ``residual`` may lie at any pitch (slices of a wider plane are read in
+    place).  Differentiable in all four tensors, once; the backward forms the pre-activation again from ``x``.  In the
+    half-width types the gradient of the pre-activation is rounded to that type before its two products (the rounding an
+    unfused layer makes when it stores that gradient)."""
+    _require_float(x, "x")
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is None and name != "weight":
+            continue
+        _require_float(t, name)
+        if t.dtype != x.dtype or t.device != x.device:
+            raise ValueError(f"{name} must be {x.dtype} on {x.device} like x, got {t.dtype} on {t.device}")
+    if weight.dim() != 2 or not all(1 <= d <= LINEAR_MAX_DIM for d in weight.shape):
+        raise ValueError(f"weight must be [out,in] with sizes in [1,{LINEAR_MAX_DIM}], got {tuple(weight.shape)}")
+    N, K = weight.shape
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"x must be [...,{K}], got {tuple(x.shape)}")
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + (N,):
+        raise ValueError(f"residual must be {tuple(x.shape[:-1] + (N,))}, got {tuple(residual.shape)}")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
+    return _LinearAct.apply(x, weight, bias, residual, ACTIVATIONS[act])
+
+
+class _TopkDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, idx, teacher, weight, temperature, reduction):
+        lib = load()
+        dev = logits.device
+        V, K = logits.shape[-1], idx.shape[-1]
+        rows = idx.numel() // K
+        per_row = reduction == REDUCTIONS["none"]
+        loss = torch.empty(logits.shape[:-1] if per_row else (), dtype=torch.float32, device=dev)
+        need = ctx.needs_input_grad[0]
+        stat = torch.empty(rows, 4, dtype=torch.float32, device=dev) if need else None
+        inv_w = torch.empty(1, dtype=torch.float32, device=dev) if need and not per_row else None
+        s2, sp = _rows(logits, V)
+        i2, ip = _rows(idx, K)
+        t2, tp = _rows(teacher, K)
+        w1 = weight.reshape(-1).contiguous() if weight is not None else None
+        with _on_device(dev):
+            nbytes = 0 if per_row else lib.fsgs_distill_scratch_bytes()
+            scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+            _run(lib.fsgs_distill_fwd, (rows, V, K, DTYPES[logits.dtype], s2.data_ptr(), sp, 64 if idx.dtype == torch.int64 else 32,
+                                        i2.data_ptr(), ip, DTYPES[teacher.dtype], t2.data_ptr(), tp, ptr(w1), temperature,
+                                        reduction, loss.data_ptr(), ptr(stat), ptr(inv_w), ptr(scratch), nbytes,
+                                        stream_ptr(dev)), "fsgs_distill_fwd")
+        ctx.save_for_backward(logits, idx, teacher, w1, stat, inv_w)
+        ctx.cfg = (temperature, per_row)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        logits, idx, teacher, w1, stat, inv_w = ctx.saved_tensors
+        temperature, per_row = ctx.cfg
+        lib = load()
+        dev = logits.device
+        V, K = logits.shape[-1], idx.shape[-1]
+        rows = idx.numel() // K
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        if rows > 0:
+            s2, sp = _rows(logits, V)
+            i2, ip = _rows(idx, K)
+            t2, tp = _rows(teacher, K)
+            g1 = g.reshape(-1).contiguous()
+            with _on_device(dev):
+                _run(lib.fsgs_distill_bwd, (rows, V, K, DTYPES[logits.dtype], s2.data_ptr(), sp,
+                                            64 if idx.dtype == torch.int64 else 32, i2.data_ptr(), ip, DTYPES[teacher.dtype],
+                                            t2.data_ptr(), tp, ptr(w1), temperature, ptr(stat), ptr(inv_w), ptr(g1),
+                                            int(per_row), ptr(grad), stream_ptr(dev)), "fsgs_distill_bwd")
+        return grad, None, None, None, None, None
+
+
+def topk_distill(logits: Tensor, teacher_idx: Tensor, teacher_logits: Tensor, temperature: float = 1.0,
+                 weight: Optional[Tensor] = None, reduction: str = "mean") -> Tensor:
+    """The operator behind :func:`fusionsense_amd.losses.topk_distill_loss` (see there)."""
+    _require_float(logits, "logits")
+    _require_float(teacher_logits, "teacher_logits")
+    if not isinstance(teacher_idx, torch.Tensor) or teacher_idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_idx must be an int32 or int64 tensor")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be [...,V] with V >= 1, got {tuple(logits.shape)}")
+    lead = logits.shape[:-1]
+    if teacher_idx.dim() != logits.dim() or teacher_idx.shape[:-1] != lead or not 1 <= teacher_idx.shape[-1] <= DISTILL_MAX_K:
+        raise ValueError(f"teacher_idx must be {tuple(lead)} + [K] with K in [1,{DISTILL_MAX_K}], got {tuple(teacher_idx.shape)}")
+    if teacher_logits.shape != teacher_idx.shape:
+        raise ValueError(f"teacher_logits must be {tuple(teacher_idx.shape)} like teacher_idx, got {tuple(teacher_logits.shape)}")
+    for name, t in (("teacher_idx", teacher_idx), ("teacher_logits", teacher_logits), ("weight", weight)):
+        if t is not None and isinstance(t, torch.Tensor) and t.device != logits.device:
+            raise ValueError(f"{name} must be on {logits.device} like logits, got {t.device}")
+    if teacher_logits.requires_grad or (weight is not None and weight.requires_grad):
+        raise ValueError("the teacher's scores and the weights are constants: detach them")
+    if weight is not None:
+        if weight.shape != lead:
+            raise ValueError(f"weight must be {tuple(lead)}, got {tuple(weight.shape)}")
+        if weight.dtype != torch.float32:
+            weight = weight.to(torch.float32)  # (a bool mask, or weights in half width)
+    temperature = float(temperature)
+    if not DISTILL_T_RANGE[0] <= temperature <= DISTILL_T_RANGE[1]:
+        raise ValueError(f"temperature must lie in {DISTILL_T_RANGE}, got {temperature}")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(REDUCTIONS)}, got {reduction!r}")
+    return _TopkDistill.apply(logits, teacher_idx, teacher_logits, weight, temperature, REDUCTIONS[reduction])

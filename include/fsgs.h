@@ -10,7 +10,8 @@
  * (registered at dn_splatter/dn_model.py:1385-1389).
  *
  * Conventions (all entry points):
- *   - plain pointers to DEVICE memory + sizes; no torch types; fp32 / int32 / int64 only
+ *   - plain pointers to DEVICE memory + sizes; no torch types; fp32 / int32 / int64 only (the semantic
+ *     head's operators also take bf16 / fp16, named by an FSGS_* element type)
  *   - all tensors contiguous, row-major, layouts as in the per-function comments
  *   - the caller owns every buffer (including scratch); the library never allocates
  *   - every call enqueues on `stream` (a hipStream_t passed as void*) and returns at once;
@@ -43,7 +44,7 @@ typedef void *fsgs_stream_t; /* hipStream_t */
 #define FSGS_ESCRATCH -3 /* scratch arena too small */
 #define FSGS_EPROTOCOL -4 /* a bounded cross-workgroup / host wait ran into its bound, or calls arrived out of order */
 
-#define FSGS_ABI_VERSION 10
+#define FSGS_ABI_VERSION 11
 int fsgs_version(void);
 int fsgs_abi_version(void); /* == FSGS_ABI_VERSION of the header the library was built from */
 /* Lines of the packed gradient accumulator a caller that passes `replica_rows` > 0 must provide per Gaussian row:
@@ -1075,6 +1076,55 @@ int fsgs_step_forward(fsgs_step_plan *plan, fsgs_stream_t stream);
 int fsgs_step_backward(fsgs_step_plan *plan, int64_t spin_limit, int64_t *n_live_out, fsgs_stream_t stream);
 int fsgs_step_run(fsgs_step_plan *plan, int64_t spin_limit, int64_t *n_live_out, fsgs_stream_t stream);
 int64_t fsgs_step_plan_bytes(void); /* sizeof(fsgs_step_plan): a binding checks its own layout against it */
+
+/* ---- semantic head: one layer, forward and backward -----------------------------------------------------------------
+ * y = act(x W^T + b) + r.  x [rows, in] with rows `x_pitch` elements apart (0: one row for all), w [out, in] contiguous,
+ * bias [out] nullable, residual [rows, out] (pitch res_pitch) nullable, y [rows, out] contiguous.  All of one element type;
+ * products in that type on the matrix cores, sums fp32.  No pointer has to be aligned beyond its element. */
+#define FSGS_F32 0
+#define FSGS_BF16 1
+#define FSGS_F16 2
+#define FSGS_ACT_NONE 0
+#define FSGS_ACT_RELU 1
+#define FSGS_ACT_GELU 2 /* z/2 (1 + erf(z / sqrt 2)) */
+#define FSGS_ACT_SILU 3
+#define FSGS_LINEAR_MAX_DIM 65536
+int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype, const void *x, int64_t x_pitch, const void *w,
+                    const void *bias, int act, const void *residual, int64_t res_pitch, void *y, fsgs_stream_t stream);
+/* VJP.  dx [rows, in], dw [out, in], db [out]: contiguous, written, each nullable (rows == 0 writes nothing: dw and db are
+ * the caller's to clear).  The pre-activation is formed again from x, w and bias.  The residual's gradient is dy itself. */
+int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int act, int want_dx, int want_dw,
+                                      int want_db);
+int fsgs_linear_bwd(int64_t rows, int in_dim, int out_dim, int dtype, const void *x, int64_t x_pitch, const void *w,
+                    const void *bias, int act, const void *dy, int64_t dy_pitch, void *dx, void *dw, void *db, void *scratch,
+                    int64_t scratch_bytes, fsgs_stream_t stream);
+
+/* ---- distillation from a teacher's top-K scores ---------------------------------------------------------------------
+ * p = softmax over the row's K entries of teacher / T, q = softmax over all classes of logits / T,
+ * L = T^2 sum_k p_k (log p_k - log q[idx_k]).  logits [rows, classes], idx [rows, K] (int32 or int64), teacher [rows, K]
+ * (an element type of its own), weight [rows] nullable; rows `*_pitch` elements apart.  An entry whose class lies outside
+ * [0, classes) is no entry; a class may stand in several entries.  Rows without entries, rows whose entries are all -inf and
+ * rows of weight zero have loss and gradient zero and are not counted.
+ *   reduction NONE: loss [rows] = weight L;  SUM: loss [1] = sum weight L;  MEAN: that over the sum of the weights.
+ * stat [rows, 4] (16-byte aligned) and inv_weight [1] carry what the backward needs; both nullable when there is none.
+ * scratch: fsgs_distill_scratch_bytes(), not used by NONE. */
+#define FSGS_DISTILL_MAX_K 256
+#define FSGS_DISTILL_MIN_T 1e-6f /* temperature range: its square and its reciprocal stay normal numbers */
+#define FSGS_DISTILL_MAX_T 1e6f
+#define FSGS_REDUCE_NONE 0
+#define FSGS_REDUCE_SUM 1
+#define FSGS_REDUCE_MEAN 2
+int64_t fsgs_distill_scratch_bytes(void);
+int fsgs_distill_fwd(int64_t rows, int classes, int top_k, int dtype, const void *logits, int64_t pitch, int idx_bits,
+                     const void *idx, int64_t idx_pitch, int teacher_dtype, const void *teacher, int64_t teacher_pitch,
+                     const float *weight, float temperature, int reduction, float *loss, float *stat, float *inv_weight,
+                     void *scratch, int64_t scratch_bytes, fsgs_stream_t stream);
+/* grad_logits [rows, classes], contiguous, written.  grad_loss: [rows] when grad_per_row (reduction NONE), else [1];
+ * inv_weight: what the forward left there (nullable: 1). */
+int fsgs_distill_bwd(int64_t rows, int classes, int top_k, int dtype, const void *logits, int64_t pitch, int idx_bits,
+                     const void *idx, int64_t idx_pitch, int teacher_dtype, const void *teacher, int64_t teacher_pitch,
+                     const float *weight, float temperature, const float *stat, const float *inv_weight,
+                     const float *grad_loss, int grad_per_row, void *grad_logits, fsgs_stream_t stream);
 
 #ifdef __cplusplus
 }
