@@ -12,14 +12,15 @@ namespace fsgs {
 
 namespace {
 
-constexpr int kRowBlocks = 2048;  // workgroups of the row kernels: 8 per CU
+constexpr int kRowBlocks = 2048;   // workgroups of the row kernels: 8 per CU, the rows go round them
+constexpr int kWideRow = 256;      // lanes of a row that has a workgroup to itself
 
 struct DistillArgs {
     const void *s, *idx, *u;
     const float *weight;
     int64_t rows, sp, ip, up;
     int V, K, tdtype, idx64;
-    float T, invT;
+    float T, invT, scale2;  // scale2 = log2(e) / T
     float *row_loss;      // fwd, reduction none: [rows]
     float4 *stat;         // [rows] max s, 1 / sum_j exp, max u, 1 / sum_k exp (0: the row counts for nothing)
     double2 *partial;     // [kRowBlocks] sum of w L, sum of w
@@ -40,64 +41,132 @@ __device__ __forceinline__ int class_at(const void *idx, int64_t i, int idx64, i
     return c >= 0 && c < V ? (int)c : -1;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+// ---- reductions over the L lanes (neighbours, L a power of two) of a row ----
+struct MaxOp {
+    __device__ static float f(float a, float b) { return fmaxf(a, b); }
+};
+struct AddOp {
+    __device__ static float f(float a, float b) { return a + b; }
+};
+template <int L, class Op>
+__device__ __forceinline__ float row_reduce(float v) {
+    if constexpr (L >= 2) v = Op::f(v, dpp_f<0xB1>(v));    // quad_perm [1,0,3,2]
+    if constexpr (L >= 4) v = Op::f(v, dpp_f<0x4E>(v));    // quad_perm [2,3,0,1]
+    if constexpr (L >= 8) v = Op::f(v, dpp_f<0x141>(v));   // row_half_mirror
+    if constexpr (L >= 16) v = Op::f(v, dpp_f<0x140>(v));  // row_mirror
+    if constexpr (L >= 32) v = Op::f(v, __shfl_xor(v, 16));
+    if constexpr (L >= 64) v = Op::f(v, __shfl_xor(v, 32));
+    if constexpr (L == kWideRow) {
+        __shared__ float part[4];
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = Op::f(Op::f(part[0], part[1]), Op::f(part[2], part[3]));
+    }
     return v;
 }
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+template <int L>
+__device__ __forceinline__ bool row_any(bool b) {
+    if constexpr (L == kWideRow) return __syncthreads_or(b);
+    const uint64_t m = __ballot(b);
+    if constexpr (L == 64) return m != 0;
+    const int first = (threadIdx.x & 63) & ~(L - 1);
+    return (m >> first) & ((1ull << (L & 63)) - 1);
 }
 
-constexpr int kMaxPerLane = FSGS_DISTILL_MAX_K / kWave;
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// One wave per row.
+// exp of a score against the running maximum; a maximum of -inf (no finite score yet) must not turn -inf - -inf into NaN
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// One pass over a row, 16 bytes per lane and step: a lane keeps the maximum of its scores and the sum of their exponentials
+// against it, rescaled when a step brings a new maximum (one exponential per 4 or 8 scores); the lanes' pairs are joined at
+// the row's end.  kStep steps are loaded before the first is used.  The last step of a row that is no multiple of a step
+// re-reads the scores before it (masked) instead of reading element by element.
+constexpr int kStep = 4;
+
 template <typename T>
-__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double sum_l = 0.0, sum_w = 0.0;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows; row += (int64_t)gridDim.x * 4) {
-        const T *s = (const T *)a.s + row * a.sp;
-        float m = -INFINITY;
-        for (int j = lane; j < a.V; j += 64) m = fmaxf(m, (float)s[j]);
-        m = wave_max(m);
-        float sum = 0.f;
-        for (int j = lane; j < a.V; j += 64) sum += expf(((float)s[j] - m) * a.invT);
-        sum = wave_add(sum);
-        const float log_sum = logf(sum);
+__device__ __forceinline__ void unpack(const Chunk &c, float *v) {
+    T t[kChunk<T>];
+    __builtin_memcpy(t, &c, sizeof(Chunk));
+#pragma unroll
+    for (int e = 0; e < kChunk<T>; ++e) v[e] = (float)t[e];
+}
 
-        int cls[kMaxPerLane];
-        float u[kMaxPerLane];
+template <typename T, int L>
+__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
+    constexpr int CE = kChunk<T>, ROWS = 256 / L;
+    const int sub = threadIdx.x & (L - 1);
+    const int chunks = (a.V + CE - 1) / CE;
+    double sum_l = 0.0, sum_w = 0.0;
+    for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS) {
+        const int64_t slot = base + threadIdx.x / L;
+        const bool here = slot < a.rows;
+        const int64_t row = here ? slot : a.rows - 1;  // (lanes behind the last row repeat it and store nothing)
+        const T *s = (const T *)a.s + row * a.sp;
+        float m = -INFINITY, sum = 0.f;
+        for (int c0 = sub; c0 < chunks; c0 += L * kStep) {
+            Chunk c[kStep];
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                const int j = (c0 + i * L) * CE;
+                if (a.V < CE) c[i] = load_chunk_n(s, j < a.V ? a.V : 0);
+                else c[i] = load_chunk(s + min(j, a.V - CE));
+            }
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                const int j = (c0 + i * L) * CE;
+                if (j >= a.V) break;
+                float v[CE];
+                unpack<T>(c[i], v);
+                if (j + CE > a.V) {
+                    // elements of this step start at V - CE (or hold zeros behind V): those before j are counted already
+                    const int from = a.V < CE ? 0 : j - (a.V - CE), to = a.V < CE ? a.V : CE;
+#pragma unroll
+                    for (int e = 0; e < CE; ++e) v[e] = e >= from && e < to ? v[e] : -INFINITY;
+                }
+                float mc = v[0];
+#pragma unroll
+                for (int e = 1; e < CE; ++e) mc = fmaxf(mc, v[e]);
+                const float mn = fmaxf(m, mc), mf = finite_max(mn);
+                sum *= exp2_hw((m - mf) * a.scale2);
+                m = mn;
+#pragma unroll
+                for (int e = 0; e < CE; ++e) sum += exp2_hw((v[e] - mf) * a.scale2);
+            }
+        }
+        const float lane_m = m;
+        m = row_reduce<L, MaxOp>(m);
+        sum = row_reduce<L, AddOp>(sum * exp2_hw((lane_m - finite_max(m)) * a.scale2));
+        // (a row of -inf only: sum 0, and the -inf - -inf below are the NaN that its softmax is)
+
         float um = -INFINITY;
         bool any = false;
-#pragma unroll
-        for (int i = 0; i < kMaxPerLane; ++i) {
-            const int k = i * 64 + lane;
-            cls[i] = k < a.K ? class_at(a.idx, row * a.ip + k, a.idx64, a.V) : -1;
-            u[i] = cls[i] >= 0 ? teacher_at(a.u, row * a.up + k, a.tdtype) : -INFINITY;
-            um = fmaxf(um, u[i]);
-            any |= u[i] != -INFINITY;  // (NaN counts: it reaches the loss)
-        }
-        um = wave_max(um);
-        const float w = a.weight ? a.weight[row] : 1.f;
-        const bool alive = __any(any) && w != 0.f;
-        float z = 0.f, loss = 0.f;
-#pragma unroll
-        for (int i = 0; i < kMaxPerLane; ++i)
-            if (cls[i] >= 0) z += expf((u[i] - um) * a.invT);
-        z = wave_add(z);
-        const float inv_z = 1.f / z, log_z = logf(z);
-#pragma unroll
-        for (int i = 0; i < kMaxPerLane; ++i)
-            if (cls[i] >= 0) {
-                const float lu = (u[i] - um) * a.invT, p = expf(lu) * inv_z;
-                const float lq = ((float)s[cls[i]] - m) * a.invT - log_sum;
-                if (p != 0.f) loss += p * (lu - log_z - lq);
+        for (int k = sub; k < a.K; k += L)
+            if (class_at(a.idx, row * a.ip + k, a.idx64, a.V) >= 0) {
+                const float u = teacher_at(a.u, row * a.up + k, a.tdtype);
+                um = fmaxf(um, u);
+                any |= u != -INFINITY;  // (NaN counts: it reaches the loss)
             }
-        loss = wave_add(loss) * a.T * a.T;
-        if (lane == 0) {
+        um = row_reduce<L, MaxOp>(um);
+        const float w = a.weight ? a.weight[row] : 1.f;
+        const bool alive = row_any<L>(any) && w != 0.f;
+        // sum_k p_k (log p_k - log q_k) = (sum_k e_k x_k) / Z - log Z + log S with e_k = exp((u_k - um) / T), Z their sum,
+        // x_k = (u_k - um) / T - (s_k - m) / T
+        float z = 0.f, ex = 0.f;
+        for (int k = sub; k < a.K; k += L) {
+            const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+            if (cls >= 0) {
+                const float lu = teacher_at(a.u, row * a.up + k, a.tdtype) - um, e = exp2_hw(lu * a.scale2);
+                z += e;
+                if (e != 0.f) ex += e * ((lu - ((float)s[cls] - m)) * a.invT);
+            }
+        }
+        z = row_reduce<L, AddOp>(z);
+        ex = row_reduce<L, AddOp>(ex);
+        if (sub == 0 && here) {
+            const float inv_z = 1.f / z;
+            const float loss = (ex * inv_z + (logf(sum) - logf(z))) * (a.T * a.T);
             const float wl = alive ? w * loss : 0.f;
             if (a.row_loss) a.row_loss[row] = wl;
             if (a.stat) a.stat[row] = make_float4(m, 1.f / sum, um, alive ? inv_z : 0.f);
@@ -105,14 +174,17 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
         }
     }
     if (a.partial) {
-        __shared__ double2 part[4];
-        if (lane == 0) part[wave] = make_double2(sum_l, sum_w);
+        __shared__ double2 part[256];
+        part[threadIdx.x] = make_double2(sum_l, sum_w);
         __syncthreads();
-        if (threadIdx.x == 0) {
-            double2 t = part[0];
-            for (int i = 1; i < 4; ++i) t.x += part[i].x, t.y += part[i].y;
-            a.partial[blockIdx.x] = t;
+        for (int o = 128; o; o >>= 1) {
+            if ((int)threadIdx.x < o) {
+                part[threadIdx.x].x += part[threadIdx.x + o].x;
+                part[threadIdx.x].y += part[threadIdx.x + o].y;
+            }
+            __syncthreads();
         }
+        if (threadIdx.x == 0) a.partial[blockIdx.x] = part[0];
     }
 }
 
@@ -139,57 +211,138 @@ __global__ __launch_bounds__(256) void distill_reduce_kernel(const double2 *__re
     }
 }
 
-// One wave per row: q for every class, then the teacher's classes once more with their mass taken off.
-template <typename T>
+// q for every class, then the teacher's classes once more with their mass taken off.  A class may stand in several entries:
+// its first entry carries their sum, taken in the entries' order.  Whether a row has such a class at all is found with one bit
+// per class in LDS; only then are its entries compared pair by pair.
+template <typename T, int L>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows; row += (int64_t)gridDim.x * 4) {
+    constexpr int CE = kChunk<T>, ROWS = 256 / L;
+    extern __shared__ uint32_t seen[];  // [ROWS][words]
+    const int sub = threadIdx.x & (L - 1), group = threadIdx.x / L;
+    const int chunks = (a.V + CE - 1) / CE, words = (a.V + 31) / 32;
+    uint32_t *bits = seen + group * words;
+    const float up = a.g_per_row ? 0.f : a.g[0];
+    const float inv_w = a.inv_w ? *a.inv_w : 1.f;
+    for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS) {
+        const int64_t slot = base + group;
+        const bool here = slot < a.rows;
+        const int64_t row = here ? slot : a.rows - 1;
         const T *s = (const T *)a.s + row * a.sp;
         T *ds = (T *)a.ds + row * a.V;
         const float4 st = a.stat[row];
-        if (st.w == 0.f) {
-            for (int j = lane; j < a.V; j += 64) ds[j] = (T)0.f;
-            continue;
+        const float m = st.x, um = st.z;
+        const bool dead = st.w == 0.f;
+        const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * (a.g_per_row ? a.g[row] : up) * inv_w;
+        const float cq = coef * st.y;
+        for (int k = sub; k < a.K; k += L) {
+            const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+            if (cls >= 0) bits[cls >> 5] = 0;
         }
-        const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * a.g[a.g_per_row ? row : 0] * (a.inv_w ? *a.inv_w : 1.f);
-        for (int j = lane; j < a.V; j += 64) ds[j] = (T)(coef * (expf(((float)s[j] - st.x) * a.invT) * st.y));
-        // the same class may stand in several entries: its first entry carries the sum
-        int cls[kMaxPerLane];
-        float p[kMaxPerLane];
+        for (int c0 = sub; c0 < chunks; c0 += L * kStep) {
+            Chunk c[kStep];
 #pragma unroll
-        for (int i = 0; i < kMaxPerLane; ++i) {
-            const int k = i * 64 + lane;
-            cls[i] = k < a.K ? class_at(a.idx, row * a.ip + k, a.idx64, a.V) : -1;
-            p[i] = cls[i] >= 0 ? expf((teacher_at(a.u, row * a.up + k, a.tdtype) - st.z) * a.invT) * st.w : 0.f;
+            for (int i = 0; i < kStep; ++i) {
+                const int j = (c0 + i * L) * CE;
+                if (a.V < CE) c[i] = load_chunk_n(s, j < a.V ? a.V : 0);
+                else c[i] = load_chunk(s + min(j, a.V - CE));
+            }
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                const int j = (c0 + i * L) * CE;
+                if (j >= a.V || !here) break;
+                float v[CE];
+                unpack<T>(c[i], v);
+                T out[CE];
+#pragma unroll
+                for (int e = 0; e < CE; ++e) out[e] = (T)(dead ? 0.f : cq * exp2_hw((v[e] - m) * a.scale2));
+                if (a.V < CE) {
+#pragma unroll
+                    for (int e = 0; e < CE; ++e)
+                        if (e < a.V) ds[e] = out[e];
+                } else {
+                    // (the last step of a row stores the elements before it a second time, with the same values)
+                    __builtin_memcpy(ds + min(j, a.V - CE), out, sizeof(Chunk));
+                }
+            }
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-        __builtin_amdgcn_s_waitcnt(0);  // the q stores have landed before any lane writes over them
-#pragma unroll
-        for (int i = 0; i < kMaxPerLane; ++i) {
-            float mass = 0.f;
-            bool first = cls[i] >= 0;
-#pragma unroll
-            for (int t = 0; t < kMaxPerLane; ++t)
-                if (t * 64 < a.K)
-                    for (int l = 0; l < 64; ++l) {
-                        const int oc = __shfl(cls[t], l);
-                        const float op = __shfl(p[t], l);
-                        const bool same = oc == cls[i];
-                        if (same) mass += op;
-                        if (same && t * 64 + l < i * 64 + lane) first = false;
-                    }
-            if (first) ds[cls[i]] = (T)(coef * (expf(((float)s[cls[i]] - st.x) * a.invT) * st.y - mass));
+        if constexpr (L == kWideRow) __syncthreads();
+        bool again = false;
+        for (int k = sub; k < a.K; k += L) {
+            const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+            if (cls >= 0) again |= (atomicOr(&bits[cls >> 5], 1u << (cls & 31)) >> (cls & 31)) & 1u;
         }
+        again = row_any<L>(again);
+        // every store above has landed before a lane writes over one of them
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (L == kWideRow) __syncthreads();
+        if (here && !dead)
+            for (int k = sub; k < a.K; k += L) {
+                const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+                if (cls < 0) continue;
+                float mass = exp2_hw((teacher_at(a.u, row * a.up + k, a.tdtype) - um) * a.scale2);
+                bool first = true;
+                if (again) {
+                    mass = 0.f;
+                    for (int t = 0; t < a.K; ++t)
+                        if (class_at(a.idx, row * a.ip + t, a.idx64, a.V) == cls) {
+                            mass += exp2_hw((teacher_at(a.u, row * a.up + t, a.tdtype) - um) * a.scale2);
+                            first &= t >= k;
+                        }
+                }
+                if (first) ds[cls] = (T)(coef * (exp2_hw(((float)s[cls] - m) * a.scale2) * st.y - mass * st.w));
+            }
+        if constexpr (L == kWideRow) __syncthreads();
     }
 }
 
-int row_blocks(int64_t rows) {
-    const int64_t b = (rows + 3) / 4;
+// Lanes per row: the fewest that leave a lane at most five steps of 16 bytes (the waves then hold many rows at once and the
+// joins over lanes stay short); rows of more than 64 lanes' worth of 16 steps get a workgroup each.
+int lanes_per_row(int V, int dtype) {
+    const int ce = dtype == FSGS_F32 ? 4 : 8, chunks = (V + ce - 1) / ce;
+    if (chunks > 64 * 16) return kWideRow;
+    int l = 1;
+    while (l < 64 && chunks > 5 * l) l *= 2;
+    return l;
+}
+
+int row_blocks(int64_t rows, int lanes) {
+    const int64_t per = 256 / lanes, b = (rows + per - 1) / per;
     return (int)(b < kRowBlocks ? b : kRowBlocks);
 }
 
+template <typename T, int L>
+void launch_rows(const DistillArgs &a, bool bwd, hipStream_t st) {
+    const int blocks = row_blocks(a.rows, L);
+    if (bwd) distill_bwd_kernel<T, L><<<blocks, 256, (256 / L) * (size_t)((a.V + 31) / 32) * 4, st>>>(a);
+    else distill_fwd_kernel<T, L><<<blocks, 256, 0, st>>>(a);
+}
+
+template <typename T>
+void launch_lanes(const DistillArgs &a, int lanes, bool bwd, hipStream_t st) {
+    switch (lanes) {
+        case 1: return launch_rows<T, 1>(a, bwd, st);
+        case 2: return launch_rows<T, 2>(a, bwd, st);
+        case 4: return launch_rows<T, 4>(a, bwd, st);
+        case 8: return launch_rows<T, 8>(a, bwd, st);
+        case 16: return launch_rows<T, 16>(a, bwd, st);
+        case 32: return launch_rows<T, 32>(a, bwd, st);
+        case 64: return launch_rows<T, 64>(a, bwd, st);
+        default: return launch_rows<T, kWideRow>(a, bwd, st);
+    }
+}
+
+int launch(const DistillArgs &a, int dtype, bool bwd, hipStream_t st) {
+    const int lanes = lanes_per_row(a.V, dtype);
+    switch (dtype) {
+        case FSGS_F32: launch_lanes<float>(a, lanes, bwd, st); break;
+        case FSGS_BF16: launch_lanes<__bf16>(a, lanes, bwd, st); break;
+        default: launch_lanes<_Float16>(a, lanes, bwd, st); break;
+    }
+    return check_launch();
+}
+
 bool bad_args(int64_t rows, int V, int K, int dtype, int tdtype, int idx_bits, float T) {
-    return rows < 0 || rows > INT32_MAX || V < 1 || K < 1 || K > FSGS_DISTILL_MAX_K || !known_dtype(dtype) || !known_dtype(tdtype) ||
+    return rows < 0 || rows > INT32_MAX || V < 1 || V > FSGS_DISTILL_MAX_CLASSES || K < 1 || K > FSGS_DISTILL_MAX_K || !known_dtype(dtype) || !known_dtype(tdtype) ||
            (idx_bits != 32 && idx_bits != 64) || !(T >= FSGS_DISTILL_MIN_T) || !(T <= FSGS_DISTILL_MAX_T);
 }
 
@@ -213,23 +366,17 @@ extern "C" int fsgs_distill_fwd(int64_t rows, int classes, int top_k, int dtype,
     DistillArgs a = {};
     a.s = logits, a.sp = pitch, a.idx = idx, a.ip = idx_pitch, a.u = teacher, a.up = teacher_pitch, a.weight = weight;
     a.rows = rows, a.V = classes, a.K = top_k, a.tdtype = teacher_dtype, a.idx64 = idx_bits == 64;
-    a.T = temperature, a.invT = 1.f / temperature;
+    a.T = temperature, a.invT = 1.f / temperature, a.scale2 = (float)(1.4426950408889634 / (double)temperature);
     a.stat = (float4 *)stat;
     if (reduction == FSGS_REDUCE_NONE) a.row_loss = loss;
     else a.partial = (double2 *)scratch;
-    const int blocks = row_blocks(rows);
     hipStream_t st = as_stream(stream);
     if (rows > 0) {
-        switch (dtype) {
-            case FSGS_F32: distill_fwd_kernel<float><<<blocks, 256, 0, st>>>(a); break;
-            case FSGS_BF16: distill_fwd_kernel<__bf16><<<blocks, 256, 0, st>>>(a); break;
-            default: distill_fwd_kernel<_Float16><<<blocks, 256, 0, st>>>(a); break;
-        }
-        const int rc = check_launch();
+        const int rc = launch(a, dtype, false, st);
         if (rc != FSGS_OK) return rc;
     }
     if (reduction == FSGS_REDUCE_NONE) return FSGS_OK;
-    distill_reduce_kernel<<<1, 256, 0, st>>>((const double2 *)scratch, rows > 0 ? blocks : 0, reduction == FSGS_REDUCE_MEAN,
+    distill_reduce_kernel<<<1, 256, 0, st>>>((const double2 *)scratch, rows > 0 ? row_blocks(rows, lanes_per_row(classes, dtype)) : 0, reduction == FSGS_REDUCE_MEAN,
                                              loss, inv_weight);
     return check_launch();
 }
@@ -246,15 +393,8 @@ extern "C" int fsgs_distill_bwd(int64_t rows, int classes, int top_k, int dtype,
     DistillArgs a = {};
     a.s = logits, a.sp = pitch, a.idx = idx, a.ip = idx_pitch, a.u = teacher, a.up = teacher_pitch, a.weight = weight;
     a.rows = rows, a.V = classes, a.K = top_k, a.tdtype = teacher_dtype, a.idx64 = idx_bits == 64;
-    a.T = temperature, a.invT = 1.f / temperature;
+    a.T = temperature, a.invT = 1.f / temperature, a.scale2 = (float)(1.4426950408889634 / (double)temperature);
     a.stat = (float4 *)const_cast<float *>(stat);
     a.g = grad_loss, a.g_per_row = grad_per_row, a.inv_w = inv_weight, a.ds = grad_logits;
-    hipStream_t st = as_stream(stream);
-    const int blocks = row_blocks(rows);
-    switch (dtype) {
-        case FSGS_F32: distill_bwd_kernel<float><<<blocks, 256, 0, st>>>(a); break;
-        case FSGS_BF16: distill_bwd_kernel<__bf16><<<blocks, 256, 0, st>>>(a); break;
-        default: distill_bwd_kernel<_Float16><<<blocks, 256, 0, st>>>(a); break;
-    }
-    return check_launch();
+    return launch(a, dtype, true, as_stream(stream));
 }

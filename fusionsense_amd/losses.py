@@ -159,7 +159,7 @@ def topk_distill_loss(logits: Tensor, teacher_idx: Tensor, teacher_logits: Tenso
 
     ``logits`` [..., V] (float32, bfloat16 or float16) are the student's scores, e.g. a rendered plane behind a
     :class:`fusionsense_amd.semantics.SemanticHead`; ``teacher_idx`` [..., K] (int32 / int64) and ``teacher_logits`` [..., K]
-    (any of the three types) the classes and scores that were kept of the teacher, K <= 256.  With p the softmax of
+    (any of the three types) the classes and scores that were kept of the teacher, K <= 256 (and V <= 524288).  With p the softmax of
     ``teacher_logits / temperature`` over a row's entries and q that of ``logits / temperature`` over all V classes, a row's
     loss is ``temperature**2 * sum_k p_k (log p_k - log q[idx_k])``.
 

@@ -1798,6 +1798,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 LINEAR_MAX_DIM = 65536
 DISTILL_MAX_K = 256
+DISTILL_MAX_CLASSES = 524288
 DISTILL_T_RANGE = (1e-6, 1e6)
 
 
@@ -1964,8 +1965,8 @@ def topk_distill(logits: Tensor, teacher_idx: Tensor, teacher_logits: Tensor, te
     _require_float(teacher_logits, "teacher_logits")
     if not isinstance(teacher_idx, torch.Tensor) or teacher_idx.dtype not in (torch.int32, torch.int64):
         raise ValueError("teacher_idx must be an int32 or int64 tensor")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be [...,V] with V >= 1, got {tuple(logits.shape)}")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= DISTILL_MAX_CLASSES:
+        raise ValueError(f"logits must be [...,V] with V in [1,{DISTILL_MAX_CLASSES}], got {tuple(logits.shape)}")
     lead = logits.shape[:-1]
     if teacher_idx.dim() != logits.dim() or teacher_idx.shape[:-1] != lead or not 1 <= teacher_idx.shape[-1] <= DISTILL_MAX_K:
         raise ValueError(f"teacher_idx must be {tuple(lead)} + [K] with K in [1,{DISTILL_MAX_K}], got {tuple(teacher_idx.shape)}")

@@ -1109,6 +1109,7 @@ int fsgs_linear_bwd(int64_t rows, int in_dim, int out_dim, int dtype, const void
  * stat [rows, 4] (16-byte aligned) and inv_weight [1] carry what the backward needs; both nullable when there is none.
  * scratch: fsgs_distill_scratch_bytes(), not used by NONE. */
 #define FSGS_DISTILL_MAX_K 256
+#define FSGS_DISTILL_MAX_CLASSES 524288 /* one bit per class in LDS */
 #define FSGS_DISTILL_MIN_T 1e-6f /* temperature range: its square and its reciprocal stay normal numbers */
 #define FSGS_DISTILL_MAX_T 1e6f
 #define FSGS_REDUCE_NONE 0

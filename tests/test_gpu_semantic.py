@@ -238,7 +238,7 @@ def _check_distill(logits, idx, top, T=1.0, weight=None, reduction="mean", seed=
 
 
 DSIZES = [(1, 1, 1), (1, 150, 8), (3, 2, 2), (5, 21, 4), (70, 64, 64), (257, 65, 7), (100, 150, 16), (33, 1203, 32), (9, 700, 100),
-          (4, 2049, 256), (3, 9000, 64), (3, 32003, 64), (2, 40001, 5), (2, 33, 256), (5000, 17, 3), (20011, 5, 2)]
+          (4, 2049, 256), (3, 9000, 64), (3, 32003, 64), (2, 40001, 5), (2, 524288, 3), (3, 8193, 9), (3, 4095, 9), (2, 33, 256), (5000, 17, 3), (20011, 5, 2)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)

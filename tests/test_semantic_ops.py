@@ -16,6 +16,7 @@ def test_limits_match_the_header():
     val = lambda n: re.search(rf"#define {n} (\S+)", h).group(1)
     assert int(val("FSGS_LINEAR_MAX_DIM")) == ops.LINEAR_MAX_DIM
     assert int(val("FSGS_DISTILL_MAX_K")) == ops.DISTILL_MAX_K
+    assert int(val("FSGS_DISTILL_MAX_CLASSES")) == ops.DISTILL_MAX_CLASSES
     assert (float(val("FSGS_DISTILL_MIN_T").rstrip("f")), float(val("FSGS_DISTILL_MAX_T").rstrip("f"))) == ops.DISTILL_T_RANGE
     for name, code in ops.ACTIVATIONS.items():
         assert int(val(f"FSGS_ACT_{name.upper()}")) == code
@@ -77,7 +78,7 @@ def _dfwd(rows=4, v=8, k=2, dt=0, s=ONE, sp=8, bits=64, idx=ONE, tdt=0, u=ONE, T
                                         nbytes, None)
 
 
-@pytest.mark.parametrize("kw", [dict(rows=-1), dict(v=0), dict(k=0), dict(k=257), dict(dt=3), dict(tdt=3), dict(bits=16),
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(v=0), dict(v=524289), dict(k=0), dict(k=257), dict(dt=3), dict(tdt=3), dict(bits=16),
                                 dict(T=0.0), dict(T=-1.0), dict(T=float("nan")), dict(T=float("inf")), dict(T=1e-7), dict(T=2e6),
                                 dict(red=3), dict(red=-1), dict(s=None), dict(idx=None), dict(u=None), dict(loss=None),
                                 dict(sp=-1)])
