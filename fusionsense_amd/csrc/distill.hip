@@ -76,14 +76,8 @@ __device__ __forceinline__ bool row_any(bool b) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// exp of a score against the running maximum; a maximum of -inf (no finite score yet) must not turn -inf - -inf into NaN
+// exp of a score against a maximum of -inf (no finite score) must not turn -inf - -inf into NaN
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
-
-// One pass over a row, 16 bytes per lane and step: a lane keeps the maximum of its scores and the sum of their exponentials
-// against it, rescaled when a step brings a new maximum (one exponential per 4 or 8 scores); the lanes' pairs are joined at
-// the row's end.  kStep steps are loaded before the first is used.  The last step of a row that is no multiple of a step
-// re-reads the scores before it (masked) instead of reading element by element.
-constexpr int kStep = 4;
 
 template <typename T>
 __device__ __forceinline__ void unpack(const Chunk &c, float *v) {
@@ -91,6 +85,41 @@ __device__ __forceinline__ void unpack(const Chunk &c, float *v) {
     __builtin_memcpy(t, &c, sizeof(Chunk));
 #pragma unroll
     for (int e = 0; e < kChunk<T>; ++e) v[e] = (float)t[e];
+}
+
+// A row is read in chunks of 16 bytes, chunk c by lane c mod L, kStep chunks per lane at a time (all of a row that has at most
+// kStep * L chunks: lanes_per_row).  Rows start at any element.  The last chunk of a row that does not end on one is read
+// shifted back to end with the row, its doubled elements masked: no element-wise reads, nothing behind the row.
+constexpr int kStep = 5;
+constexpr int kHeld = 4;  // entries per lane kept in registers; further ones are read again where they are needed
+
+template <typename T, int L>
+__device__ __forceinline__ void load_step(Chunk (&c)[kStep], const T *s, int c0, int V) {
+    constexpr int CE = kChunk<T>;
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+        const int j = (c0 + i * L) * CE;
+        if (V < CE) c[i] = load_chunk_n(s, j < V ? V : 0);
+        else c[i] = load_chunk(s + min(j, V - CE));
+    }
+}
+
+// -inf in place of what other chunks count, or of what lies behind the row, in the chunk at element j.
+template <typename T>
+__device__ __forceinline__ void mask_chunk(Chunk &c, int j, int V) {
+    constexpr int CE = kChunk<T>;
+    if (j + CE <= V) return;
+    const int from = V < CE ? 0 : j - (V - CE), to = j >= V ? 0 : (V < CE ? V : CE);
+    T t[CE];
+    __builtin_memcpy(t, &c, sizeof(Chunk));
+#pragma unroll
+    for (int e = 0; e < CE; ++e) t[e] = e >= from && e < to ? t[e] : (T)-INFINITY;
+    __builtin_memcpy(&c, t, sizeof(Chunk));
+}
+
+// The compiler must not keep a chunk's floats from one pass over it to the next (8 registers against 4).
+__device__ __forceinline__ void forget(Chunk &c) {
+    asm volatile("" : "+v"(c.u[0]), "+v"(c.u[1]), "+v"(c.u[2]), "+v"(c.u[3]));
 }
 
 template <typename T, int L>
@@ -104,36 +133,53 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
         const bool here = slot < a.rows;
         const int64_t row = here ? slot : a.rows - 1;  // (lanes behind the last row repeat it and store nothing)
         const T *s = (const T *)a.s + row * a.sp;
-        float m = -INFINITY, sum = 0.f;
-        for (int c0 = sub; c0 < chunks; c0 += L * kStep) {
-            Chunk c[kStep];
+        Chunk c[kStep];
+        load_step<T, L>(c, s, sub, a.V);
+        int cls[kHeld];
+        float u[kHeld], sv[kHeld];
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                const int j = (c0 + i * L) * CE;
-                if (a.V < CE) c[i] = load_chunk_n(s, j < a.V ? a.V : 0);
-                else c[i] = load_chunk(s + min(j, a.V - CE));
+        for (int i = 0; i < kHeld; ++i) {
+            const int k = i * L + sub;
+            cls[i] = -1;
+            if (i * L < a.K && k < a.K) cls[i] = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            u[i] = sv[i] = -INFINITY;
+            if (i * L < a.K && cls[i] >= 0) {
+                u[i] = teacher_at(a.u, row * a.up + i * L + sub, a.tdtype);
+                sv[i] = (float)s[cls[i]];
             }
+        }
+        const float w = a.weight ? a.weight[row] : 1.f;
+
+        // maximum and sum of the row: held whole, or step by step with the sum rescaled to each step's maximum
+        float m = -INFINITY, sum = 0.f;
+        for (int c0 = sub;;) {
+            float mn = m;
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
-                const int j = (c0 + i * L) * CE;
-                if (j >= a.V) break;
                 float v[CE];
+                mask_chunk<T>(c[i], (c0 + i * L) * CE, a.V);
                 unpack<T>(c[i], v);
-                if (j + CE > a.V) {
-                    // elements of this step start at V - CE (or hold zeros behind V): those before j are counted already
-                    const int from = a.V < CE ? 0 : j - (a.V - CE), to = a.V < CE ? a.V : CE;
 #pragma unroll
-                    for (int e = 0; e < CE; ++e) v[e] = e >= from && e < to ? v[e] : -INFINITY;
-                }
-                float mc = v[0];
+                for (int e = 0; e < CE; ++e) mn = fmaxf(mn, v[e]);
+            }
+            const float mf = finite_max(mn);
+            sum *= exp2_hw((m - mf) * a.scale2);
+            m = mn;
 #pragma unroll
-                for (int e = 1; e < CE; ++e) mc = fmaxf(mc, v[e]);
-                const float mn = fmaxf(m, mc), mf = finite_max(mn);
-                sum *= exp2_hw((m - mf) * a.scale2);
-                m = mn;
+            for (int i = 0; i < kStep; ++i) {
+                float v[CE];
+                if constexpr (sizeof(T) == 2) forget(c[i]);
+                unpack<T>(c[i], v);
 #pragma unroll
                 for (int e = 0; e < CE; ++e) sum += exp2_hw((v[e] - mf) * a.scale2);
             }
+            if constexpr (L != kWideRow) break;
+            c0 += kStep * L;
+            if (c0 - sub >= chunks) break;
+            load_step<T, L>(c, s, c0, a.V);
         }
         const float lane_m = m;
         m = row_reduce<L, MaxOp>(m);
@@ -142,25 +188,33 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
 
         float um = -INFINITY;
         bool any = false;
-        for (int k = sub; k < a.K; k += L)
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            um = fmaxf(um, u[i]);
+            any |= u[i] != -INFINITY;  // (NaN counts: it reaches the loss)
+        }
+        for (int k = kHeld * L + sub; k < a.K; k += L)
             if (class_at(a.idx, row * a.ip + k, a.idx64, a.V) >= 0) {
-                const float u = teacher_at(a.u, row * a.up + k, a.tdtype);
-                um = fmaxf(um, u);
-                any |= u != -INFINITY;  // (NaN counts: it reaches the loss)
+                const float uk = teacher_at(a.u, row * a.up + k, a.tdtype);
+                um = fmaxf(um, uk);
+                any |= uk != -INFINITY;
             }
         um = row_reduce<L, MaxOp>(um);
-        const float w = a.weight ? a.weight[row] : 1.f;
         const bool alive = row_any<L>(any) && w != 0.f;
         // sum_k p_k (log p_k - log q_k) = (sum_k e_k x_k) / Z - log Z + log S with e_k = exp((u_k - um) / T), Z their sum,
         // x_k = (u_k - um) / T - (s_k - m) / T
         float z = 0.f, ex = 0.f;
-        for (int k = sub; k < a.K; k += L) {
-            const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
-            if (cls >= 0) {
-                const float lu = teacher_at(a.u, row * a.up + k, a.tdtype) - um, e = exp2_hw(lu * a.scale2);
-                z += e;
-                if (e != 0.f) ex += e * ((lu - ((float)s[cls] - m)) * a.invT);
-            }
+        auto entry = [&](float uk, float sk) {
+            const float lu = uk - um, e = exp2_hw(lu * a.scale2);
+            z += e;
+            if (e != 0.f) ex += e * ((lu - (sk - m)) * a.invT);
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (i * L < a.K && cls[i] >= 0) entry(u[i], sv[i]);
+        for (int k = kHeld * L + sub; k < a.K; k += L) {
+            const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+            if (ck >= 0) entry(teacher_at(a.u, row * a.up + k, a.tdtype), (float)s[ck]);
         }
         z = row_reduce<L, AddOp>(z);
         ex = row_reduce<L, AddOp>(ex);
@@ -229,23 +283,35 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a) {
         const int64_t row = here ? slot : a.rows - 1;
         const T *s = (const T *)a.s + row * a.sp;
         T *ds = (T *)a.ds + row * a.V;
+        Chunk c[kStep];
+        load_step<T, L>(c, s, sub, a.V);
         const float4 st = a.stat[row];
         const float m = st.x, um = st.z;
         const bool dead = st.w == 0.f;
+        int cls[kHeld];
+        float u[kHeld], sv[kHeld];
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int k = i * L + sub;
+            cls[i] = -1;
+            if (i * L < a.K && k < a.K) cls[i] = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            u[i] = sv[i] = 0.f;
+            if (i * L < a.K && cls[i] >= 0) {
+                u[i] = teacher_at(a.u, row * a.up + i * L + sub, a.tdtype);
+                sv[i] = (float)s[cls[i]];
+                bits[cls[i] >> 5] = 0;
+            }
+        }
+        for (int k = kHeld * L + sub; k < a.K; k += L) {
+            const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+            if (ck >= 0) bits[ck >> 5] = 0;
+        }
         const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * (a.g_per_row ? a.g[row] : up) * inv_w;
         const float cq = coef * st.y;
-        for (int k = sub; k < a.K; k += L) {
-            const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
-            if (cls >= 0) bits[cls >> 5] = 0;
-        }
-        for (int c0 = sub; c0 < chunks; c0 += L * kStep) {
-            Chunk c[kStep];
-#pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                const int j = (c0 + i * L) * CE;
-                if (a.V < CE) c[i] = load_chunk_n(s, j < a.V ? a.V : 0);
-                else c[i] = load_chunk(s + min(j, a.V - CE));
-            }
+        for (int c0 = sub;;) {
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
                 const int j = (c0 + i * L) * CE;
@@ -260,49 +326,63 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a) {
                     for (int e = 0; e < CE; ++e)
                         if (e < a.V) ds[e] = out[e];
                 } else {
-                    // (the last step of a row stores the elements before it a second time, with the same values)
+                    // (the last chunk of a row stores the elements before it a second time, with the same values)
                     __builtin_memcpy(ds + min(j, a.V - CE), out, sizeof(Chunk));
                 }
             }
+            if constexpr (L != kWideRow) break;
+            c0 += kStep * L;
+            if (c0 - sub >= chunks) break;
+            load_step<T, L>(c, s, c0, a.V);
         }
         if constexpr (L == kWideRow) __syncthreads();
         bool again = false;
-        for (int k = sub; k < a.K; k += L) {
-            const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
-            if (cls >= 0) again |= (atomicOr(&bits[cls >> 5], 1u << (cls & 31)) >> (cls & 31)) & 1u;
+        auto mark = [&](int ck) { again |= (atomicOr(&bits[ck >> 5], 1u << (ck & 31)) >> (ck & 31)) & 1u; };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (i * L < a.K && cls[i] >= 0) mark(cls[i]);
+        for (int k = kHeld * L + sub; k < a.K; k += L) {
+            const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+            if (ck >= 0) mark(ck);
         }
         again = row_any<L>(again);
         // every store above has landed before a lane writes over one of them
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if constexpr (L == kWideRow) __syncthreads();
-        if (here && !dead)
-            for (int k = sub; k < a.K; k += L) {
-                const int cls = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
-                if (cls < 0) continue;
-                float mass = exp2_hw((teacher_at(a.u, row * a.up + k, a.tdtype) - um) * a.scale2);
+        auto fix = [&](int k, int ck, float uk, float sk) {
+            float mass = exp2_hw((uk - um) * a.scale2);
+            if (again) {
+                mass = 0.f;
                 bool first = true;
-                if (again) {
-                    mass = 0.f;
-                    for (int t = 0; t < a.K; ++t)
-                        if (class_at(a.idx, row * a.ip + t, a.idx64, a.V) == cls) {
-                            mass += exp2_hw((teacher_at(a.u, row * a.up + t, a.tdtype) - um) * a.scale2);
-                            first &= t >= k;
-                        }
-                }
-                if (first) ds[cls] = (T)(coef * (exp2_hw(((float)s[cls] - m) * a.scale2) * st.y - mass * st.w));
+                for (int t = 0; t < a.K; ++t)
+                    if (class_at(a.idx, row * a.ip + t, a.idx64, a.V) == ck) {
+                        mass += exp2_hw((teacher_at(a.u, row * a.up + t, a.tdtype) - um) * a.scale2);
+                        first &= t >= k;
+                    }
+                if (!first) return;
             }
+            ds[ck] = (T)(coef * (exp2_hw((sk - m) * a.scale2) * st.y - mass * st.w));
+        };
+        if (here && !dead) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (i * L < a.K && cls[i] >= 0) fix(i * L + sub, cls[i], u[i], sv[i]);
+            for (int k = kHeld * L + sub; k < a.K; k += L) {
+                const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+                if (ck >= 0) fix(k, ck, teacher_at(a.u, row * a.up + k, a.tdtype), (float)s[ck]);
+            }
+        }
         if constexpr (L == kWideRow) __syncthreads();
     }
 }
 
-// Lanes per row: the fewest that leave a lane at most five steps of 16 bytes (the waves then hold many rows at once and the
-// joins over lanes stay short); rows of more than 64 lanes' worth of 16 steps get a workgroup each.
+// Lanes per row: the fewest that hold the row in kStep chunks each (a wave then has many rows in flight and the joins over
+// lanes stay short); a row that 64 lanes cannot hold gets a workgroup.
 int lanes_per_row(int V, int dtype) {
     const int ce = dtype == FSGS_F32 ? 4 : 8, chunks = (V + ce - 1) / ce;
-    if (chunks > 64 * 16) return kWideRow;
     int l = 1;
-    while (l < 64 && chunks > 5 * l) l *= 2;
-    return l;
+    while (l <= 64 && chunks > kStep * l) l *= 2;
+    return l <= 64 ? l : kWideRow;
 }
 
 int row_blocks(int64_t rows, int lanes) {
