@@ -12,7 +12,10 @@ namespace fsgs {
 
 namespace {
 
-constexpr int kRowBlocks = 2048;   // workgroups of the row kernels: 8 per CU, the rows go round them
+#ifndef RB
+#define RB 1536
+#endif
+constexpr int kRowBlocks = RB;   // workgroups of the row kernels: 8 per CU, the rows go round them
 constexpr int kWideRow = 256;      // lanes of a row that has a workgroup to itself
 
 struct DistillArgs {
@@ -20,7 +23,7 @@ struct DistillArgs {
     const float *weight;
     int64_t rows, sp, ip, up;
     int V, K, tdtype, idx64;
-    float T, invT, scale2;  // scale2 = log2(e) / T
+    float T, scale2, loss_scale;  // log2(e) / T, T^2 ln 2
     float *row_loss;      // fwd, reduction none: [rows]
     float4 *stat;         // [rows] max s, 1 / sum_j exp, max u, 1 / sum_k exp (0: the row counts for nothing)
     double2 *partial;     // [kRowBlocks] sum of w L, sum of w
@@ -76,9 +79,6 @@ __device__ __forceinline__ bool row_any(bool b) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// exp of a score against a maximum of -inf (no finite score) must not turn -inf - -inf into NaN
-__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
-
 template <typename T>
 __device__ __forceinline__ void unpack(const Chunk &c, float *v) {
     T t[kChunk<T>];
@@ -91,13 +91,14 @@ __device__ __forceinline__ void unpack(const Chunk &c, float *v) {
 // kStep * L chunks: lanes_per_row).  Rows start at any element.  The last chunk of a row that does not end on one is read
 // shifted back to end with the row, its doubled elements masked: no element-wise reads, nothing behind the row.
 constexpr int kStep = 5;
-constexpr int kHeld = 4;  // entries per lane kept in registers; further ones are read again where they are needed
+constexpr int kFullSteps = 2;  // with several lanes per row every row has more than kStep / 2 chunks a lane
+constexpr int kHeld = 2;  // entries per lane kept in registers; further ones are read again where they are needed
 
-template <typename T, int L>
-__device__ __forceinline__ void load_step(Chunk (&c)[kStep], const T *s, int c0, int V) {
+template <typename T, int L, int STEPS>
+__device__ __forceinline__ void load_step(Chunk (&c)[STEPS], const T *s, int c0, int V) {
     constexpr int CE = kChunk<T>;
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) {
+    for (int i = 0; i < STEPS; ++i) {
         const int j = (c0 + i * L) * CE;
         if (V < CE) c[i] = load_chunk_n(s, j < V ? V : 0);
         else c[i] = load_chunk(s + min(j, V - CE));
@@ -122,8 +123,48 @@ __device__ __forceinline__ void forget(Chunk &c) {
     asm volatile("" : "+v"(c.u[0]), "+v"(c.u[1]), "+v"(c.u[2]), "+v"(c.u[3]));
 }
 
-template <typename T, int L>
-__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// Maximum of a lane's chunks.  Half-width types: two elements per instruction on their bits.  As signed integers non-negative
+// floats order as they should and lie above all negative ones; if there is none, the largest negative float has the smallest
+// unsigned bits.  (A NaN is either the largest of all, and then the maximum, or ignored: it reaches the sum either way.)
+template <typename T, int STEPS>
+__device__ __forceinline__ float chunks_max(const Chunk (&c)[STEPS]) {
+    if constexpr (sizeof(T) == 4) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, __builtin_bit_cast(float, c[i].u[e]));
+        return m;
+    } else {
+        i16x2 hi = __builtin_bit_cast(i16x2, c[0].u[0]);
+        u16x2 lo = __builtin_bit_cast(u16x2, c[0].u[0]);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                hi = __builtin_elementwise_max(hi, __builtin_bit_cast(i16x2, c[i].u[e]));
+                lo = __builtin_elementwise_min(lo, __builtin_bit_cast(u16x2, c[i].u[e]));
+            }
+        const int h = max((int)hi.x, (int)hi.y), l = min((int)lo.x, (int)lo.y);
+        return (float)__builtin_bit_cast(T, (unsigned short)(h >= 0 ? h : l));
+    }
+}
+
+// Exponents of a row against its maximum m, in base 2: one multiply-add per score, v scale2 - round(m scale2).  The shift's
+// rounding is the same for every score of the row and cancels in the softmax as long as all of its parts use this form; only
+// where m scale2 itself leaves the range (a row of nothing but the type's lowest value) the difference is taken first.
+struct RowExp {
+    float m, scale2, shift;
+    bool far;
+    __device__ RowExp(float m_, float s) : m(m_ == -INFINITY ? 0.f : m_), scale2(s), shift(m * s), far(!(fabsf(shift) < 1e38f)) {}
+    __device__ __forceinline__ float of(float v) const { return far ? (v - m) * scale2 : fmaf(v, scale2, -shift); }
+};
+
+template <typename T, int L, int STEPS>
+__global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel(DistillArgs a) {
     constexpr int CE = kChunk<T>, ROWS = 256 / L;
     const int sub = threadIdx.x & (L - 1);
     const int chunks = (a.V + CE - 1) / CE;
@@ -133,7 +174,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
         const bool here = slot < a.rows;
         const int64_t row = here ? slot : a.rows - 1;  // (lanes behind the last row repeat it and store nothing)
         const T *s = (const T *)a.s + row * a.sp;
-        Chunk c[kStep];
+        Chunk c[STEPS];
         load_step<T, L>(c, s, sub, a.V);
         int cls[kHeld];
         float u[kHeld], sv[kHeld];
@@ -156,35 +197,40 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
         // maximum and sum of the row: held whole, or step by step with the sum rescaled to each step's maximum
         float m = -INFINITY, sum = 0.f;
         for (int c0 = sub;;) {
-            float mn = m;
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                float v[CE];
-                mask_chunk<T>(c[i], (c0 + i * L) * CE, a.V);
-                unpack<T>(c[i], v);
+            for (int i = 0; i < STEPS; ++i)
+                if (!(L > 1 && L < kWideRow && i < kFullSteps)) mask_chunk<T>(c[i], (c0 + i * L) * CE, a.V);
+            float mc = chunks_max<T>(c);
+            if constexpr (L != kWideRow) mc = row_reduce<L, MaxOp>(mc);
+            const float before = m;
+            m = fmaxf(m, mc);
+            const RowExp x(m, a.scale2);
+            if constexpr (L == kWideRow) sum *= exp2_hw(x.of(before));
+            auto add = [&](auto exponent) {
 #pragma unroll
-                for (int e = 0; e < CE; ++e) mn = fmaxf(mn, v[e]);
-            }
-            const float mf = finite_max(mn);
-            sum *= exp2_hw((m - mf) * a.scale2);
-            m = mn;
+                for (int i = 0; i < STEPS; ++i) {
+                    float v[CE];
+                    if constexpr (sizeof(T) == 2) forget(c[i]);
+                    unpack<T>(c[i], v);
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                float v[CE];
-                if constexpr (sizeof(T) == 2) forget(c[i]);
-                unpack<T>(c[i], v);
-#pragma unroll
-                for (int e = 0; e < CE; ++e) sum += exp2_hw((v[e] - mf) * a.scale2);
-            }
+                    for (int e = 0; e < CE; ++e) sum += exp2_hw(exponent(v[e]));
+                }
+            };
+            if (__any(x.far)) add([&](float v) { return x.of(v); });
+            else add([&](float v) { return fmaf(v, x.scale2, -x.shift); });
             if constexpr (L != kWideRow) break;
-            c0 += kStep * L;
+            c0 += STEPS * L;
             if (c0 - sub >= chunks) break;
             load_step<T, L>(c, s, c0, a.V);
         }
-        const float lane_m = m;
-        m = row_reduce<L, MaxOp>(m);
-        sum = row_reduce<L, AddOp>(sum * exp2_hw((lane_m - finite_max(m)) * a.scale2));
-        // (a row of -inf only: sum 0, and the -inf - -inf below are the NaN that its softmax is)
+        if constexpr (L == kWideRow) {
+            const float lane_m = m;
+            m = row_reduce<L, MaxOp>(m);
+            sum *= exp2_hw(RowExp(m, a.scale2).of(lane_m));
+        }
+        sum = row_reduce<L, AddOp>(sum);
+        const RowExp x(m, a.scale2);
+        if (m == -INFINITY) sum = NAN;  // (a row of -inf only has no softmax)
 
         float um = -INFINITY;
         bool any = false;
@@ -201,13 +247,13 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
             }
         um = row_reduce<L, MaxOp>(um);
         const bool alive = row_any<L>(any) && w != 0.f;
-        // sum_k p_k (log p_k - log q_k) = (sum_k e_k x_k) / Z - log Z + log S with e_k = exp((u_k - um) / T), Z their sum,
-        // x_k = (u_k - um) / T - (s_k - m) / T
+        // sum_k p_k (log p_k - log q_k) = (sum_k e_k y_k) / Z - log Z + log S with e_k = exp((u_k - um) / T), Z their sum,
+        // y_k = (u_k - um) / T - (s_k - m) / T; exponents and logarithms in base 2, ln 2 at the end
         float z = 0.f, ex = 0.f;
         auto entry = [&](float uk, float sk) {
-            const float lu = uk - um, e = exp2_hw(lu * a.scale2);
+            const float lu = (uk - um) * a.scale2, e = exp2_hw(lu);
             z += e;
-            if (e != 0.f) ex += e * ((lu - (sk - m)) * a.invT);
+            if (e != 0.f) ex += e * (lu - x.of(sk));
         };
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
@@ -219,11 +265,11 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
         z = row_reduce<L, AddOp>(z);
         ex = row_reduce<L, AddOp>(ex);
         if (sub == 0 && here) {
-            const float inv_z = 1.f / z;
-            const float loss = (ex * inv_z + (logf(sum) - logf(z))) * (a.T * a.T);
+            const float inv_z = __builtin_amdgcn_rcpf(z);
+            const float loss = (ex * inv_z + (__builtin_amdgcn_logf(sum) - __builtin_amdgcn_logf(z))) * a.loss_scale;
             const float wl = alive ? w * loss : 0.f;
             if (a.row_loss) a.row_loss[row] = wl;
-            if (a.stat) a.stat[row] = make_float4(m, 1.f / sum, um, alive ? inv_z : 0.f);
+            if (a.stat) a.stat[row] = make_float4(m, __builtin_amdgcn_rcpf(sum), um, alive ? inv_z : 0.f);
             if (alive) sum_l += (double)wl, sum_w += (double)w;
         }
     }
@@ -265,114 +311,196 @@ __global__ __launch_bounds__(256) void distill_reduce_kernel(const double2 *__re
     }
 }
 
-// q for every class, then the teacher's classes once more with their mass taken off.  A class may stand in several entries:
-// its first entry carries their sum, taken in the entries' order.  Whether a row has such a class at all is found with one bit
-// per class in LDS; only then are its entries compared pair by pair.
+// LDS of one wave of the backward: its rows' gradients behind up to one chunk of offset, then a bit per class and row.
 template <typename T, int L>
-__global__ __launch_bounds__(256) void distill_bwd_kernel(DistillArgs a) {
-    constexpr int CE = kChunk<T>, ROWS = 256 / L;
-    extern __shared__ uint32_t seen[];  // [ROWS][words]
-    const int sub = threadIdx.x & (L - 1), group = threadIdx.x / L;
-    const int chunks = (a.V + CE - 1) / CE, words = (a.V + 31) / 32;
-    uint32_t *bits = seen + group * words;
+struct BwdLds {
+    int words, bits_at, bytes;
+    __host__ __device__ explicit BwdLds(int V) {
+        words = (V + 31) / 32;
+        bits_at = ((kWave / L) * V * (int)sizeof(T) + 31) / 16 * 16;
+        bytes = bits_at + ((kWave / L) * words * 4 + 15) / 16 * 16;
+    }
+};
+
+// A wave's rows (64 / L of them, neighbours in the gradient) are put together in LDS and leave it as aligned 16-byte
+// streaming stores: rows start at any element, and the line that two stores share would otherwise be written twice.  q of every
+// class goes first, then the teacher's classes once more with their mass taken off.  A class may stand in several entries: its
+// first entry carries their sum, taken in the entries' order; whether a row has such a class at all is found with one bit per
+// class.  A row's lanes are one wave's, and LDS runs in a wave's order: no barrier.
+template <typename T, int L, int STEPS>
+__global__ __launch_bounds__(256, 5) void distill_bwd_kernel(DistillArgs a) {
+    constexpr int CE = kChunk<T>, ROWS = kWave / L;
+    extern __shared__ Chunk lds[];
+    const int lane = threadIdx.x & 63, sub = lane & (L - 1), group = lane / L;
+    const BwdLds<T, L> lay(a.V);
+    char *mine = (char *)lds + (threadIdx.x >> 6) * lay.bytes;
+    uint32_t *bits = (uint32_t *)(mine + lay.bits_at) + group * lay.words;
     const float up = a.g_per_row ? 0.f : a.g[0];
     const float inv_w = a.inv_w ? *a.inv_w : 1.f;
-    for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS) {
+    const int64_t waves = (int64_t)gridDim.x * 4;
+    for (int64_t base = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS; base < a.rows; base += waves * ROWS) {
         const int64_t slot = base + group;
         const bool here = slot < a.rows;
         const int64_t row = here ? slot : a.rows - 1;
         const T *s = (const T *)a.s + row * a.sp;
-        T *ds = (T *)a.ds + row * a.V;
-        Chunk c[kStep];
+        Chunk c[STEPS];
         load_step<T, L>(c, s, sub, a.V);
         const float4 st = a.stat[row];
-        const float m = st.x, um = st.z;
-        const bool dead = st.w == 0.f;
+        const bool dead = st.w == 0.f || !here;
+        const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * (a.g_per_row ? a.g[row] : up) * inv_w;
+        const RowExp x(st.x, a.scale2);
+        const float cq = dead ? 0.f : coef * st.y, cp = coef * st.w;
+        auto class_of = [&](int k) { return class_at(a.idx, row * a.ip + k, a.idx64, a.V); };
+        auto mass_of = [&](int k) { return cp * exp2_hw((teacher_at(a.u, row * a.up + k, a.tdtype) - st.z) * a.scale2); };
         int cls[kHeld];
-        float u[kHeld], sv[kHeld];
+        float p[kHeld], sv[kHeld];
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
             const int k = i * L + sub;
-            cls[i] = -1;
-            if (i * L < a.K && k < a.K) cls[i] = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
+            cls[i] = i * L < a.K && k < a.K && !dead ? class_of(k) : -1;
         }
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            u[i] = sv[i] = 0.f;
+        for (int i = 0; i < kHeld; ++i)
             if (i * L < a.K && cls[i] >= 0) {
-                u[i] = teacher_at(a.u, row * a.up + i * L + sub, a.tdtype);
+                p[i] = mass_of(i * L + sub);
                 sv[i] = (float)s[cls[i]];
                 bits[cls[i] >> 5] = 0;
             }
-        }
-        for (int k = kHeld * L + sub; k < a.K; k += L) {
-            const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
-            if (ck >= 0) bits[ck >> 5] = 0;
-        }
-        const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * (a.g_per_row ? a.g[row] : up) * inv_w;
-        const float cq = coef * st.y;
-        for (int c0 = sub;;) {
+        if (!dead)
+            for (int k = kHeld * L + sub; k < a.K; k += L) {
+                const int ck = class_of(k);
+                if (ck >= 0) bits[ck >> 5] = 0;
+            }
+        // the wave's part of the gradient, at the offset that its start has from a 16-byte boundary
+        T *to = (T *)a.ds + base * a.V;
+        const int off = (int)(((uintptr_t)to & 15) / sizeof(T));
+        T *tile = (T *)mine + off, *out_row = tile + group * a.V;
+        auto put = [&](auto exponent) {
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                const int j = (c0 + i * L) * CE;
+            for (int i = 0; i < STEPS; ++i) {
+                const int j = (sub + i * L) * CE;
                 if (j >= a.V || !here) break;
                 float v[CE];
                 unpack<T>(c[i], v);
                 T out[CE];
 #pragma unroll
-                for (int e = 0; e < CE; ++e) out[e] = (T)(dead ? 0.f : cq * exp2_hw((v[e] - m) * a.scale2));
+                for (int e = 0; e < CE; ++e) out[e] = (T)(cq * exp2_hw(exponent(v[e])));
                 if (a.V < CE) {
 #pragma unroll
                     for (int e = 0; e < CE; ++e)
-                        if (e < a.V) ds[e] = out[e];
+                        if (e < a.V) out_row[e] = out[e];
                 } else {
                     // (the last chunk of a row stores the elements before it a second time, with the same values)
-                    __builtin_memcpy(ds + min(j, a.V - CE), out, sizeof(Chunk));
+                    __builtin_memcpy(out_row + min(j, a.V - CE), out, sizeof(Chunk));
                 }
             }
-            if constexpr (L != kWideRow) break;
-            c0 += kStep * L;
-            if (c0 - sub >= chunks) break;
-            load_step<T, L>(c, s, c0, a.V);
-        }
-        if constexpr (L == kWideRow) __syncthreads();
+        };
+        // (a row that counts for nothing gives zeros, whatever it holds)
+        if (__any(x.far || dead)) put([&](float v) { return dead ? -INFINITY : x.of(v); });
+        else put([&](float v) { return fmaf(v, x.scale2, -x.shift); });
         bool again = false;
         auto mark = [&](int ck) { again |= (atomicOr(&bits[ck >> 5], 1u << (ck & 31)) >> (ck & 31)) & 1u; };
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
             if (i * L < a.K && cls[i] >= 0) mark(cls[i]);
-        for (int k = kHeld * L + sub; k < a.K; k += L) {
-            const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
-            if (ck >= 0) mark(ck);
-        }
+        if (!dead)
+            for (int k = kHeld * L + sub; k < a.K; k += L) {
+                const int ck = class_of(k);
+                if (ck >= 0) mark(ck);
+            }
         again = row_any<L>(again);
-        // every store above has landed before a lane writes over one of them
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if constexpr (L == kWideRow) __syncthreads();
-        auto fix = [&](int k, int ck, float uk, float sk) {
-            float mass = exp2_hw((uk - um) * a.scale2);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        auto fix = [&](int k, int ck, float pk, float sk) {
             if (again) {
-                mass = 0.f;
+                pk = 0.f;
                 bool first = true;
                 for (int t = 0; t < a.K; ++t)
-                    if (class_at(a.idx, row * a.ip + t, a.idx64, a.V) == ck) {
-                        mass += exp2_hw((teacher_at(a.u, row * a.up + t, a.tdtype) - um) * a.scale2);
-                        first &= t >= k;
-                    }
+                    if (class_of(t) == ck) pk += mass_of(t), first &= t >= k;
                 if (!first) return;
             }
-            ds[ck] = (T)(coef * (exp2_hw((sk - m) * a.scale2) * st.y - mass * st.w));
+            out_row[ck] = (T)fmaf(cq, exp2_hw(x.of(sk)), -pk);
         };
-        if (here && !dead) {
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i)
-                if (i * L < a.K && cls[i] >= 0) fix(i * L + sub, cls[i], u[i], sv[i]);
+        for (int i = 0; i < kHeld; ++i)
+            if (i * L < a.K && cls[i] >= 0) fix(i * L + sub, cls[i], p[i], sv[i]);
+        if (!dead)
             for (int k = kHeld * L + sub; k < a.K; k += L) {
-                const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
-                if (ck >= 0) fix(k, ck, teacher_at(a.u, row * a.up + k, a.tdtype), (float)s[ck]);
+                const int ck = class_of(k);
+                if (ck >= 0) fix(k, ck, mass_of(k), (float)s[ck]);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const int n = off + (int)min((int64_t)ROWS, a.rows - base) * a.V;  // elements [off, n) of the wave's LDS
+        T *from = (T *)mine, *dst = to - off;
+        for (int e0 = lane * CE; e0 < n; e0 += kWave * CE) {
+            if (e0 >= off && e0 + CE <= n) {
+                store_streaming(dst + e0, *(const Chunk *)(from + e0));
+            } else {
+#pragma unroll
+                for (int e = 0; e < CE; ++e)
+                    if (e0 + e >= off && e0 + e < n) dst[e0 + e] = from[e0 + e];
             }
         }
-        if constexpr (L == kWideRow) __syncthreads();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// One row per workgroup, too long for a float per class in LDS: q for every class first, then the teacher's classes once more
+// with their mass taken off.  One bit per class finds a class that stands in several entries.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_bwd_wide_kernel(DistillArgs a) {
+    constexpr int CE = kChunk<T>, L = kWideRow;
+    extern __shared__ uint32_t seen[];
+    const int sub = threadIdx.x;
+    const int chunks = (a.V + CE - 1) / CE;
+    const float up = a.g_per_row ? 0.f : a.g[0];
+    const float inv_w = a.inv_w ? *a.inv_w : 1.f;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *s = (const T *)a.s + row * a.sp;
+        T *ds = (T *)a.ds + row * a.V;
+        Chunk c[kStep];
+        load_step<T, L>(c, s, sub, a.V);
+        const float4 st = a.stat[row];
+        const bool dead = st.w == 0.f;
+        const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * (a.g_per_row ? a.g[row] : up) * inv_w;
+        const RowExp x(st.x, a.scale2);
+        const float cq = coef * st.y, cp = coef * st.w;
+        // (at most one entry per lane: K <= 256)
+        const int cls = sub < a.K && !dead ? class_at(a.idx, row * a.ip + sub, a.idx64, a.V) : -1;
+        auto mass_of = [&](int k) { return cp * exp2_hw((teacher_at(a.u, row * a.up + k, a.tdtype) - st.z) * a.scale2); };
+        float q = 0.f, mass = 0.f;
+        if (cls >= 0) {
+            q = cq * exp2_hw(x.of((float)s[cls]));
+            mass = mass_of(sub);
+            seen[cls >> 5] = 0;
+        }
+        for (int c0 = sub;;) {
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                const int j = (c0 + i * L) * CE;
+                if (j >= a.V) break;
+                float v[CE];
+                unpack<T>(c[i], v);
+                T out[CE];
+#pragma unroll
+                for (int e = 0; e < CE; ++e) out[e] = (T)(dead ? 0.f : cq * exp2_hw(x.of(v[e])));
+                __builtin_memcpy(ds + min(j, a.V - CE), out, sizeof(Chunk));
+            }
+            c0 += kStep * L;
+            if (c0 - sub >= chunks) break;
+            load_step<T, L>(c, s, c0, a.V);
+        }
+        // every store above has landed before a lane writes over one of them
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const bool taken = cls >= 0 && ((atomicOr(&seen[cls >> 5], 1u << (cls & 31)) >> (cls & 31)) & 1u);
+        bool first = cls >= 0;
+        if (__syncthreads_or(taken) && cls >= 0) {
+            mass = 0.f;
+            for (int t = 0; t < a.K; ++t)
+                if (class_at(a.idx, row * a.ip + t, a.idx64, a.V) == cls) mass += mass_of(t), first &= t >= sub;
+        }
+        if (first) ds[cls] = (T)(q - mass);
+        __syncthreads();
     }
 }
 
@@ -390,24 +518,35 @@ int row_blocks(int64_t rows, int lanes) {
     return (int)(b < kRowBlocks ? b : kRowBlocks);
 }
 
-template <typename T, int L>
+template <typename T, int L, int STEPS>
 void launch_rows(const DistillArgs &a, bool bwd, hipStream_t st) {
     const int blocks = row_blocks(a.rows, L);
-    if (bwd) distill_bwd_kernel<T, L><<<blocks, 256, (256 / L) * (size_t)((a.V + 31) / 32) * 4, st>>>(a);
-    else distill_fwd_kernel<T, L><<<blocks, 256, 0, st>>>(a);
+    if constexpr (L == kWideRow) {
+        if (bwd) return distill_bwd_wide_kernel<T><<<blocks, 256, (size_t)((a.V + 31) / 32) * 4, st>>>(a);
+    } else {
+        if (bwd) return distill_bwd_kernel<T, L, STEPS><<<blocks, 256, 4 * BwdLds<T, L>(a.V).bytes, st>>>(a);
+    }
+    distill_fwd_kernel<T, L, STEPS><<<blocks, 256, 0, st>>>(a);
+}
+
+template <typename T, int L>
+void launch_steps(const DistillArgs &a, bool bwd, hipStream_t st) {
+    // (a row of three steps does not carry the registers and the idle steps of five: 1080p, V = 21: 67 -> 58 us)
+    if (a.V <= 3 * L * kChunk<T>) launch_rows<T, L, 3>(a, bwd, st);
+    else launch_rows<T, L, kStep>(a, bwd, st);
 }
 
 template <typename T>
 void launch_lanes(const DistillArgs &a, int lanes, bool bwd, hipStream_t st) {
     switch (lanes) {
-        case 1: return launch_rows<T, 1>(a, bwd, st);
-        case 2: return launch_rows<T, 2>(a, bwd, st);
-        case 4: return launch_rows<T, 4>(a, bwd, st);
-        case 8: return launch_rows<T, 8>(a, bwd, st);
-        case 16: return launch_rows<T, 16>(a, bwd, st);
-        case 32: return launch_rows<T, 32>(a, bwd, st);
-        case 64: return launch_rows<T, 64>(a, bwd, st);
-        default: return launch_rows<T, kWideRow>(a, bwd, st);
+        case 1: return launch_steps<T, 1>(a, bwd, st);
+        case 2: return launch_steps<T, 2>(a, bwd, st);
+        case 4: return launch_steps<T, 4>(a, bwd, st);
+        case 8: return launch_steps<T, 8>(a, bwd, st);
+        case 16: return launch_steps<T, 16>(a, bwd, st);
+        case 32: return launch_steps<T, 32>(a, bwd, st);
+        case 64: return launch_steps<T, 64>(a, bwd, st);
+        default: return launch_rows<T, kWideRow, kStep>(a, bwd, st);
     }
 }
 
@@ -446,7 +585,8 @@ extern "C" int fsgs_distill_fwd(int64_t rows, int classes, int top_k, int dtype,
     DistillArgs a = {};
     a.s = logits, a.sp = pitch, a.idx = idx, a.ip = idx_pitch, a.u = teacher, a.up = teacher_pitch, a.weight = weight;
     a.rows = rows, a.V = classes, a.K = top_k, a.tdtype = teacher_dtype, a.idx64 = idx_bits == 64;
-    a.T = temperature, a.invT = 1.f / temperature, a.scale2 = (float)(1.4426950408889634 / (double)temperature);
+    a.T = temperature, a.scale2 = (float)(1.4426950408889634 / (double)temperature);
+    a.loss_scale = (float)((double)temperature * temperature * 0.69314718055994531);
     a.stat = (float4 *)stat;
     if (reduction == FSGS_REDUCE_NONE) a.row_loss = loss;
     else a.partial = (double2 *)scratch;
@@ -473,7 +613,8 @@ extern "C" int fsgs_distill_bwd(int64_t rows, int classes, int top_k, int dtype,
     DistillArgs a = {};
     a.s = logits, a.sp = pitch, a.idx = idx, a.ip = idx_pitch, a.u = teacher, a.up = teacher_pitch, a.weight = weight;
     a.rows = rows, a.V = classes, a.K = top_k, a.tdtype = teacher_dtype, a.idx64 = idx_bits == 64;
-    a.T = temperature, a.invT = 1.f / temperature, a.scale2 = (float)(1.4426950408889634 / (double)temperature);
+    a.T = temperature, a.scale2 = (float)(1.4426950408889634 / (double)temperature);
+    a.loss_scale = (float)((double)temperature * temperature * 0.69314718055994531);
     a.stat = (float4 *)const_cast<float *>(stat);
     a.g = grad_loss, a.g_per_row = grad_per_row, a.inv_w = inv_weight, a.ds = grad_logits;
     return launch(a, dtype, true, as_stream(stream));

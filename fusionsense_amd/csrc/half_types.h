@@ -37,6 +37,12 @@ __device__ __forceinline__ Chunk load_chunk_n(const T *p, int n) {
     return c;
 }
 
+// Past the caches: for outputs that no kernel reads while they could still be there.  16-byte aligned.
+__device__ __forceinline__ void store_streaming(void *p, const Chunk &c) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, c), (u32x4 *)p);
+}
+
 // acc += A B for one 16x16 tile: lane l holds row (l & 15) of A and column (l & 15) of B; its 16 bytes cover the same part
 // of the summed axis in both, so their order along that axis does not matter.  Result: column l & 15, rows 4 (l >> 4) .. + 3.
 template <typename T>
