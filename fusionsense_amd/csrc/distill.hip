@@ -12,10 +12,8 @@ namespace fsgs {
 
 namespace {
 
-#ifndef RB
-#define RB 1536
-#endif
-constexpr int kRowBlocks = RB;   // workgroups of the row kernels: 8 per CU, the rows go round them
+constexpr int kRowBlocks = 1536;   // workgroups that go round the rows: the 6 per CU that are resident at once
+constexpr int kMaxBlocks = 4096;   // ... where a row fills a workgroup: handed out as they finish
 constexpr int kWideRow = 256;      // lanes of a row that has a workgroup to itself
 
 struct DistillArgs {
@@ -26,7 +24,7 @@ struct DistillArgs {
     float T, scale2, loss_scale;  // log2(e) / T, T^2 ln 2
     float *row_loss;      // fwd, reduction none: [rows]
     float4 *stat;         // [rows] max s, 1 / sum_j exp, max u, 1 / sum_k exp (0: the row counts for nothing)
-    double2 *partial;     // [kRowBlocks] sum of w L, sum of w
+    double2 *partial;     // [workgroups] sum of w L, sum of w
     const float *g;       // bwd: upstream gradient (one value, or one per row)
     const float *inv_w;   // bwd: 1 / sum of weights, or null
     int g_per_row;
@@ -52,25 +50,33 @@ struct AddOp {
     __device__ static float f(float a, float b) { return a + b; }
 };
 template <int L, class Op>
-__device__ __forceinline__ float row_reduce(float v) {
+__device__ __forceinline__ float lanes_reduce(float v) {
     if constexpr (L >= 2) v = Op::f(v, dpp_f<0xB1>(v));    // quad_perm [1,0,3,2]
     if constexpr (L >= 4) v = Op::f(v, dpp_f<0x4E>(v));    // quad_perm [2,3,0,1]
     if constexpr (L >= 8) v = Op::f(v, dpp_f<0x141>(v));   // row_half_mirror
     if constexpr (L >= 16) v = Op::f(v, dpp_f<0x140>(v));  // row_mirror
     if constexpr (L >= 32) v = Op::f(v, __shfl_xor(v, 16));
     if constexpr (L >= 64) v = Op::f(v, __shfl_xor(v, 32));
-    if constexpr (L == kWideRow) {
-        __shared__ float part[4];
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = Op::f(Op::f(part[0], part[1]), Op::f(part[2], part[3]));
-    }
     return v;
 }
+// three at once: a row that fills a workgroup joins its waves behind one barrier
+template <int L, class Op>
+__device__ __forceinline__ void row_reduce(float &x, float &y, float &z) {
+    x = lanes_reduce<L, Op>(x), y = lanes_reduce<L, Op>(y), z = lanes_reduce<L, Op>(z);
+    if constexpr (L == kWideRow) {
+        __shared__ float part[3][4];
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            const int w = threadIdx.x >> 6;
+            part[0][w] = x, part[1][w] = y, part[2][w] = z;
+        }
+        __syncthreads();
+        auto all = [](const float *p) { return Op::f(Op::f(p[0], p[1]), Op::f(p[2], p[3])); };
+        x = all(part[0]), y = all(part[1]), z = all(part[2]);
+    }
+}
 template <int L>
-__device__ __forceinline__ bool row_any(bool b) {
-    if constexpr (L == kWideRow) return __syncthreads_or(b);
+__device__ __forceinline__ bool lanes_any(bool b) {
     const uint64_t m = __ballot(b);
     if constexpr (L == 64) return m != 0;
     const int first = (threadIdx.x & 63) & ~(L - 1);
@@ -194,16 +200,31 @@ __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel
         }
         const float w = a.weight ? a.weight[row] : 1.f;
 
-        // maximum and sum of the row: held whole, or step by step with the sum rescaled to each step's maximum
+        float um = -INFINITY, any = 0.f;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            um = fmaxf(um, u[i]);
+            any = u[i] != -INFINITY ? 1.f : any;  // (NaN counts: it reaches the loss)
+        }
+        for (int k = kHeld * L + sub; k < a.K; k += L)
+            if (class_at(a.idx, row * a.ip + k, a.idx64, a.V) >= 0) {
+                const float uk = teacher_at(a.u, row * a.up + k, a.tdtype);
+                um = fmaxf(um, uk);
+                any = uk != -INFINITY ? 1.f : any;
+            }
+
+        // maximum and sum of the row: held whole, or step by step with a lane's sum rescaled to its new maximum
         float m = -INFINITY, sum = 0.f;
         for (int c0 = sub;;) {
+            const bool more = L == kWideRow && c0 - sub + STEPS * L < chunks;
+            Chunk ahead[STEPS];
+            if (more) load_step<T, L>(ahead, s, c0 + STEPS * L, a.V);
 #pragma unroll
             for (int i = 0; i < STEPS; ++i)
                 if (!(L > 1 && L < kWideRow && i < kFullSteps)) mask_chunk<T>(c[i], (c0 + i * L) * CE, a.V);
-            float mc = chunks_max<T>(c);
-            if constexpr (L != kWideRow) mc = row_reduce<L, MaxOp>(mc);
             const float before = m;
-            m = fmaxf(m, mc);
+            m = fmaxf(m, chunks_max<T>(c));
+            if constexpr (L != kWideRow) row_reduce<L, MaxOp>(m, um, any);
             const RowExp x(m, a.scale2);
             if constexpr (L == kWideRow) sum *= exp2_hw(x.of(before));
             auto add = [&](auto exponent) {
@@ -218,35 +239,18 @@ __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel
             };
             if (__any(x.far)) add([&](float v) { return x.of(v); });
             else add([&](float v) { return fmaf(v, x.scale2, -x.shift); });
-            if constexpr (L != kWideRow) break;
+            if (!more) break;
             c0 += STEPS * L;
-            if (c0 - sub >= chunks) break;
-            load_step<T, L>(c, s, c0, a.V);
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) c[i] = ahead[i];
         }
         if constexpr (L == kWideRow) {
             const float lane_m = m;
-            m = row_reduce<L, MaxOp>(m);
+            row_reduce<L, MaxOp>(m, um, any);
             sum *= exp2_hw(RowExp(m, a.scale2).of(lane_m));
         }
-        sum = row_reduce<L, AddOp>(sum);
         const RowExp x(m, a.scale2);
-        if (m == -INFINITY) sum = NAN;  // (a row of -inf only has no softmax)
-
-        float um = -INFINITY;
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            um = fmaxf(um, u[i]);
-            any |= u[i] != -INFINITY;  // (NaN counts: it reaches the loss)
-        }
-        for (int k = kHeld * L + sub; k < a.K; k += L)
-            if (class_at(a.idx, row * a.ip + k, a.idx64, a.V) >= 0) {
-                const float uk = teacher_at(a.u, row * a.up + k, a.tdtype);
-                um = fmaxf(um, uk);
-                any |= uk != -INFINITY;
-            }
-        um = row_reduce<L, MaxOp>(um);
-        const bool alive = row_any<L>(any) && w != 0.f;
+        const bool alive = any != 0.f && w != 0.f;
         // sum_k p_k (log p_k - log q_k) = (sum_k e_k y_k) / Z - log Z + log S with e_k = exp((u_k - um) / T), Z their sum,
         // y_k = (u_k - um) / T - (s_k - m) / T; exponents and logarithms in base 2, ln 2 at the end
         float z = 0.f, ex = 0.f;
@@ -262,8 +266,8 @@ __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel
             const int ck = class_at(a.idx, row * a.ip + k, a.idx64, a.V);
             if (ck >= 0) entry(teacher_at(a.u, row * a.up + k, a.tdtype), (float)s[ck]);
         }
-        z = row_reduce<L, AddOp>(z);
-        ex = row_reduce<L, AddOp>(ex);
+        row_reduce<L, AddOp>(sum, z, ex);
+        if (m == -INFINITY) sum = NAN;  // (a row of -inf only has no softmax)
         if (sub == 0 && here) {
             const float inv_z = __builtin_amdgcn_rcpf(z);
             const float loss = (ex * inv_z + (__builtin_amdgcn_logf(sum) - __builtin_amdgcn_logf(z))) * a.loss_scale;
@@ -408,7 +412,7 @@ __global__ __launch_bounds__(256, 5) void distill_bwd_kernel(DistillArgs a) {
                 const int ck = class_of(k);
                 if (ck >= 0) mark(ck);
             }
-        again = row_any<L>(again);
+        again = lanes_any<L>(again);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         auto fix = [&](int k, int ck, float pk, float sk) {
             if (again) {
@@ -514,8 +518,8 @@ int lanes_per_row(int V, int dtype) {
 }
 
 int row_blocks(int64_t rows, int lanes) {
-    const int64_t per = 256 / lanes, b = (rows + per - 1) / per;
-    return (int)(b < kRowBlocks ? b : kRowBlocks);
+    const int64_t per = 256 / lanes, b = (rows + per - 1) / per, most = lanes == kWideRow ? kMaxBlocks : kRowBlocks;
+    return (int)(b < most ? b : most);
 }
 
 template <typename T, int L, int STEPS>
@@ -570,7 +574,7 @@ bool bad_args(int64_t rows, int V, int K, int dtype, int tdtype, int idx_bits, f
 
 using namespace fsgs;
 
-extern "C" int64_t fsgs_distill_scratch_bytes(void) { return (int64_t)kRowBlocks * sizeof(double2); }
+extern "C" int64_t fsgs_distill_scratch_bytes(void) { return (int64_t)kMaxBlocks * sizeof(double2); }
 
 extern "C" int fsgs_distill_fwd(int64_t rows, int classes, int top_k, int dtype, const void *logits, int64_t pitch,
                                 int idx_bits, const void *idx, int64_t idx_pitch, int teacher_dtype, const void *teacher,
