@@ -151,6 +151,130 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
     }
 }
 
+// ---- short summed axis: rows go straight from memory to the matrix pipe ------------------------------------------------
+// One wave takes 16 * MT rows at a time and all columns of its workgroup's range.  W (its range) lies in LDS for the life of
+// the workgroup, a row of x is read once, 16 bytes per lane, directly in the layout of the B operand: no barrier and no staging
+// in the loop.  Columns go by groups of 32 (two A tiles): in the half-width types tile t holds the rows of W with
+// column = 8 (r / 4) + 4 t + r % 4 of the group, so that a lane ends with 8 neighbouring columns of one row, 16 bytes.
+struct RowsArgs {
+    LinArgs l;
+    int range;      // columns per workgroup (a multiple of 32)
+    int transpose;  // W is given as [K,N] (its element (n,k) at k * N + n)
+};
+
+template <typename T>
+__device__ __forceinline__ int group_column(int t, int r) {
+    return sizeof(T) == 2 ? (r >> 2) * 8 + t * 4 + (r & 3) : t * 16 + r;
+}
+
+template <typename T, int KC>
+constexpr int rows_pitch() { return KC * 4 + 1; }  // chunks between two rows of W in LDS: 16 rows then lie in 16 bank quads
+
+// W's rows [n0, n0 + range) into LDS, zero behind N and K.
+template <typename T, int KC>
+__device__ __forceinline__ void fill_weights(Chunk *wl, const T *w, int n0, int range, int N, int K, int transpose) {
+    constexpr int CE = kChunk<T>, P = rows_pitch<T, KC>();
+    if (!transpose) {
+        for (int c = threadIdx.x; c < range * KC * 4; c += blockDim.x) {
+            const int n = c / (KC * 4), k = (c % (KC * 4)) * CE;
+            wl[n * P + c % (KC * 4)] = load_chunk_n(w + (int64_t)(n0 + n) * K + k, n0 + n < N ? K - k : 0);
+        }
+    } else {
+        for (int c = threadIdx.x; c < range * KC * 4 * CE; c += blockDim.x) {
+            const int k = c / range, n = c % range;
+            ((T *)(wl + n * P))[k] = n0 + n < N && k < K ? w[(int64_t)k * N + n0 + n] : (T)0.f;
+        }
+    }
+}
+
+template <typename T, int MODE, int KC, int MT, bool FULL>
+__global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
+    constexpr int CE = kChunk<T>, P = rows_pitch<T, KC>();
+    extern __shared__ Chunk lds[];
+    const LinArgs &a = ra.l;
+    const T *x = (const T *)a.x;
+    T *y = (T *)a.y;
+    Chunk *wl = lds;
+    float *bl = (float *)(lds + ra.range * P);
+    const int n0 = blockIdx.y * ra.range, ncols = min(ra.range, a.N - n0);
+    fill_weights<T, KC>(wl, (const T *)a.w, n0, ra.range, a.N, a.K, ra.transpose);
+    for (int n = threadIdx.x; n < ra.range; n += 256)
+        bl[n] = a.bias && n < ncols ? (float)((const T *)a.bias)[n0 + n] : 0.f;
+    __syncthreads();
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    constexpr int CPG = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of a row that a lane holds of a group
+    const T *side = (const T *)(MODE == kModeDz ? a.dy : a.res);
+    const int64_t sp = MODE == kModeDz ? a.dyp : a.rp;
+    const int64_t tiles = (a.rows + 16 * MT - 1) / (16 * MT), step = (int64_t)gridDim.x * 4;
+    for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < tiles; t += step) {
+        int64_t m[MT];
+        Chunk xf[MT][KC];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            m[j] = t * (16 * MT) + j * 16 + li;
+            const T *xr = x + min(m[j], a.rows - 1) * a.xp;  // (lanes behind the last row repeat it and store nothing)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const int k = (c * 4 + lg) * CE;
+                xf[j][c] = FULL ? load_chunk(xr + k) : load_chunk_n(xr + k, a.K - k);
+            }
+        }
+        auto load_side = [&](Chunk (&s)[MT][CPG], int g) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int q = 0; q < CPG; ++q) {
+                    const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                    s[j][q] = load_chunk_n(side + min(m[j], a.rows - 1) * sp + n0 + n, ncols - n);
+                }
+        };
+        Chunk sc[MT][CPG];
+        if (side) load_side(sc, 0);
+        for (int g = 0; g * 32 < ncols; ++g) {
+            f32x4 acc[2][MT] = {};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const Chunk wf = wl[(g * 32 + group_column<T>(i, li)) * P + c * 4 + lg];
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) mma_chunk<T>(acc[i][j], wf, xf[j][c]);
+                }
+            }
+            Chunk sn[MT][CPG];
+            if (side && (g + 1) * 32 < ncols) load_side(sn, g + 1);
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int q = 0; q < CPG; ++q) {
+                    const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                    T sv[CE], out[CE];
+                    if (side) __builtin_memcpy(sv, &sc[j][q], sizeof(Chunk));
+#pragma unroll
+                    for (int e = 0; e < CE; ++e) {
+                        const float z = (CPG == 1 ? acc[e >> 2][j][e & 3] : acc[q][j][e]) + bl[n + e];
+                        float v;
+                        if constexpr (MODE == kModeDz) v = (float)sv[e] * act_slope(z, a.act);
+                        else v = act_fwd(z, a.act) + (side ? (float)sv[e] : 0.f);
+                        out[e] = (T)v;
+                    }
+                    if (m[j] < a.rows) {
+                        T *dst = y + m[j] * a.yp + n0 + n;
+                        if (n + CE <= ncols) __builtin_memcpy(dst, out, sizeof(Chunk));
+                        else
+#pragma unroll
+                            for (int e = 0; e < CE; ++e)
+                                if (n + e < ncols) dst[e] = out[e];
+                    }
+                }
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int q = 0; q < CPG; ++q) sc[j][q] = sn[j][q];
+        }
+    }
+}
+
 // W [N,K] -> W^T [K,N]: the operand of dx = dz W with its summed axis contiguous.
 template <typename T>
 __global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w, T *__restrict__ wt, int N, int K) {
@@ -262,8 +386,47 @@ __global__ __launch_bounds__(256) void reduce_slices_kernel(const float *__restr
     }
 }
 
+// LDS of a workgroup of the rows kernel: at most 40 KB, four workgroups per CU.
+constexpr int kRowsLds = 40 * 1024;
+
+template <typename T, int MODE, int KC, int MT>
+int launch_rows_mt(const RowsArgs &r, int64_t tiles, hipStream_t s) {
+    const int ranges = (r.l.N + r.range - 1) / r.range;
+    const int64_t want = (tiles + 3) / 4;
+    const unsigned blocks = (unsigned)(want < 1024 ? want : 1024);
+    const size_t bytes = (size_t)r.range * (rows_pitch<T, KC>() * 16 + 4);
+    const dim3 grid(blocks, ranges);
+    if (r.l.K == KC * 4 * kChunk<T>) linear_rows_kernel<T, MODE, KC, MT, true><<<grid, 256, bytes, s>>>(r);
+    else linear_rows_kernel<T, MODE, KC, MT, false><<<grid, 256, bytes, s>>>(r);
+    return check_launch();
+}
+
+template <typename T, int MODE, int KC>
+int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
+    RowsArgs r;
+    r.l = a;
+    r.transpose = transpose;
+    const int fit = kRowsLds / (rows_pitch<T, KC>() * 16 + 4) / 32 * 32, need = (a.N + 31) / 32 * 32;
+    r.range = need < fit ? need : fit;
+    if (a.rows >= 1 << 17) return launch_rows_mt<T, MODE, KC, 2>(r, (a.rows + 31) / 32, s);
+    return launch_rows_mt<T, MODE, KC, 1>(r, (a.rows + 15) / 16, s);
+}
+
+template <typename T>
+bool rows_fit(int K) { return (size_t)K * sizeof(T) <= 512; }
+
+template <typename T, int MODE>
+int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
+    const int bytes = a.K * (int)sizeof(T);
+    if (bytes <= 64) return launch_rows_kc<T, MODE, 1>(a, transpose, s);
+    if (bytes <= 128) return launch_rows_kc<T, MODE, 2>(a, transpose, s);
+    if (bytes <= 256) return launch_rows_kc<T, MODE, 4>(a, transpose, s);
+    return launch_rows_kc<T, MODE, 8>(a, transpose, s);
+}
+
 template <typename T, int MODE>
 int launch_tile(const LinArgs &a, hipStream_t s) {
+    if (rows_fit<T>(a.K)) return launch_rows<T, MODE>(a, 0, s);
     const int64_t mt = (a.rows + kBM - 1) / kBM;
     const int bn = a.N > 64 ? 128 : 64;
     const int64_t tiles = mt * ((a.N + bn - 1) / bn);
