@@ -22,25 +22,63 @@ struct LinArgs {
     int K, N, act;
 };
 
-__device__ __forceinline__ float act_fwd(float z, int act) {
-    switch (act) {
-        case FSGS_ACT_RELU: return z > 0.f ? z : (z == z ? 0.f : z);
-        case FSGS_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-        case FSGS_ACT_SILU: return z / (1.f + expf(-z));
-        default: return z;
+// The normal distribution's tail h = P(t) exp(-z^2 / 2) at |z|, t = 1 / (1 + 0.34 |z|), P of degree 7 without a constant term
+// (fitted here to erfc: |error of h| < 9e-9, a seventh of half an fp32 step at 1), and the exponential itself.
+__device__ __forceinline__ float normal_tail(float z, float &e) {
+    const float az = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(0.34f, az, 1.f));
+    e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    float p = 0.04310445f;
+    p = fmaf(p, t, -0.19278112f);
+    p = fmaf(p, t, 0.24988606f);
+    p = fmaf(p, t, -0.0172307f);
+    p = fmaf(p, t, 0.1495994f);
+    p = fmaf(p, t, 0.13158924f);
+    p = fmaf(p, t, 0.13583268f);
+    return p * t * e;
+}
+
+// z -> act(z) for N values (one uniform branch for all of them).
+template <int N>
+__device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
+    if (act == FSGS_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = z[i] < 0.f ? 0.f : z[i];  // (NaN stays)
+    } else if (act == FSGS_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float e;
+            const float h = normal_tail(z[i], e);
+            z[i] *= z[i] < 0.f ? h : 1.f - h;
+        }
+    } else if (act == FSGS_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            z[i] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[i] * -1.4426950408889634f));
     }
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case FSGS_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case FSGS_ACT_GELU:
-            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-        case FSGS_ACT_SILU: {
-            const float s = 1.f / (1.f + expf(-z));
-            return s * (1.f + z * (1.f - s));
+// z -> act'(z) for N values.
+template <int N>
+__device__ __forceinline__ void act_slope(float (&z)[N], int act) {
+    if (act == FSGS_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? 1.f : 0.f;
+    } else if (act == FSGS_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float e;
+            const float h = normal_tail(z[i], e);
+            z[i] = (z[i] < 0.f ? h : 1.f - h) + z[i] * 0.39894228040143268f * e;
         }
-        default: return 1.f;
+    } else if (act == FSGS_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[i] * -1.4426950408889634f));
+            z[i] = s * fmaf(z[i], 1.f - s, 1.f);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = 1.f;
     }
 }
 
@@ -136,13 +174,16 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
                 if (nv == 4) __builtin_memcpy(sv, side, sizeof(sv));
                 else for (int q = 0; q < nv; ++q) sv[q] = side[q];
             }
+            float z[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[q] = acc[i][j][q] + b[q];
+            if constexpr (MODE == kModeDz) act_slope(z, a.act);
+            else act_fwd(z, a.act);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float z = acc[i][j][q] + b[q];
-                float v;
-                if constexpr (MODE == kModeDz) v = (float)sv[q] * act_slope(z, a.act);
-                else v = act_fwd(z, a.act) + (side ? (float)sv[q] : 0.f);
-                out[q] = (T)v;
+                if constexpr (MODE == kModeDz) z[q] *= (float)sv[q];
+                else z[q] += side ? (float)sv[q] : 0.f;
+                out[q] = (T)z[q];
             }
             T *dst = y + m * a.yp + n;
             if (nv == 4) __builtin_memcpy(dst, out, sizeof(out));
@@ -152,14 +193,22 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
 }
 
 // ---- short summed axis: rows go straight from memory to the matrix pipe ------------------------------------------------
-// One wave takes 16 * MT rows at a time and all columns of its workgroup's range.  W (its range) lies in LDS for the life of
-// the workgroup, a row of x is read once, 16 bytes per lane, directly in the layout of the B operand: no barrier and no staging
+// One wave takes 16 rows at a time and all columns of its workgroup's range.  W (its range) lies in LDS for the life of the
+// workgroup, a row of x is read once, 16 bytes per lane, directly in the layout of the B operand: no barrier and no staging
 // in the loop.  Columns go by groups of 32 (two A tiles): in the half-width types tile t holds the rows of W with
 // column = 8 (r / 4) + 4 t + r % 4 of the group, so that a lane ends with 8 neighbouring columns of one row, 16 bytes.
+//
+// How y is stored (640 000 rows, 64 -> 128 bf16: plain 77 us, streaming 49; 32 -> 150 fp32: plain 190, streaming 463):
+//   kStorePlain   through the caches: small outputs, which the next kernel finds there
+//   kStoreStream  past the caches; rows must start at 64-byte boundaries, which a store instruction then covers whole
+//   kStoreTile    the wave's 16 rows (neighbours in y) are put together in LDS and leave it as aligned streaming stores
+enum { kStorePlain = 0, kStoreStream = 1, kStoreTile = 2 };
+
 struct RowsArgs {
     LinArgs l;
     int range;      // columns per workgroup (a multiple of 32)
     int transpose;  // W is given as [K,N] (its element (n,k) at k * N + n)
+    int store;
 };
 
 template <typename T>
@@ -169,6 +218,9 @@ __device__ __forceinline__ int group_column(int t, int r) {
 
 template <typename T, int KC>
 constexpr int rows_pitch() { return KC * 4 + 1; }  // chunks between two rows of W in LDS: 16 rows then lie in 16 bank quads
+
+template <typename T>
+constexpr int tile_bytes(int N) { return (16 * N * (int)sizeof(T) + 31) / 16 * 16; }  // (with an offset of up to a chunk)
 
 // W's rows [n0, n0 + range) into LDS, zero behind N and K.
 template <typename T, int KC>
@@ -187,7 +239,7 @@ __device__ __forceinline__ void fill_weights(Chunk *wl, const T *w, int n0, int 
     }
 }
 
-template <typename T, int MODE, int KC, int MT, bool FULL>
+template <typename T, int MODE, int KC, bool FULL>
 __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     constexpr int CE = kChunk<T>, P = rows_pitch<T, KC>();
     extern __shared__ Chunk lds[];
@@ -201,76 +253,85 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     for (int n = threadIdx.x; n < ra.range; n += 256)
         bl[n] = a.bias && n < ncols ? (float)((const T *)a.bias)[n0 + n] : 0.f;
     __syncthreads();
-    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+    char *mine = (char *)(bl + ra.range) + wave * tile_bytes<T>(a.N);  // (kStoreTile)
     constexpr int CPG = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of a row that a lane holds of a group
     const T *side = (const T *)(MODE == kModeDz ? a.dy : a.res);
     const int64_t sp = MODE == kModeDz ? a.dyp : a.rp;
-    const int64_t tiles = (a.rows + 16 * MT - 1) / (16 * MT), step = (int64_t)gridDim.x * 4;
-    for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < tiles; t += step) {
-        int64_t m[MT];
-        Chunk xf[MT][KC];
+    const int64_t tiles = (a.rows + 15) / 16, step = (int64_t)gridDim.x * 4;
+    for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < tiles; t += step) {
+        const int64_t m = t * 16 + li, mr = min(m, a.rows - 1);  // (lanes behind the last row repeat it and store nothing)
+        Chunk xf[KC];
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            m[j] = t * (16 * MT) + j * 16 + li;
-            const T *xr = x + min(m[j], a.rows - 1) * a.xp;  // (lanes behind the last row repeat it and store nothing)
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const int k = (c * 4 + lg) * CE;
-                xf[j][c] = FULL ? load_chunk(xr + k) : load_chunk_n(xr + k, a.K - k);
-            }
+        for (int c = 0; c < KC; ++c) {
+            const int k = (c * 4 + lg) * CE;
+            xf[c] = FULL ? load_chunk(x + mr * a.xp + k) : load_chunk_n(x + mr * a.xp + k, a.K - k);
         }
-        auto load_side = [&](Chunk (&s)[MT][CPG], int g) {
+        auto load_side = [&](Chunk (&s)[CPG], int g) {
 #pragma unroll
-            for (int j = 0; j < MT; ++j)
-#pragma unroll
-                for (int q = 0; q < CPG; ++q) {
-                    const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
-                    s[j][q] = load_chunk_n(side + min(m[j], a.rows - 1) * sp + n0 + n, ncols - n);
-                }
+            for (int q = 0; q < CPG; ++q) {
+                const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                s[q] = load_chunk_n(side + mr * sp + n0 + n, ncols - n);
+            }
         };
-        Chunk sc[MT][CPG];
+        T *to = y + t * 16 * a.yp;  // (kStoreTile: yp == N, one range)
+        const int off = ra.store == kStoreTile ? (int)(((uintptr_t)to & 15) / sizeof(T)) : 0;
+        Chunk sc[CPG];
         if (side) load_side(sc, 0);
         for (int g = 0; g * 32 < ncols; ++g) {
-            f32x4 acc[2][MT] = {};
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const Chunk wf = wl[(g * 32 + group_column<T>(i, li)) * P + c * 4 + lg];
-#pragma unroll
-                    for (int j = 0; j < MT; ++j) mma_chunk<T>(acc[i][j], wf, xf[j][c]);
-                }
-            }
-            Chunk sn[MT][CPG];
+            Chunk sn[CPG];
             if (side && (g + 1) * 32 < ncols) load_side(sn, g + 1);
+            f32x4 acc[2] = {};
 #pragma unroll
-            for (int j = 0; j < MT; ++j)
+            for (int c = 0; c < KC; ++c)
 #pragma unroll
-                for (int q = 0; q < CPG; ++q) {
-                    const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
-                    T sv[CE], out[CE];
-                    if (side) __builtin_memcpy(sv, &sc[j][q], sizeof(Chunk));
+                for (int i = 0; i < 2; ++i)
+                    mma_chunk<T>(acc[i], wl[(g * 32 + group_column<T>(i, li)) * P + c * 4 + lg], xf[c]);
+            float z[8];
+            T sv[8], out[8];
 #pragma unroll
-                    for (int e = 0; e < CE; ++e) {
-                        const float z = (CPG == 1 ? acc[e >> 2][j][e & 3] : acc[q][j][e]) + bl[n + e];
-                        float v;
-                        if constexpr (MODE == kModeDz) v = (float)sv[e] * act_slope(z, a.act);
-                        else v = act_fwd(z, a.act) + (side ? (float)sv[e] : 0.f);
-                        out[e] = (T)v;
-                    }
-                    if (m[j] < a.rows) {
-                        T *dst = y + m[j] * a.yp + n0 + n;
-                        if (n + CE <= ncols) __builtin_memcpy(dst, out, sizeof(Chunk));
-                        else
+            for (int q = 0; q < CPG; ++q) __builtin_memcpy(sv + q * CE, &sc[q], sizeof(Chunk));
 #pragma unroll
-                            for (int e = 0; e < CE; ++e)
-                                if (n + e < ncols) dst[e] = out[e];
-                    }
+            for (int e = 0; e < 8; ++e) z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
+            if constexpr (MODE == kModeDz) act_slope(z, a.act);
+            else act_fwd(z, a.act);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (MODE == kModeDz) z[e] *= (float)sv[e];
+                else if (side) z[e] += (float)sv[e];
+                out[e] = (T)z[e];
+            }
+#pragma unroll
+            for (int q = 0; q < CPG; ++q) {
+                const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                if (m < a.rows && n < ncols) {
+                    T *dst = ra.store == kStoreTile ? (T *)mine + off + li * a.N + n : y + m * a.yp + n0 + n;
+                    if (n + CE <= ncols) {
+                        Chunk o;
+                        __builtin_memcpy(&o, out + q * CE, sizeof(Chunk));
+                        if (ra.store == kStoreStream) store_streaming(dst, o);
+                        else __builtin_memcpy(dst, &o, sizeof(Chunk));
+                    } else
+#pragma unroll
+                        for (int e = 0; e < CE; ++e)
+                            if (n + e < ncols) dst[e] = out[q * CE + e];
                 }
+                sc[q] = sn[q];
+            }
+        }
+        if (ra.store == kStoreTile) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (LDS runs in the wave's order: no barrier)
+            const int n = off + (int)min((int64_t)16, a.rows - t * 16) * a.N;
+            const T *from = (const T *)mine;
+            T *dst = to - off;
+            for (int e0 = lane * CE; e0 < n; e0 += kWave * CE) {
+                if (e0 >= off && e0 + CE <= n) store_streaming(dst + e0, *(const Chunk *)(from + e0));
+                else
 #pragma unroll
-            for (int j = 0; j < MT; ++j)
-#pragma unroll
-                for (int q = 0; q < CPG; ++q) sc[j][q] = sn[j][q];
+                    for (int e = 0; e < CE; ++e)
+                        if (e0 + e >= off && e0 + e < n) dst[e0 + e] = from[e0 + e];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
 }
@@ -386,30 +447,37 @@ __global__ __launch_bounds__(256) void reduce_slices_kernel(const float *__restr
     }
 }
 
-// LDS of a workgroup of the rows kernel: at most 40 KB, four workgroups per CU.
+// LDS of a workgroup of the rows kernel: weights up to 40 KB, four workgroups per CU; with the waves' output tiles up to 80 KB.
 constexpr int kRowsLds = 40 * 1024;
-
-template <typename T, int MODE, int KC, int MT>
-int launch_rows_mt(const RowsArgs &r, int64_t tiles, hipStream_t s) {
-    const int ranges = (r.l.N + r.range - 1) / r.range;
-    const int64_t want = (tiles + 3) / 4;
-    const unsigned blocks = (unsigned)(want < 1024 ? want : 1024);
-    const size_t bytes = (size_t)r.range * (rows_pitch<T, KC>() * 16 + 4);
-    const dim3 grid(blocks, ranges);
-    if (r.l.K == KC * 4 * kChunk<T>) linear_rows_kernel<T, MODE, KC, MT, true><<<grid, 256, bytes, s>>>(r);
-    else linear_rows_kernel<T, MODE, KC, MT, false><<<grid, 256, bytes, s>>>(r);
-    return check_launch();
-}
+constexpr int64_t kStreamBytes = 32 << 20;  // outputs from here on are stored past the caches
 
 template <typename T, int MODE, int KC>
 int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
     RowsArgs r;
     r.l = a;
     r.transpose = transpose;
-    const int fit = kRowsLds / (rows_pitch<T, KC>() * 16 + 4) / 32 * 32, need = (a.N + 31) / 32 * 32;
+    const int row_bytes = rows_pitch<T, KC>() * 16 + 4;
+    const int fit = kRowsLds / row_bytes / 32 * 32, need = (a.N + 31) / 32 * 32;
     r.range = need < fit ? need : fit;
-    if (a.rows >= 1 << 17) return launch_rows_mt<T, MODE, KC, 2>(r, (a.rows + 31) / 32, s);
-    return launch_rows_mt<T, MODE, KC, 1>(r, (a.rows + 15) / 16, s);
+    const int ranges = (a.N + r.range - 1) / r.range;
+    size_t bytes = (size_t)r.range * row_bytes;
+    r.store = kStorePlain;
+    if (a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes) {
+        const size_t tiles = 4 * (size_t)tile_bytes<T>(a.N);
+        if (a.N * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0) r.store = kStoreStream;
+        else if (ranges == 1 && a.yp == a.N && bytes + tiles <= 2 * kRowsLds) r.store = kStoreTile, bytes += tiles;
+    }
+    const int64_t want = (a.rows + 63) / 64;
+    const dim3 grid((unsigned)(want < 1024 ? want : 1024), ranges);
+    const bool full = a.K == KC * 4 * kChunk<T>;
+    int rc = FSGS_OK;
+    if (bytes > 64 * 1024)
+        rc = full ? ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, true>>(bytes)
+                  : ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, false>>(bytes);
+    if (rc != FSGS_OK) return rc;
+    if (full) linear_rows_kernel<T, MODE, KC, true><<<grid, 256, bytes, s>>>(r);
+    else linear_rows_kernel<T, MODE, KC, false><<<grid, 256, bytes, s>>>(r);
+    return check_launch();
 }
 
 template <typename T>
