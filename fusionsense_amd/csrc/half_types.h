@@ -37,6 +37,32 @@ __device__ __forceinline__ Chunk load_chunk_n(const T *p, int n) {
     return c;
 }
 
+// kChunk floats rounded (to nearest, ties to even) to a chunk: two per instruction in the half-width types.
+template <typename T>
+__device__ __forceinline__ Chunk pack_chunk(const float *v) {
+    Chunk c;
+    if constexpr (sizeof(T) == 4) {
+        __builtin_memcpy(&c, v, sizeof(Chunk));
+    } else {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef T tx2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x2 p = {v[2 * i], v[2 * i + 1]};
+            c.u[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, tx2));
+        }
+    }
+    return c;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_chunk(const Chunk &c, float *v) {
+    T t[kChunk<T>];
+    __builtin_memcpy(t, &c, sizeof(Chunk));
+#pragma unroll
+    for (int e = 0; e < kChunk<T>; ++e) v[e] = (float)t[e];
+}
+
 // Past the caches: for outputs that no kernel reads while they could still be there.  16-byte aligned.
 __device__ __forceinline__ void store_streaming(void *p, const Chunk &c) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -47,8 +47,7 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float e;
-            const float h = normal_tail(z[i], e);
-            z[i] *= z[i] < 0.f ? h : 1.f - h;
+            z[i] = fmaf(-fabsf(z[i]), normal_tail(z[i], e), fmaxf(z[i], 0.f));  // z >= 0: z - z h; z < 0: -|z| h
         }
     } else if (act == FSGS_ACT_SILU) {
 #pragma unroll
@@ -208,7 +207,6 @@ struct RowsArgs {
     LinArgs l;
     int range;      // columns per workgroup (a multiple of 32)
     int transpose;  // W is given as [K,N] (its element (n,k) at k * N + n)
-    int store;
 };
 
 template <typename T>
@@ -239,7 +237,22 @@ __device__ __forceinline__ void fill_weights(Chunk *wl, const T *w, int n0, int 
     }
 }
 
-template <typename T, int MODE, int KC, bool FULL>
+// The first n (at least one) elements of a chunk.
+template <typename T>
+__device__ __forceinline__ void put_chunk(T *to, const Chunk &c, int n, bool stream) {
+    if (n >= kChunk<T>) {
+        if (stream) store_streaming(to, c);
+        else __builtin_memcpy(to, &c, sizeof(Chunk));
+    } else {
+        T t[kChunk<T>];
+        __builtin_memcpy(t, &c, sizeof(Chunk));
+#pragma unroll
+        for (int e = 0; e < kChunk<T>; ++e)
+            if (e < n) to[e] = t[e];
+    }
+}
+
+template <typename T, int MODE, int KC, int STORE>
 __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     constexpr int CE = kChunk<T>, P = rows_pitch<T, KC>();
     extern __shared__ Chunk lds[];
@@ -255,6 +268,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     __syncthreads();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
     char *mine = (char *)(bl + ra.range) + wave * tile_bytes<T>(a.N);  // (kStoreTile)
+    const bool full = a.K == KC * 4 * CE;
     constexpr int CPG = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of a row that a lane holds of a group
     const T *side = (const T *)(MODE == kModeDz ? a.dy : a.res);
     const int64_t sp = MODE == kModeDz ? a.dyp : a.rp;
@@ -265,7 +279,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             const int k = (c * 4 + lg) * CE;
-            xf[c] = FULL ? load_chunk(x + mr * a.xp + k) : load_chunk_n(x + mr * a.xp + k, a.K - k);
+            xf[c] = full ? load_chunk(x + mr * a.xp + k) : load_chunk_n(x + mr * a.xp + k, a.K - k);
         }
         auto load_side = [&](Chunk (&s)[CPG], int g) {
 #pragma unroll
@@ -275,7 +289,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
             }
         };
         T *to = y + t * 16 * a.yp;  // (kStoreTile: yp == N, one range)
-        const int off = ra.store == kStoreTile ? (int)(((uintptr_t)to & 15) / sizeof(T)) : 0;
+        const int off = (int)(((uintptr_t)to & 15) / sizeof(T));
         Chunk sc[CPG];
         if (side) load_side(sc, 0);
         for (int g = 0; g * 32 < ncols; ++g) {
@@ -288,38 +302,29 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
                 for (int i = 0; i < 2; ++i)
                     mma_chunk<T>(acc[i], wl[(g * 32 + group_column<T>(i, li)) * P + c * 4 + lg], xf[c]);
             float z[8];
-            T sv[8], out[8];
-#pragma unroll
-            for (int q = 0; q < CPG; ++q) __builtin_memcpy(sv + q * CE, &sc[q], sizeof(Chunk));
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
             if constexpr (MODE == kModeDz) act_slope(z, a.act);
             else act_fwd(z, a.act);
+            if (side) {
+                float sv[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (MODE == kModeDz) z[e] *= (float)sv[e];
-                else if (side) z[e] += (float)sv[e];
-                out[e] = (T)z[e];
+                for (int q = 0; q < CPG; ++q) unpack_chunk<T>(sc[q], sv + q * CE);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = MODE == kModeDz ? z[e] * sv[e] : z[e] + sv[e];
             }
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
                 const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                const Chunk o = pack_chunk<T>(z + q * CE);
                 if (m < a.rows && n < ncols) {
-                    T *dst = ra.store == kStoreTile ? (T *)mine + off + li * a.N + n : y + m * a.yp + n0 + n;
-                    if (n + CE <= ncols) {
-                        Chunk o;
-                        __builtin_memcpy(&o, out + q * CE, sizeof(Chunk));
-                        if (ra.store == kStoreStream) store_streaming(dst, o);
-                        else __builtin_memcpy(dst, &o, sizeof(Chunk));
-                    } else
-#pragma unroll
-                        for (int e = 0; e < CE; ++e)
-                            if (n + e < ncols) dst[e] = out[q * CE + e];
+                    if constexpr (STORE == kStoreTile) put_chunk((T *)mine + off + li * a.N + n, o, ncols - n, false);
+                    else put_chunk(y + m * a.yp + n0 + n, o, ncols - n, STORE == kStoreStream);
                 }
                 sc[q] = sn[q];
             }
         }
-        if (ra.store == kStoreTile) {
+        if constexpr (STORE == kStoreTile) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (LDS runs in the wave's order: no barrier)
             const int n = off + (int)min((int64_t)16, a.rows - t * 16) * a.N;
             const T *from = (const T *)mine;
@@ -461,22 +466,22 @@ int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
     r.range = need < fit ? need : fit;
     const int ranges = (a.N + r.range - 1) / r.range;
     size_t bytes = (size_t)r.range * row_bytes;
-    r.store = kStorePlain;
-    if (a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes) {
-        const size_t tiles = 4 * (size_t)tile_bytes<T>(a.N);
-        if (a.N * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0) r.store = kStoreStream;
-        else if (ranges == 1 && a.yp == a.N && bytes + tiles <= 2 * kRowsLds) r.store = kStoreTile, bytes += tiles;
-    }
     const int64_t want = (a.rows + 63) / 64;
     const dim3 grid((unsigned)(want < 1024 ? want : 1024), ranges);
-    const bool full = a.K == KC * 4 * kChunk<T>;
-    int rc = FSGS_OK;
-    if (bytes > 64 * 1024)
-        rc = full ? ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, true>>(bytes)
-                  : ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, false>>(bytes);
-    if (rc != FSGS_OK) return rc;
-    if (full) linear_rows_kernel<T, MODE, KC, true><<<grid, 256, bytes, s>>>(r);
-    else linear_rows_kernel<T, MODE, KC, false><<<grid, 256, bytes, s>>>(r);
+    if (a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes) {
+        if (a.N * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0) {
+            linear_rows_kernel<T, MODE, KC, kStoreStream><<<grid, 256, bytes, s>>>(r);
+            return check_launch();
+        }
+        const size_t tiled = bytes + 4 * (size_t)tile_bytes<T>(a.N);
+        if (ranges == 1 && a.yp == a.N && tiled <= 2 * kRowsLds) {
+            const int rc = ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, kStoreTile>>(tiled);
+            if (rc != FSGS_OK) return rc;
+            linear_rows_kernel<T, MODE, KC, kStoreTile><<<grid, 256, tiled, s>>>(r);
+            return check_launch();
+        }
+    }
+    linear_rows_kernel<T, MODE, KC, kStorePlain><<<grid, 256, bytes, s>>>(r);
     return check_launch();
 }
 
