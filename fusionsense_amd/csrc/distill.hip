@@ -85,14 +85,6 @@ __device__ __forceinline__ bool lanes_any(bool b) {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <typename T>
-__device__ __forceinline__ void unpack(const Chunk &c, float *v) {
-    T t[kChunk<T>];
-    __builtin_memcpy(t, &c, sizeof(Chunk));
-#pragma unroll
-    for (int e = 0; e < kChunk<T>; ++e) v[e] = (float)t[e];
-}
-
 // A row is read in chunks of 16 bytes, chunk c by lane c mod L, kStep chunks per lane at a time (all of a row that has at most
 // kStep * L chunks: lanes_per_row).  Rows start at any element.  The last chunk of a row that does not end on one is read
 // shifted back to end with the row, its doubled elements masked: no element-wise reads, nothing behind the row.
@@ -232,7 +224,7 @@ __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel
                 for (int i = 0; i < STEPS; ++i) {
                     float v[CE];
                     if constexpr (sizeof(T) == 2) forget(c[i]);
-                    unpack<T>(c[i], v);
+                    unpack_chunk<T>(c[i], v);
 #pragma unroll
                     for (int e = 0; e < CE; ++e) sum += exp2_hw(exponent(v[e]));
                 }
@@ -385,17 +377,17 @@ __global__ __launch_bounds__(256, 5) void distill_bwd_kernel(DistillArgs a) {
                 const int j = (sub + i * L) * CE;
                 if (j >= a.V || !here) break;
                 float v[CE];
-                unpack<T>(c[i], v);
-                T out[CE];
+                unpack_chunk<T>(c[i], v);
 #pragma unroll
-                for (int e = 0; e < CE; ++e) out[e] = (T)(cq * exp2_hw(exponent(v[e])));
+                for (int e = 0; e < CE; ++e) v[e] = cq * exp2_hw(exponent(v[e]));
                 if (a.V < CE) {
 #pragma unroll
                     for (int e = 0; e < CE; ++e)
-                        if (e < a.V) out_row[e] = out[e];
+                        if (e < a.V) out_row[e] = (T)v[e];
                 } else {
                     // (the last chunk of a row stores the elements before it a second time, with the same values)
-                    __builtin_memcpy(out_row + min(j, a.V - CE), out, sizeof(Chunk));
+                    const Chunk out = pack_chunk<T>(v);
+                    __builtin_memcpy(out_row + min(j, a.V - CE), &out, sizeof(Chunk));
                 }
             }
         };
@@ -483,11 +475,11 @@ __global__ __launch_bounds__(256) void distill_bwd_wide_kernel(DistillArgs a) {
                 const int j = (c0 + i * L) * CE;
                 if (j >= a.V) break;
                 float v[CE];
-                unpack<T>(c[i], v);
-                T out[CE];
+                unpack_chunk<T>(c[i], v);
 #pragma unroll
-                for (int e = 0; e < CE; ++e) out[e] = (T)(dead ? 0.f : cq * exp2_hw(x.of(v[e])));
-                __builtin_memcpy(ds + min(j, a.V - CE), out, sizeof(Chunk));
+                for (int e = 0; e < CE; ++e) v[e] = dead ? 0.f : cq * exp2_hw(x.of(v[e]));
+                const Chunk out = pack_chunk<T>(v);
+                __builtin_memcpy(ds + min(j, a.V - CE), &out, sizeof(Chunk));
             }
             c0 += kStep * L;
             if (c0 - sub >= chunks) break;
