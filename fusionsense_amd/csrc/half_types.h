@@ -89,6 +89,28 @@ __device__ __forceinline__ void mma_chunk<float>(f32x4 &acc, const Chunk &a, con
                                                    0, 0, 0);
 }
 
+// The operand of mma_chunk whose 16 rows are columns of a matrix that lies row by row in LDS (`pitch` bytes apart).
+// Half width: gfx950's transposing LDS read (16 lanes read 4 rows x 16 columns, lane i leaves with column i); the lanes of
+// group lg get the rows lo .. lo + 3 and hi .. hi + 3, columns by `col` (lane j of a group points at 4 neighbouring ones of row
+// j / 4).  fp32: plain reads, rows lo .. lo + 3.
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+template <typename T>
+__device__ __forceinline__ Chunk load_columns(const char *lds, int pitch, int lo, int hi, int col) {
+    Chunk c;
+    if constexpr (sizeof(T) == 2) {
+        const int j = threadIdx.x & 15;
+        const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds + (lo + (j >> 2)) * pitch + col * 2));
+        const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds + (hi + (j >> 2)) * pitch + col * 2));
+        __builtin_memcpy(c.u, &a, 8);
+        __builtin_memcpy(c.u + 2, &b, 8);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c.u[e] = *(const uint32_t *)(lds + (lo + e) * pitch + col * 4);
+    }
+    return c;
+}
+
 inline bool known_dtype(int d) { return d == FSGS_F32 || d == FSGS_BF16 || d == FSGS_F16; }
 
 }  // namespace fsgs

@@ -341,6 +341,199 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     }
 }
 
+// ---- backward of a layer whose two axes are both short: one pass over x and dy -----------------------------------------
+// A workgroup takes 64 rows at a time, a wave 16 of them.  Per 32 columns: z from W (LDS) and the wave's rows of x, dz =
+// dy act'(z) in fp32 registers (db is summed from these), rounded once to T and used twice: as it stands it is the B operand
+// of dx^T = W^T dz^T, and through LDS it meets x again in dW = dz^T x, whose whole [N,K] lies in the workgroup's registers for
+// the life of the workgroup.  x and dy are read once, dx is written once; W is held once, read along its rows for z and along
+// its columns for dx.
+struct BwdRowsArgs {
+    const void *x, *w, *bias, *dy;
+    void *dx;
+    float *part_w, *part_b;  // [workgroups][N*K], [workgroups][N]
+    int64_t rows, xp, dyp;
+    int K, N, act, stream;
+};
+
+// LDS: W [32 ceil(N/32)][K], dz [64][N], x [64][K], bias; pitches that keep 16 or 32 lanes on different banks.
+template <typename T>
+struct BwdRowsLds {
+    int pk, pn, w, dz, x, bias, bytes;
+    __host__ __device__ BwdRowsLds(int KC, int N) {
+        const int cols = (N + 31) / 32 * 32, pad = sizeof(T) == 2 ? 32 : 16;
+        pk = KC * 64 + pad, pn = cols * (int)sizeof(T) + pad;
+        w = 0, dz = w + cols * pk, x = dz + 64 * pn, bias = x + 64 * pk, bytes = bias + cols * 4;
+    }
+};
+
+template <typename T, int KC, int NTW>
+__global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) {
+    constexpr int CE = kChunk<T>, CPG = sizeof(T) == 2 ? 1 : 2, NG = 2 * NTW;
+    constexpr int KT = KC * 4 / (int)sizeof(T);  // 16-column tiles of K
+    extern __shared__ Chunk lds[];
+    char *const mem = (char *)lds;
+    const BwdRowsLds<T> lay(KC, a.N);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+    const int cols = (a.N + 31) / 32 * 32, ng = cols / 32;
+    float *bl = (float *)(mem + lay.bias);
+    for (int c = threadIdx.x; c < cols * KC * 4; c += 256) {
+        const int n = c / (KC * 4), k = c % (KC * 4);
+        *(Chunk *)(mem + lay.w + n * lay.pk + k * 16) =
+            load_chunk_n((const T *)a.w + (int64_t)n * a.K + k * CE, n < a.N ? a.K - k * CE : 0);
+    }
+    for (int n = threadIdx.x; n < cols; n += 256) bl[n] = a.bias && n < a.N ? (float)((const T *)a.bias)[n] : 0.f;
+    __syncthreads();
+
+    const bool full = a.K == KC * 4 * CE;
+    auto load_x = [&](Chunk (&f)[KC], int64_t m) {
+        const T *xr = (const T *)a.x + m * a.xp;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int k = (c * 4 + lg) * CE;
+            f[c] = load_chunk_n(xr + k, m < a.rows ? (full ? CE : a.K - k) : 0);
+        }
+    };
+    auto load_dy = [&](Chunk (&f)[CPG], int64_t m, int g) {
+        const T *gr = (const T *)a.dy + m * a.dyp;
+#pragma unroll
+        for (int q = 0; q < CPG; ++q) {
+            const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+            f[q] = load_chunk_n(gr + n, m < a.rows ? a.N - n : 0);
+        }
+    };
+    f32x4 accw[NTW][KT] = {};
+    float db[NG][8] = {};
+    Chunk xf[KC], dyc[NG][CPG];
+    const int64_t blocks = (a.rows + 63) / 64;
+    int64_t m = (int64_t)blockIdx.x * 64 + wave * 16 + li;
+    load_x(xf, m);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+        if (g < ng) load_dy(dyc[g], m, g);
+    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+        const int64_t next = m + (int64_t)gridDim.x * 64;
+        const int row = wave * 16 + li;
+        f32x4 accx[KT] = {};
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            if (g >= ng) break;
+            float z[8], d[8];
+            if (a.act != FSGS_ACT_NONE) {
+                f32x4 acc[2] = {};
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        mma_chunk<T>(acc[i], *(const Chunk *)(mem + lay.w + (g * 32 + group_column<T>(i, li)) * lay.pk + (c * 4 + lg) * 16),
+                                     xf[c]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
+            }
+#pragma unroll
+            for (int q = 0; q < CPG; ++q) unpack_chunk<T>(dyc[g][q], d + q * CE);
+            load_dy(dyc[g], next, g);
+            if (a.act != FSGS_ACT_NONE) {
+                act_slope(z, a.act);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] *= z[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) db[g][e] += d[e];
+            Chunk dzc[CPG];
+#pragma unroll
+            for (int q = 0; q < CPG; ++q) {
+                dzc[q] = pack_chunk<T>(d + q * CE);
+                *(Chunk *)(mem + lay.dz + row * lay.pn + (g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4)) * (int)sizeof(T)) = dzc[q];
+            }
+            if (a.dx) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int q = 0; q < CPG; ++q) {
+                        // rows k of the tile: by pairs of tiles 8 neighbours per lane in half width, 4 in fp32
+                        const int col = CPG == 1 ? (kt >> 1) * 32 + (li & 3) * 8 + (kt & 1) * 4 : kt * 16 + li;
+                        const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                        mma_chunk<T>(accx[kt], load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col), dzc[q]);
+                    }
+            }
+        }
+        if (a.dx && m < a.rows) {
+            T *dst = (T *)a.dx + m * a.K;
+#pragma unroll
+            for (int kt = 0; kt < KT; kt += 3 - CPG) {
+                const int k = kt * 16 + lg * CE;
+                float v[CE];
+#pragma unroll
+                for (int e = 0; e < CE; ++e) v[e] = accx[kt + (e >> 2)][e & 3];
+                if (k < a.K) put_chunk(dst + k, pack_chunk<T>(v), a.K - k, a.stream);
+            }
+        }
+        if (a.part_w) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) *(Chunk *)(mem + lay.x + row * lay.pk + (c * 4 + lg) * 16) = xf[c];
+        }
+        m = next;
+        load_x(xf, m);
+        if (a.part_w) {
+            __syncthreads();
+            constexpr int STEP = 4 * CE;  // rows per matrix instruction: 32, or 16 by four instructions
+#pragma unroll
+            for (int s = 0; s < 64 / STEP; ++s) {
+                const int lo = s * STEP + lg * 4, hi = lo + 16;
+                Chunk xc[KT];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+                    xc[kt] = load_columns<T>(mem + lay.x, lay.pk, lo, hi, kt * 16 + (CPG == 1 ? (li & 3) * 4 : li));
+#pragma unroll
+                for (int i = 0; i < NTW; ++i) {
+                    const int n = (i * 4 + wave) * 16;
+                    if (n >= cols) break;
+                    const Chunk zc = load_columns<T>(mem + lay.dz, lay.pn, lo, hi, n + (CPG == 1 ? (li & 3) * 4 : li));
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) mma_chunk<T>(accw[i][kt], zc, xc[kt]);
+                }
+            }
+            __syncthreads();
+        }
+    }
+    if (a.part_w) {
+        float *pw = a.part_w + (int64_t)blockIdx.x * a.N * a.K;
+#pragma unroll
+        for (int i = 0; i < NTW; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = (i * 4 + wave) * 16 + lg * 4 + q;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int k = kt * 16 + li;
+                    if (n < a.N && k < a.K) pw[(int64_t)n * a.K + k] = accw[i][kt][q];
+                }
+            }
+    }
+    if (a.part_b) {
+        float *wb = (float *)(mem + lay.dz) + wave * cols;  // (the tiles are done with: every wave is behind its last barrier)
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            if (g >= ng) break;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float v = db[g][e];
+                v += dpp_f<0xB1>(v);
+                v += dpp_f<0x4E>(v);
+                v += dpp_f<0x141>(v);
+                v += dpp_f<0x140>(v);  // over the 16 rows of the wave
+                if (li == 0) wb[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))] = v;
+            }
+        }
+        __syncthreads();
+        const float *all = (const float *)(mem + lay.dz);
+        for (int n = threadIdx.x; n < a.N; n += 256)
+            a.part_b[(int64_t)blockIdx.x * a.N + n] = (all[n] + all[cols + n]) + (all[2 * cols + n] + all[3 * cols + n]);
+    }
+}
+
 // W [N,K] -> W^T [K,N]: the operand of dx = dz W with its summed axis contiguous.
 template <typename T>
 __global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w, T *__restrict__ wt, int N, int K) {
@@ -434,22 +627,35 @@ __global__ __launch_bounds__(256) void linear_dw_kernel(DwArgs a) {
         }
 }
 
-// Sum of the slices' partial gradients, in the slices' order.
+// Sum of the slices' partial gradients: 64 neighbouring values per workgroup, 16 threads take every 16th slice of a value, in
+// an order that the sizes alone fix.  Values behind N*K are those of db.
 template <typename T>
-__global__ __launch_bounds__(256) void reduce_slices_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b,
-                                                            T *__restrict__ dw, T *__restrict__ db, int64_t nk, int N,
-                                                            int slices) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < nk) {
-        if (!dw) return;
-        float s = 0.f;
-        for (int t = 0; t < slices; ++t) s += part_w[t * nk + i];
-        dw[i] = (T)s;
-    } else if (db && i - nk < N) {
-        float s = 0.f;
-        for (int t = 0; t < slices; ++t) s += part_b[(int64_t)t * N + (i - nk)];
-        db[i - nk] = (T)s;
+__global__ __launch_bounds__(1024) void reduce_slices_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b,
+                                                             T *__restrict__ dw, T *__restrict__ db, int64_t nk, int N,
+                                                             int slices) {
+    __shared__ float part[16][64];
+    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
+    const int64_t i = (int64_t)blockIdx.x * 64 + c;
+    const bool w = i < nk && dw, b = i >= nk && i < nk + N && db;
+    const float *from = w ? part_w + i : b ? part_b + (i - nk) : nullptr;
+    const int64_t pitch = w ? nk : N;
+    float s = 0.f;
+    if (from)
+        for (int t = r; t < slices; t += 16) s += from[t * pitch];
+    part[r][c] = s;
+    __syncthreads();
+    if (r == 0 && from) {
+        for (int t = 1; t < 16; ++t) s += part[t][c];
+        if (w) dw[i] = (T)s;
+        else db[i - nk] = (T)s;
     }
+}
+
+template <typename T>
+int launch_reduce(const float *part_w, const float *part_b, void *dw, void *db, int K, int N, int slices, hipStream_t s) {
+    const int64_t nk = (int64_t)N * K;
+    reduce_slices_kernel<T><<<(unsigned)((nk + N + 63) / 64), 1024, 0, s>>>(part_w, part_b, (T *)dw, (T *)db, nk, N, slices);
+    return check_launch();
 }
 
 // LDS of a workgroup of the rows kernel: weights up to 40 KB, four workgroups per CU; with the waves' output tiles up to 80 KB.
@@ -516,6 +722,65 @@ int dw_slices(int64_t rows, int K, int N) {
     return (int)(s < 1 ? 1 : s);
 }
 
+// The one-pass backward takes a layer whose weights, and the tiles of 64 rows, fit LDS, and whose dW fits a workgroup's
+// registers (NTW tiles of 16 columns of dz per wave, KT of x: at most 64 accumulators a lane).  Two workgroups per CU up to
+// 80 KB of LDS, one beyond.
+struct BwdRowsPlan {
+    int kc, ntw, bytes, blocks;  // kc == 0: the layer is too wide
+};
+
+template <typename T>
+BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N) {
+    BwdRowsPlan p = {0, 0, 0, 0};
+    const int row = K * (int)sizeof(T), kt = sizeof(T) == 2 ? 2 : 1;
+    if (row > 512 || N > 256) return p;
+    const int kc = row <= 64 ? 1 : row <= 128 ? 2 : row <= 256 ? 4 : 8;
+    const int ntw = N <= 64 ? 1 : N <= 128 ? 2 : N <= 192 ? 3 : 4;
+    if (ntw * kc * kt * 4 > 64) return p;
+    p.bytes = BwdRowsLds<T>(kc, N).bytes;
+    if (p.bytes > 160 * 1024) return p;
+    p.kc = kc, p.ntw = ntw;
+    const int64_t want = (rows + 63) / 64, most = p.bytes <= 80 * 1024 ? 512 : 256;
+    p.blocks = (int)(want < most ? want : most);
+    return p;
+}
+
+BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N, size_t e) {
+    return e == 4 ? bwd_rows_plan<float>(rows, K, N) : bwd_rows_plan<__bf16>(rows, K, N);
+}
+
+template <typename T, int KC, int NTW>
+int launch_bwd_rows(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
+    if constexpr (NTW * KC * (sizeof(T) == 2 ? 2 : 1) * 4 <= 64) {
+        const int rc = ensure_dynamic_lds<linear_bwd_rows_kernel<T, KC, NTW>>(p.bytes);
+        if (rc != FSGS_OK) return rc;
+        linear_bwd_rows_kernel<T, KC, NTW><<<p.blocks, 256, p.bytes, s>>>(a);
+        return check_launch();
+    } else {
+        return FSGS_EINVAL;
+    }
+}
+
+template <typename T, int KC>
+int launch_bwd_rows_n(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
+    switch (p.ntw) {
+        case 1: return launch_bwd_rows<T, KC, 1>(a, p, s);
+        case 2: return launch_bwd_rows<T, KC, 2>(a, p, s);
+        case 3: return launch_bwd_rows<T, KC, 3>(a, p, s);
+        default: return launch_bwd_rows<T, KC, 4>(a, p, s);
+    }
+}
+
+template <typename T>
+int launch_bwd_rows_k(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
+    switch (p.kc) {
+        case 1: return launch_bwd_rows_n<T, 1>(a, p, s);
+        case 2: return launch_bwd_rows_n<T, 2>(a, p, s);
+        case 4: return launch_bwd_rows_n<T, 4>(a, p, s);
+        default: return launch_bwd_rows_n<T, 8>(a, p, s);
+    }
+}
+
 struct BwdScratch {
     size_t dz, wt, part_w, part_b, total;
 };
@@ -523,6 +788,13 @@ struct BwdScratch {
 BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bool dw, bool db) {
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     BwdScratch l;
+    const BwdRowsPlan p = bwd_rows_plan(rows, K, N, e);
+    if (p.kc) {
+        l.dz = l.wt = l.part_w = 0;
+        l.part_b = dw ? up((size_t)p.blocks * K * N * 4) : 0;
+        l.total = l.part_b + (db ? up((size_t)p.blocks * N * 4) : 0);
+        return l;
+    }
     const size_t s = (size_t)dw_slices(rows, K, N);
     l.dz = 0;
     l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
@@ -534,6 +806,18 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
 
 template <typename T>
 int run_bwd(LinArgs a, void *dx, void *dw, void *db, char *scratch, const BwdScratch &l, hipStream_t s) {
+    const BwdRowsPlan p = bwd_rows_plan<T>(a.rows, a.K, a.N);
+    if (p.kc) {
+        BwdRowsArgs b = {};
+        b.x = a.x, b.xp = a.xp, b.w = a.w, b.bias = a.bias, b.dy = a.dy, b.dyp = a.dyp, b.dx = dx;
+        b.rows = a.rows, b.K = a.K, b.N = a.N, b.act = a.act;
+        b.part_w = dw ? (float *)(scratch + l.part_w) : nullptr;
+        b.part_b = db ? (float *)(scratch + l.part_b) : nullptr;
+        b.stream = a.rows * a.K * (int64_t)sizeof(T) >= kStreamBytes && a.K * sizeof(T) % 64 == 0 && (uintptr_t)dx % 64 == 0;
+        const int rc = launch_bwd_rows_k<T>(b, p, s);
+        if (rc != FSGS_OK || (!dw && !db)) return rc;
+        return launch_reduce<T>(b.part_w, b.part_b, dw, db, a.K, a.N, p.blocks, s);
+    }
     const void *dz = a.dy;
     int64_t dzp = a.dyp;
     if (a.act != FSGS_ACT_NONE) {
@@ -566,10 +850,7 @@ int run_bwd(LinArgs a, void *dx, void *dw, void *db, char *scratch, const BwdScr
         linear_dw_kernel<T><<<dim3(kt, (a.N + 63) / 64, slices), 256, 0, s>>>(d);
         int rc = check_launch();
         if (rc != FSGS_OK) return rc;
-        const int64_t nk = (int64_t)a.N * a.K;
-        reduce_slices_kernel<T><<<(unsigned)((nk + a.N + 255) / 256), 256, 0, s>>>(d.part_w, d.part_b, (T *)dw, (T *)db, nk,
-                                                                                  a.N, slices);
-        return check_launch();
+        return launch_reduce<T>(d.part_w, d.part_b, dw, db, a.K, a.N, slices, s);
     }
     return FSGS_OK;
 }
