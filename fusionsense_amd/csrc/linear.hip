@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
 }
 
 // ---- backward of a layer whose two axes are both short: one pass over x and dy -----------------------------------------
-// A workgroup takes 64 rows at a time, a wave 16 of them.  Per 32 columns: z from W (LDS) and the wave's rows of x, dz =
+// A workgroup of eight waves takes 128 rows at a time, a wave 16 of them.  Per 32 columns: z from W (LDS) and the wave's rows of x, dz =
 // dy act'(z) in fp32 registers (db is summed from these), rounded once to T and used twice: as it stands it is the B operand
 // of dx^T = W^T dz^T, and through LDS it meets x again in dW = dz^T x, whose whole [N,K] lies in the workgroup's registers for
 // the life of the workgroup.  x and dy are read once, dx is written once; W is held once, read along its rows for z and along
@@ -355,20 +355,24 @@ struct BwdRowsArgs {
     int K, N, act, stream;
 };
 
-// LDS: W [32 ceil(N/32)][K], dz [64][N], x [64][K], bias; pitches that keep 16 or 32 lanes on different banks.
+constexpr int kBwdWaves = 8, kBwdRows = 16 * kBwdWaves;
+
+// LDS: W [32 ceil(N/32)][K], dz [128][N], x [128][K], bias; pitches that keep 16 or 32 lanes on different banks.
 template <typename T>
 struct BwdRowsLds {
     int pk, pn, w, dz, x, bias, bytes;
     __host__ __device__ BwdRowsLds(int KC, int N) {
         const int cols = (N + 31) / 32 * 32, pad = sizeof(T) == 2 ? 32 : 16;
         pk = KC * 64 + pad, pn = cols * (int)sizeof(T) + pad;
-        w = 0, dz = w + cols * pk, x = dz + 64 * pn, bias = x + 64 * pk, bytes = bias + cols * 4;
+        w = 0, dz = w + cols * pk, x = dz + kBwdRows * pn, bias = x + kBwdRows * pk, bytes = bias + cols * 4;
     }
 };
 
-template <typename T, int KC, int NTW>
-__global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) {
-    constexpr int CE = kChunk<T>, CPG = sizeof(T) == 2 ? 1 : 2, NG = 2 * NTW;
+// NG: groups of 32 columns that the registers provide for.
+template <typename T, int KC, int NG>
+__global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) {
+    constexpr int CE = kChunk<T>, CPG = sizeof(T) == 2 ? 1 : 2;
+    constexpr int NTW = (2 * NG + kBwdWaves - 1) / kBwdWaves;  // 16-column tiles of dW's other axis per wave
     constexpr int KT = KC * 4 / (int)sizeof(T);  // 16-column tiles of K
     extern __shared__ Chunk lds[];
     char *const mem = (char *)lds;
@@ -376,12 +380,12 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
     const int cols = (a.N + 31) / 32 * 32, ng = cols / 32;
     float *bl = (float *)(mem + lay.bias);
-    for (int c = threadIdx.x; c < cols * KC * 4; c += 256) {
+    for (int c = threadIdx.x; c < cols * KC * 4; c += 64 * kBwdWaves) {
         const int n = c / (KC * 4), k = c % (KC * 4);
         *(Chunk *)(mem + lay.w + n * lay.pk + k * 16) =
             load_chunk_n((const T *)a.w + (int64_t)n * a.K + k * CE, n < a.N ? a.K - k * CE : 0);
     }
-    for (int n = threadIdx.x; n < cols; n += 256) bl[n] = a.bias && n < a.N ? (float)((const T *)a.bias)[n] : 0.f;
+    for (int n = threadIdx.x; n < cols; n += 64 * kBwdWaves) bl[n] = a.bias && n < a.N ? (float)((const T *)a.bias)[n] : 0.f;
     __syncthreads();
 
     const bool full = a.K == KC * 4 * CE;
@@ -402,16 +406,19 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
         }
     };
     f32x4 accw[NTW][KT] = {};
-    float db[NG][8] = {};
+    constexpr bool kRegDb = sizeof(T) == 2;
+    float db[kRegDb ? NG : 1][8] = {};
+    f32x4 accb[kRegDb ? 1 : NTW] = {};
+    const bool tiles = a.part_w || (!kRegDb && a.part_b);
     Chunk xf[KC], dyc[NG][CPG];
-    const int64_t blocks = (a.rows + 63) / 64;
-    int64_t m = (int64_t)blockIdx.x * 64 + wave * 16 + li;
+    const int64_t blocks = (a.rows + kBwdRows - 1) / kBwdRows;
+    int64_t m = (int64_t)blockIdx.x * kBwdRows + wave * 16 + li;
     load_x(xf, m);
 #pragma unroll
     for (int g = 0; g < NG; ++g)
         if (g < ng) load_dy(dyc[g], m, g);
     for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-        const int64_t next = m + (int64_t)gridDim.x * 64;
+        const int64_t next = m + (int64_t)gridDim.x * kBwdRows;
         const int row = wave * 16 + li;
         f32x4 accx[KT] = {};
 #pragma unroll
@@ -438,8 +445,9 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] *= z[e];
             }
+            if constexpr (kRegDb)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) db[g][e] += d[e];
+                for (int e = 0; e < 8; ++e) db[g][e] += d[e];
             Chunk dzc[CPG];
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
@@ -475,11 +483,11 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
         }
         m = next;
         load_x(xf, m);
-        if (a.part_w) {
+        if (tiles) {
             __syncthreads();
             constexpr int STEP = 4 * CE;  // rows per matrix instruction: 32, or 16 by four instructions
 #pragma unroll
-            for (int s = 0; s < 64 / STEP; ++s) {
+            for (int s = 0; s < kBwdRows / STEP; ++s) {
                 const int lo = s * STEP + lg * 4, hi = lo + 16;
                 Chunk xc[KT];
 #pragma unroll
@@ -487,9 +495,10 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
                     xc[kt] = load_columns<T>(mem + lay.x, lay.pk, lo, hi, kt * 16 + (CPG == 1 ? (li & 3) * 4 : li));
 #pragma unroll
                 for (int i = 0; i < NTW; ++i) {
-                    const int n = (i * 4 + wave) * 16;
+                    const int n = (i * kBwdWaves + wave) * 16;
                     if (n >= cols) break;
                     const Chunk zc = load_columns<T>(mem + lay.dz, lay.pn, lo, hi, n + (CPG == 1 ? (li & 3) * 4 : li));
+                    if constexpr (!kRegDb) mma_chunk<T>(accb[i], zc, Chunk{{0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u}});
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt) mma_chunk<T>(accw[i][kt], zc, xc[kt]);
                 }
@@ -503,7 +512,7 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
         for (int i = 0; i < NTW; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int n = (i * 4 + wave) * 16 + lg * 4 + q;
+                const int n = (i * kBwdWaves + wave) * 16 + lg * 4 + q;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
                     const int k = kt * 16 + li;
@@ -511,7 +520,16 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
                 }
             }
     }
-    if (a.part_b) {
+    if constexpr (!kRegDb) {
+        if (a.part_b && li == 0)
+#pragma unroll
+            for (int i = 0; i < NTW; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int n = (i * kBwdWaves + wave) * 16 + lg * 4 + q;
+                    if (n < a.N) a.part_b[(int64_t)blockIdx.x * a.N + n] = accb[i][q];
+                }
+    } else if (a.part_b) {
         float *wb = (float *)(mem + lay.dz) + wave * cols;  // (the tiles are done with: every wave is behind its last barrier)
         __syncthreads();
 #pragma unroll
@@ -529,8 +547,12 @@ __global__ __launch_bounds__(256, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) 
         }
         __syncthreads();
         const float *all = (const float *)(mem + lay.dz);
-        for (int n = threadIdx.x; n < a.N; n += 256)
-            a.part_b[(int64_t)blockIdx.x * a.N + n] = (all[n] + all[cols + n]) + (all[2 * cols + n] + all[3 * cols + n]);
+        for (int n = threadIdx.x; n < a.N; n += 64 * kBwdWaves)
+{
+            float v = 0.f;
+            for (int w = 0; w < kBwdWaves; ++w) v += all[w * cols + n];
+            a.part_b[(int64_t)blockIdx.x * a.N + n] = v;
+        }
     }
 }
 
@@ -722,26 +744,29 @@ int dw_slices(int64_t rows, int K, int N) {
     return (int)(s < 1 ? 1 : s);
 }
 
-// The one-pass backward takes a layer whose weights, and the tiles of 64 rows, fit LDS, and whose dW fits a workgroup's
-// registers (NTW tiles of 16 columns of dz per wave, KT of x: at most 64 accumulators a lane).  Two workgroups per CU up to
-// 80 KB of LDS, one beyond.
+// The one-pass backward takes a layer whose weights, and the tiles of 128 rows, fit LDS, and whose accumulators (dW, dx, db)
+// and rows under way fit 256 registers with something left for the work on them.
 struct BwdRowsPlan {
-    int kc, ntw, bytes, blocks;  // kc == 0: the layer is too wide
+    int kc, ng, bytes, blocks;  // kc == 0: the layer is too wide
 };
+
+template <typename T>
+constexpr bool bwd_rows_fits(int kc, int ng) {
+    const int kt = kc * 4 / (int)sizeof(T), ntw = (2 * ng + kBwdWaves - 1) / kBwdWaves;
+    return ntw * kt * 4 + kt * 4 + ng * (sizeof(T) == 2 ? 12 : 8) + kc * 4 <= 144;
+}
 
 template <typename T>
 BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N) {
     BwdRowsPlan p = {0, 0, 0, 0};
-    const int row = K * (int)sizeof(T), kt = sizeof(T) == 2 ? 2 : 1;
+    const int row = K * (int)sizeof(T);
     if (row > 512 || N > 256) return p;
-    const int kc = row <= 64 ? 1 : row <= 128 ? 2 : row <= 256 ? 4 : 8;
-    const int ntw = N <= 64 ? 1 : N <= 128 ? 2 : N <= 192 ? 3 : 4;
-    if (ntw * kc * kt * 4 > 64) return p;
+    const int kc = row <= 64 ? 1 : row <= 128 ? 2 : row <= 256 ? 4 : 8, ng = (N + 63) / 64 * 2;
     p.bytes = BwdRowsLds<T>(kc, N).bytes;
-    if (p.bytes > 160 * 1024) return p;
-    p.kc = kc, p.ntw = ntw;
-    const int64_t want = (rows + 63) / 64, most = p.bytes <= 80 * 1024 ? 512 : 256;
-    p.blocks = (int)(want < most ? want : most);
+    if (!bwd_rows_fits<T>(kc, ng) || p.bytes > 160 * 1024) return p;
+    p.kc = kc, p.ng = ng;
+    const int64_t want = (rows + kBwdRows - 1) / kBwdRows;
+    p.blocks = (int)(want < 256 ? want : 256);
     return p;
 }
 
@@ -749,12 +774,12 @@ BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N, size_t e) {
     return e == 4 ? bwd_rows_plan<float>(rows, K, N) : bwd_rows_plan<__bf16>(rows, K, N);
 }
 
-template <typename T, int KC, int NTW>
+template <typename T, int KC, int NG>
 int launch_bwd_rows(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
-    if constexpr (NTW * KC * (sizeof(T) == 2 ? 2 : 1) * 4 <= 64) {
-        const int rc = ensure_dynamic_lds<linear_bwd_rows_kernel<T, KC, NTW>>(p.bytes);
+    if constexpr (bwd_rows_fits<T>(KC, NG)) {
+        const int rc = ensure_dynamic_lds<linear_bwd_rows_kernel<T, KC, NG>>(p.bytes);
         if (rc != FSGS_OK) return rc;
-        linear_bwd_rows_kernel<T, KC, NTW><<<p.blocks, 256, p.bytes, s>>>(a);
+        linear_bwd_rows_kernel<T, KC, NG><<<p.blocks, 64 * kBwdWaves, p.bytes, s>>>(a);
         return check_launch();
     } else {
         return FSGS_EINVAL;
@@ -763,11 +788,11 @@ int launch_bwd_rows(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
 
 template <typename T, int KC>
 int launch_bwd_rows_n(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
-    switch (p.ntw) {
-        case 1: return launch_bwd_rows<T, KC, 1>(a, p, s);
+    switch (p.ng) {
         case 2: return launch_bwd_rows<T, KC, 2>(a, p, s);
-        case 3: return launch_bwd_rows<T, KC, 3>(a, p, s);
-        default: return launch_bwd_rows<T, KC, 4>(a, p, s);
+        case 4: return launch_bwd_rows<T, KC, 4>(a, p, s);
+        case 6: return launch_bwd_rows<T, KC, 6>(a, p, s);
+        default: return launch_bwd_rows<T, KC, 8>(a, p, s);
     }
 }
 
