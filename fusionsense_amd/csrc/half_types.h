@@ -37,6 +37,39 @@ __device__ __forceinline__ Chunk load_chunk_n(const T *p, int n) {
     return c;
 }
 
+// Rows of a matrix read in chunks that need not end with the row: raw() reads 16 bytes wherever they start (held back only at
+// the matrix' last element, so nothing outside it is read) and has no branch, so it can be under way long before it is used;
+// fix() then moves what was held back to its place and zeroes what lies behind `valid` elements.
+template <typename T>
+struct RowReader {
+    const T *p;
+    int64_t pitch, lim;  // lim: the last element a chunk may start at
+    __device__ RowReader(const void *base, int64_t rows, int64_t pitch_, int width)
+        : p((const T *)base), pitch(pitch_), lim((rows - 1) * pitch_ + width - kChunk<T>) {}
+    __device__ __forceinline__ Chunk raw(int64_t at) const { return load_chunk(p + min(at, lim)); }
+    // may_end: some lane's chunk may reach the matrix' end (the same for the whole wave)
+    __device__ __forceinline__ void fix(Chunk &c, int64_t at, int valid, bool may_end) const {
+        constexpr int CE = kChunk<T>;
+        if (may_end) {
+            const int s = at > lim ? (int)min(at - lim, (int64_t)(CE - 1)) : 0;
+            if (s & (CE / 2)) c.u[0] = c.u[2], c.u[1] = c.u[3], c.u[2] = c.u[3] = 0;
+            if (s & (CE / 4)) c.u[0] = c.u[1], c.u[1] = c.u[2], c.u[2] = c.u[3], c.u[3] = 0;
+            if (sizeof(T) == 2 && (s & 1)) {
+                c.u[0] = c.u[0] >> 16 | c.u[1] << 16, c.u[1] = c.u[1] >> 16 | c.u[2] << 16;
+                c.u[2] = c.u[2] >> 16 | c.u[3] << 16, c.u[3] >>= 16;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int left = valid - i * (CE / 4);
+            if constexpr (sizeof(T) == 2) c.u[i] = left >= 2 ? c.u[i] : left == 1 ? c.u[i] & 0xffffu : 0;
+            else c.u[i] = left >= 1 ? c.u[i] : 0;
+        }
+    }
+};
+template <typename T>
+inline bool row_reader_fits(int64_t rows, int64_t pitch, int width) { return (rows - 1) * pitch + width >= kChunk<T>; }
+
 // kChunk floats rounded (to nearest, ties to even) to a chunk: two per instruction in the half-width types.
 template <typename T>
 __device__ __forceinline__ Chunk pack_chunk(const float *v) {

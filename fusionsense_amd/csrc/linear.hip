@@ -81,6 +81,10 @@ __device__ __forceinline__ void act_slope(float (&z)[N], int act) {
     }
 }
 
+// A chunk that starts inside a row reaches behind the matrix only in its last 8 rows (rows at least one element apart) or
+// where all rows are one.
+constexpr int kEndRows = 8;
+
 enum { kModeFwd = 0, kModeDz = 1 };
 
 // Tile of 128 rows x BN columns, four waves of 64 x BN/2.  Both operands go through LDS in 128-byte slabs of the summed
@@ -268,33 +272,49 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     __syncthreads();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
     char *mine = (char *)(bl + ra.range) + wave * tile_bytes<T>(a.N);  // (kStoreTile)
-    const bool full = a.K == KC * 4 * CE;
     constexpr int CPG = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of a row that a lane holds of a group
-    const T *side = (const T *)(MODE == kModeDz ? a.dy : a.res);
-    const int64_t sp = MODE == kModeDz ? a.dyp : a.rp;
+    const RowReader<T> xr(a.x, a.rows, a.xp, a.K);
+    const bool has_side = MODE == kModeDz || a.res;
+    const RowReader<T> sr(MODE == kModeDz ? a.dy : a.res, a.rows, MODE == kModeDz ? a.dyp : a.rp, a.N);
+    const bool ragged_x = a.K != KC * 4 * CE, ragged_n = ncols % 32 != 0;
     const int64_t tiles = (a.rows + 15) / 16, step = (int64_t)gridDim.x * 4;
-    for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < tiles; t += step) {
+    auto column = [&](int g, int q) { return g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4); };
+    auto load_x = [&](Chunk (&f)[KC], int64_t row) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) f[c] = xr.raw(row * a.xp + (c * 4 + lg) * CE);
+    };
+    auto load_side = [&](Chunk (&f)[CPG], int64_t row, int g) {
+#pragma unroll
+        for (int q = 0; q < CPG; ++q) f[q] = sr.raw(row * sr.pitch + n0 + column(g, q));
+    };
+    int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    // the next tile's rows, and of the side input the next group, are under way while this one is worked on
+    Chunk xn[KC], sn[CPG];
+    if (t < tiles) {
+        load_x(xn, min(t * 16 + li, a.rows - 1));
+        if (has_side) load_side(sn, min(t * 16 + li, a.rows - 1), 0);
+    }
+    for (; t < tiles; t += step) {
         const int64_t m = t * 16 + li, mr = min(m, a.rows - 1);  // (lanes behind the last row repeat it and store nothing)
+        const int64_t mn = min((t + step) * 16 + li, a.rows - 1);
+        const bool end = (t + 1) * 16 + kEndRows >= a.rows;
         Chunk xf[KC];
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int k = (c * 4 + lg) * CE;
-            xf[c] = full ? load_chunk(x + mr * a.xp + k) : load_chunk_n(x + mr * a.xp + k, a.K - k);
-        }
-        auto load_side = [&](Chunk (&s)[CPG], int g) {
+        for (int c = 0; c < KC; ++c) xf[c] = xn[c];
+        load_x(xn, mn);
+        if (ragged_x)
 #pragma unroll
-            for (int q = 0; q < CPG; ++q) {
-                const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
-                s[q] = load_chunk_n(side + mr * sp + n0 + n, ncols - n);
-            }
-        };
+            for (int c = 0; c < KC; ++c) xr.fix(xf[c], mr * a.xp + (c * 4 + lg) * CE, a.K - (c * 4 + lg) * CE, end || a.xp == 0);
         T *to = y + t * 16 * a.yp;  // (kStoreTile: yp == N, one range)
         const int off = (int)(((uintptr_t)to & 15) / sizeof(T));
-        Chunk sc[CPG];
-        if (side) load_side(sc, 0);
         for (int g = 0; g * 32 < ncols; ++g) {
-            Chunk sn[CPG];
-            if (side && (g + 1) * 32 < ncols) load_side(sn, g + 1);
+            Chunk sc[CPG];
+#pragma unroll
+            for (int q = 0; q < CPG; ++q) sc[q] = sn[q];
+            if (has_side) {
+                const bool more = (g + 1) * 32 < ncols;
+                load_side(sn, more ? mr : mn, more ? g + 1 : 0);
+            }
             f32x4 acc[2] = {};
 #pragma unroll
             for (int c = 0; c < KC; ++c)
@@ -306,22 +326,24 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
             for (int e = 0; e < 8; ++e) z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
             if constexpr (MODE == kModeDz) act_slope(z, a.act);
             else act_fwd(z, a.act);
-            if (side) {
+            if (has_side) {
                 float sv[8];
 #pragma unroll
-                for (int q = 0; q < CPG; ++q) unpack_chunk<T>(sc[q], sv + q * CE);
+                for (int q = 0; q < CPG; ++q) {
+                    if (ragged_n) sr.fix(sc[q], mr * sr.pitch + n0 + column(g, q), ncols - column(g, q), end || sr.pitch == 0);
+                    unpack_chunk<T>(sc[q], sv + q * CE);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) z[e] = MODE == kModeDz ? z[e] * sv[e] : z[e] + sv[e];
             }
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
-                const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                const int n = column(g, q);
                 const Chunk o = pack_chunk<T>(z + q * CE);
                 if (m < a.rows && n < ncols) {
                     if constexpr (STORE == kStoreTile) put_chunk((T *)mine + off + li * a.N + n, o, ncols - n, false);
                     else put_chunk(y + m * a.yp + n0 + n, o, ncols - n, STORE == kStoreStream);
                 }
-                sc[q] = sn[q];
             }
         }
         if constexpr (STORE == kStoreTile) {
@@ -388,38 +410,38 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
     for (int n = threadIdx.x; n < cols; n += 64 * kBwdWaves) bl[n] = a.bias && n < a.N ? (float)((const T *)a.bias)[n] : 0.f;
     __syncthreads();
 
-    const bool full = a.K == KC * 4 * CE;
-    auto load_x = [&](Chunk (&f)[KC], int64_t m) {
-        const T *xr = (const T *)a.x + m * a.xp;
+    const RowReader<T> xr(a.x, a.rows, a.xp, a.K), gr(a.dy, a.rows, a.dyp, a.N);
+    const bool ragged_x = a.K != KC * 4 * CE, ragged_n = a.N % 32 != 0;
+    auto column = [&](int g, int q) { return g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4); };
+    auto load_x = [&](Chunk (&f)[KC], int64_t row) {
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int k = (c * 4 + lg) * CE;
-            f[c] = load_chunk_n(xr + k, m < a.rows ? (full ? CE : a.K - k) : 0);
-        }
+        for (int c = 0; c < KC; ++c) f[c] = xr.raw(row * a.xp + (c * 4 + lg) * CE);
     };
-    auto load_dy = [&](Chunk (&f)[CPG], int64_t m, int g) {
-        const T *gr = (const T *)a.dy + m * a.dyp;
+    auto load_dy = [&](Chunk (&f)[CPG], int64_t row, int g) {
 #pragma unroll
-        for (int q = 0; q < CPG; ++q) {
-            const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
-            f[q] = load_chunk_n(gr + n, m < a.rows ? a.N - n : 0);
-        }
+        for (int q = 0; q < CPG; ++q) f[q] = gr.raw(row * a.dyp + column(g, q));
     };
     f32x4 accw[NTW][KT] = {};
     constexpr bool kRegDb = sizeof(T) == 2;
     float db[kRegDb ? NG : 1][8] = {};
-    f32x4 accb[kRegDb ? 1 : NTW] = {};
+    float accb[kRegDb ? 1 : NTW] = {};
     const bool tiles = a.part_w || (!kRegDb && a.part_b);
     Chunk xf[KC], dyc[NG][CPG];
     const int64_t blocks = (a.rows + kBwdRows - 1) / kBwdRows;
     int64_t m = (int64_t)blockIdx.x * kBwdRows + wave * 16 + li;
-    load_x(xf, m);
+    load_x(xf, min(m, a.rows - 1));
 #pragma unroll
     for (int g = 0; g < NG; ++g)
-        if (g < ng) load_dy(dyc[g], m, g);
+        if (g < ng) load_dy(dyc[g], min(m, a.rows - 1), g);
     for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
         const int64_t next = m + (int64_t)gridDim.x * kBwdRows;
         const int row = wave * 16 + li;
+        const int64_t mr = min(m, a.rows - 1), nr = min(next, a.rows - 1);
+        const bool end = (blk + 1) * kBwdRows + kEndRows >= a.rows;
+        if (ragged_x || end)
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+                xr.fix(xf[c], mr * a.xp + (c * 4 + lg) * CE, m < a.rows ? a.K - (c * 4 + lg) * CE : 0, end || a.xp == 0);
         f32x4 accx[KT] = {};
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -437,9 +459,13 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                 for (int e = 0; e < 8; ++e)
                     z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
             }
+            if (ragged_n || end)
+#pragma unroll
+                for (int q = 0; q < CPG; ++q)
+                    gr.fix(dyc[g][q], mr * a.dyp + column(g, q), m < a.rows ? a.N - column(g, q) : 0, end || a.dyp == 0);
 #pragma unroll
             for (int q = 0; q < CPG; ++q) unpack_chunk<T>(dyc[g][q], d + q * CE);
-            load_dy(dyc[g], next, g);
+            load_dy(dyc[g], nr, g);
             if (a.act != FSGS_ACT_NONE) {
                 act_slope(z, a.act);
 #pragma unroll
@@ -452,7 +478,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
                 dzc[q] = pack_chunk<T>(d + q * CE);
-                *(Chunk *)(mem + lay.dz + row * lay.pn + (g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4)) * (int)sizeof(T)) = dzc[q];
+                *(Chunk *)(mem + lay.dz + row * lay.pn + column(g, q) * (int)sizeof(T)) = dzc[q];
             }
             if (a.dx) {
 #pragma unroll
@@ -461,7 +487,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                     for (int q = 0; q < CPG; ++q) {
                         // rows k of the tile: by pairs of tiles 8 neighbours per lane in half width, 4 in fp32
                         const int col = CPG == 1 ? (kt >> 1) * 32 + (li & 3) * 8 + (kt & 1) * 4 : kt * 16 + li;
-                        const int n = g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                        const int n = column(g, q);
                         mma_chunk<T>(accx[kt], load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col), dzc[q]);
                     }
             }
@@ -482,7 +508,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
             for (int c = 0; c < KC; ++c) *(Chunk *)(mem + lay.x + row * lay.pk + (c * 4 + lg) * 16) = xf[c];
         }
         m = next;
-        load_x(xf, m);
+        load_x(xf, nr);
         if (tiles) {
             __syncthreads();
             constexpr int STEP = 4 * CE;  // rows per matrix instruction: 32, or 16 by four instructions
@@ -498,7 +524,11 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                     const int n = (i * kBwdWaves + wave) * 16;
                     if (n >= cols) break;
                     const Chunk zc = load_columns<T>(mem + lay.dz, lay.pn, lo, hi, n + (CPG == 1 ? (li & 3) * 4 : li));
-                    if constexpr (!kRegDb) mma_chunk<T>(accb[i], zc, Chunk{{0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u}});
+                    if constexpr (!kRegDb) {
+                        float v[4];
+                        __builtin_memcpy(v, &zc, sizeof(v));
+                        accb[i] += (v[0] + v[1]) + (v[2] + v[3]);
+                    }
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt) mma_chunk<T>(accw[i][kt], zc, xc[kt]);
                 }
@@ -521,14 +551,15 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
             }
     }
     if constexpr (!kRegDb) {
-        if (a.part_b && li == 0)
+        if (a.part_b)
 #pragma unroll
-            for (int i = 0; i < NTW; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int n = (i * kBwdWaves + wave) * 16 + lg * 4 + q;
-                    if (n < a.N) a.part_b[(int64_t)blockIdx.x * a.N + n] = accb[i][q];
-                }
+            for (int i = 0; i < NTW; ++i) {
+                float v = accb[i];  // column li of the tile, rows of this lane group
+                v += __shfl_xor(v, 16);
+                v += __shfl_xor(v, 32);
+                const int n = (i * kBwdWaves + wave) * 16 + li;
+                if (lg == 0 && n < a.N) a.part_b[(int64_t)blockIdx.x * a.N + n] = v;
+            }
     } else if (a.part_b) {
         float *wb = (float *)(mem + lay.dz) + wave * cols;  // (the tiles are done with: every wave is behind its last barrier)
         __syncthreads();
@@ -713,8 +744,12 @@ int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
     return check_launch();
 }
 
-template <typename T>
-bool rows_fit(int K) { return (size_t)K * sizeof(T) <= 512; }
+template <typename T, int MODE>
+bool rows_fit(const LinArgs &a) {
+    const bool side = MODE == kModeDz || a.res;
+    return (size_t)a.K * sizeof(T) <= 512 && row_reader_fits<T>(a.rows, a.xp, a.K) &&
+           (!side || row_reader_fits<T>(a.rows, MODE == kModeDz ? a.dyp : a.rp, a.N));
+}
 
 template <typename T, int MODE>
 int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
@@ -727,7 +762,7 @@ int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
 
 template <typename T, int MODE>
 int launch_tile(const LinArgs &a, hipStream_t s) {
-    if (rows_fit<T>(a.K)) return launch_rows<T, MODE>(a, 0, s);
+    if (rows_fit<T, MODE>(a)) return launch_rows<T, MODE>(a, 0, s);
     const int64_t mt = (a.rows + kBM - 1) / kBM;
     const int bn = a.N > 64 ? 128 : 64;
     const int64_t tiles = mt * ((a.N + bn - 1) / bn);
@@ -760,7 +795,7 @@ template <typename T>
 BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N) {
     BwdRowsPlan p = {0, 0, 0, 0};
     const int row = K * (int)sizeof(T);
-    if (row > 512 || N > 256) return p;
+    if (row > 512 || N > 256 || K < kChunk<T> || N < kChunk<T>) return p;
     const int kc = row <= 64 ? 1 : row <= 128 ? 2 : row <= 256 ? 4 : 8, ng = (N + 63) / 64 * 2;
     p.bytes = BwdRowsLds<T>(kc, N).bytes;
     if (!bwd_rows_fits<T>(kc, ng) || p.bytes > 160 * 1024) return p;
