@@ -144,6 +144,14 @@ __device__ __forceinline__ Chunk load_columns(const char *lds, int pitch, int lo
     return c;
 }
 
+// A workgroup barrier for LDS alone: __syncthreads also waits for every global load under way, which is what a kernel that
+// reads ahead must not do.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 inline bool known_dtype(int d) { return d == FSGS_F32 || d == FSGS_BF16 || d == FSGS_F16; }
 
 }  // namespace fsgs

@@ -22,23 +22,33 @@ struct LinArgs {
     int K, N, act;
 };
 
-// The normal distribution's tail h = P(t) exp(-z^2 / 2) at |z|, t = 1 / (1 + 0.34 |z|), P of degree 7 without a constant term
-// (fitted here to erfc: |error of h| < 9e-9, a seventh of half an fp32 step at 1), and the exponential itself.
+// The normal distribution's tail h = P(t) exp(-z^2 / 2) at |z|, t = 1 / (1 + c |z|), P a polynomial without a constant term
+// fitted to erfc here; P and the exponential apart.  fp32: degree 7, |error of h| < 9e-9, a seventh of half an fp32 step at 1;
+// half width: degree 5, < 4e-7, a six-hundredth of half an fp16 step.
+template <typename T>
 __device__ __forceinline__ float normal_tail(float z, float &e) {
-    const float az = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(0.34f, az, 1.f));
+    constexpr float c = sizeof(T) == 4 ? 0.34f : 0.35f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(c, fabsf(z), 1.f));
     e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
-    float p = 0.04310445f;
-    p = fmaf(p, t, -0.19278112f);
-    p = fmaf(p, t, 0.24988606f);
-    p = fmaf(p, t, -0.0172307f);
-    p = fmaf(p, t, 0.1495994f);
-    p = fmaf(p, t, 0.13158924f);
-    p = fmaf(p, t, 0.13583268f);
-    return p * t * e;
+    float p;
+    if constexpr (sizeof(T) == 4) {
+        p = fmaf(0.04310445f, t, -0.19278112f);
+        p = fmaf(p, t, 0.24988606f);
+        p = fmaf(p, t, -0.0172307f);
+        p = fmaf(p, t, 0.1495994f);
+        p = fmaf(p, t, 0.13158924f);
+        p = fmaf(p, t, 0.13583268f);
+    } else {
+        p = fmaf(-0.09327425f, t, 0.2608071f);
+        p = fmaf(p, t, 0.03706592f);
+        p = fmaf(p, t, 0.15632539f);
+        p = fmaf(p, t, 0.1390755f);
+    }
+    return p * t;
 }
 
 // z -> act(z) for N values (one uniform branch for all of them).
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
     if (act == FSGS_ACT_RELU) {
 #pragma unroll
@@ -47,7 +57,8 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float e;
-            z[i] = fmaf(-fabsf(z[i]), normal_tail(z[i], e), fmaxf(z[i], 0.f));  // z >= 0: z - z h; z < 0: -|z| h
+            const float p = normal_tail<T>(z[i], e);
+            z[i] = fmaf(-fabsf(z[i]), p * e, fmaxf(z[i], 0.f));  // z >= 0: z - z h; z < 0: -|z| h
         }
     } else if (act == FSGS_ACT_SILU) {
 #pragma unroll
@@ -57,7 +68,7 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
 }
 
 // z -> act'(z) for N values.
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void act_slope(float (&z)[N], int act) {
     if (act == FSGS_ACT_RELU) {
 #pragma unroll
@@ -66,8 +77,8 @@ __device__ __forceinline__ void act_slope(float (&z)[N], int act) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float e;
-            const float h = normal_tail(z[i], e);
-            z[i] = (z[i] < 0.f ? h : 1.f - h) + z[i] * 0.39894228040143268f * e;
+            const float p = normal_tail<T>(z[i], e), r = e * fmaf(-0.39894228040143268f, fabsf(z[i]), p);
+            z[i] = z[i] < 0.f ? r : 1.f - r;  // z < 0: h + z density; z >= 0: 1 - h + z density
         }
     } else if (act == FSGS_ACT_SILU) {
 #pragma unroll
@@ -180,8 +191,8 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
             float z[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) z[q] = acc[i][j][q] + b[q];
-            if constexpr (MODE == kModeDz) act_slope(z, a.act);
-            else act_fwd(z, a.act);
+            if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
+            else act_fwd<T>(z, a.act);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if constexpr (MODE == kModeDz) z[q] *= (float)sv[q];
@@ -324,8 +335,8 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
             float z[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
-            if constexpr (MODE == kModeDz) act_slope(z, a.act);
-            else act_fwd(z, a.act);
+            if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
+            else act_fwd<T>(z, a.act);
             if (has_side) {
                 float sv[8];
 #pragma unroll
@@ -379,6 +390,8 @@ struct BwdRowsArgs {
 
 constexpr int kBwdWaves = 8, kBwdRows = 16 * kBwdWaves;
 
+constexpr int bwd_wave_cols(int kt) { return kt >= 2 ? 2 : 1; }
+
 // LDS: W [32 ceil(N/32)][K], dz [128][N], x [128][K], bias; pitches that keep 16 or 32 lanes on different banks.
 template <typename T>
 struct BwdRowsLds {
@@ -394,8 +407,9 @@ struct BwdRowsLds {
 template <typename T, int KC, int NG>
 __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) {
     constexpr int CE = kChunk<T>, CPG = sizeof(T) == 2 ? 1 : 2;
-    constexpr int NTW = (2 * NG + kBwdWaves - 1) / kBwdWaves;  // 16-column tiles of dW's other axis per wave
     constexpr int KT = KC * 4 / (int)sizeof(T);  // 16-column tiles of K
+    // dW's tiles over the waves: 4 x 2 (fewer operands to fetch than 8 x 1, and 10 x 2 tiles come out as 3, not 4, per wave)
+    constexpr int WK = bwd_wave_cols(KT), WN = kBwdWaves / WK, NTW = (2 * NG + WN - 1) / WN, KTW = KT / WK;
     extern __shared__ Chunk lds[];
     char *const mem = (char *)lds;
     const BwdRowsLds<T> lay(KC, a.N);
@@ -421,7 +435,8 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
 #pragma unroll
         for (int q = 0; q < CPG; ++q) f[q] = gr.raw(row * a.dyp + column(g, q));
     };
-    f32x4 accw[NTW][KT] = {};
+    const int wn = wave / WK, wk = wave % WK;
+    f32x4 accw[NTW][KTW] = {};
     constexpr bool kRegDb = sizeof(T) == 2;
     float db[kRegDb ? NG : 1][8] = {};
     float accb[kRegDb ? 1 : NTW] = {};
@@ -467,7 +482,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
             for (int q = 0; q < CPG; ++q) unpack_chunk<T>(dyc[g][q], d + q * CE);
             load_dy(dyc[g], nr, g);
             if (a.act != FSGS_ACT_NONE) {
-                act_slope(z, a.act);
+                act_slope<T>(z, a.act);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] *= z[e];
             }
@@ -510,18 +525,18 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
         m = next;
         load_x(xf, nr);
         if (tiles) {
-            __syncthreads();
+            lds_barrier();
             constexpr int STEP = 4 * CE;  // rows per matrix instruction: 32, or 16 by four instructions
 #pragma unroll
             for (int s = 0; s < kBwdRows / STEP; ++s) {
                 const int lo = s * STEP + lg * 4, hi = lo + 16;
-                Chunk xc[KT];
+                Chunk xc[KTW];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-                    xc[kt] = load_columns<T>(mem + lay.x, lay.pk, lo, hi, kt * 16 + (CPG == 1 ? (li & 3) * 4 : li));
+                for (int j = 0; j < KTW; ++j)
+                    xc[j] = load_columns<T>(mem + lay.x, lay.pk, lo, hi, (wk * KTW + j) * 16 + (CPG == 1 ? (li & 3) * 4 : li));
 #pragma unroll
                 for (int i = 0; i < NTW; ++i) {
-                    const int n = (i * kBwdWaves + wave) * 16;
+                    const int n = (i * WN + wn) * 16;
                     if (n >= cols) break;
                     const Chunk zc = load_columns<T>(mem + lay.dz, lay.pn, lo, hi, n + (CPG == 1 ? (li & 3) * 4 : li));
                     if constexpr (!kRegDb) {
@@ -530,10 +545,10 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                         accb[i] += (v[0] + v[1]) + (v[2] + v[3]);
                     }
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) mma_chunk<T>(accw[i][kt], zc, xc[kt]);
+                    for (int j = 0; j < KTW; ++j) mma_chunk<T>(accw[i][j], zc, xc[j]);
                 }
             }
-            __syncthreads();
+            lds_barrier();
         }
     }
     if (a.part_w) {
@@ -542,11 +557,11 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
         for (int i = 0; i < NTW; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int n = (i * kBwdWaves + wave) * 16 + lg * 4 + q;
+                const int n = (i * WN + wn) * 16 + lg * 4 + q;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int k = kt * 16 + li;
-                    if (n < a.N && k < a.K) pw[(int64_t)n * a.K + k] = accw[i][kt][q];
+                for (int j = 0; j < KTW; ++j) {
+                    const int k = (wk * KTW + j) * 16 + li;
+                    if (n < a.N && k < a.K) pw[(int64_t)n * a.K + k] = accw[i][j][q];
                 }
             }
     }
@@ -557,8 +572,8 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                 float v = accb[i];  // column li of the tile, rows of this lane group
                 v += __shfl_xor(v, 16);
                 v += __shfl_xor(v, 32);
-                const int n = (i * kBwdWaves + wave) * 16 + li;
-                if (lg == 0 && n < a.N) a.part_b[(int64_t)blockIdx.x * a.N + n] = v;
+                const int n = (i * WN + wn) * 16 + li;
+                if (lg == 0 && wk == 0 && n < a.N) a.part_b[(int64_t)blockIdx.x * a.N + n] = v;
             }
     } else if (a.part_b) {
         float *wb = (float *)(mem + lay.dz) + wave * cols;  // (the tiles are done with: every wave is behind its last barrier)
@@ -787,8 +802,8 @@ struct BwdRowsPlan {
 
 template <typename T>
 constexpr bool bwd_rows_fits(int kc, int ng) {
-    const int kt = kc * 4 / (int)sizeof(T), ntw = (2 * ng + kBwdWaves - 1) / kBwdWaves;
-    return ntw * kt * 4 + kt * 4 + ng * (sizeof(T) == 2 ? 12 : 8) + kc * 4 <= 144;
+    const int kt = kc * 4 / (int)sizeof(T), wk = bwd_wave_cols(kt), wn = kBwdWaves / wk, ntw = (2 * ng + wn - 1) / wn;
+    return ntw * (kt / wk) * 4 + kt * 4 + ng * (sizeof(T) == 2 ? 12 : 8) + kc * 4 <= 144;
 }
 
 template <typename T>
