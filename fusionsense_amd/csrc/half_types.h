@@ -38,14 +38,14 @@ __device__ __forceinline__ Chunk load_chunk_n(const T *p, int n) {
 }
 
 // Rows of a matrix read in chunks that need not end with the row: raw() reads 16 bytes wherever they start (held back only at
-// the matrix' last element, so nothing outside it is read) and has no branch, so it can be under way long before it is used;
+// the matrix' last element, so nothing outside it is read; a matrix of less than 16 bytes is read from its start) and has no branch, so it can be under way long before it is used;
 // fix() then moves what was held back to its place and zeroes what lies behind `valid` elements.
 template <typename T>
 struct RowReader {
     const T *p;
     int64_t pitch, lim;  // lim: the last element a chunk may start at
     __device__ RowReader(const void *base, int64_t rows, int64_t pitch_, int width)
-        : p((const T *)base), pitch(pitch_), lim((rows - 1) * pitch_ + width - kChunk<T>) {}
+        : p((const T *)base), pitch(pitch_), lim(max((rows - 1) * pitch_ + width - kChunk<T>, (int64_t)0)) {}
     __device__ __forceinline__ Chunk raw(int64_t at) const { return load_chunk(p + min(at, lim)); }
     // may_end: some lane's chunk may reach the matrix' end (the same for the whole wave)
     __device__ __forceinline__ void fix(Chunk &c, int64_t at, int valid, bool may_end) const {
@@ -67,9 +67,6 @@ struct RowReader {
         }
     }
 };
-template <typename T>
-inline bool row_reader_fits(int64_t rows, int64_t pitch, int width) { return (rows - 1) * pitch + width >= kChunk<T>; }
-
 // kChunk floats rounded (to nearest, ties to even) to a chunk: two per instruction in the half-width types.
 template <typename T>
 __device__ __forceinline__ Chunk pack_chunk(const float *v) {

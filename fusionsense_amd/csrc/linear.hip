@@ -12,14 +12,15 @@ namespace fsgs {
 
 namespace {
 
-constexpr int kBM = 128;      // rows of x per tile
-constexpr int kSlabBytes = 128;  // one step along the summed axis: 64 half-width or 32 fp32 values
+constexpr int kSlabBytes = 128;  // one step along the summed axis of the general tile: 64 half-width or 32 fp32 values
 
 struct LinArgs {
     const void *x, *w, *bias, *res, *dy;
     void *y;
     int64_t rows, xp, rp, dyp, yp;
     int K, N, act;
+    int stream;     // general tile: store past the caches
+    float *part_b;  // dz kernels: partial column sums of dz, or null
 };
 
 // The normal distribution's tail h = P(t) exp(-z^2 / 2) at |z|, t = 1 / (1 + c |z|), P a polynomial without a constant term
@@ -98,66 +99,119 @@ constexpr int kEndRows = 8;
 
 enum { kModeFwd = 0, kModeDz = 1 };
 
-// Tile of 128 rows x BN columns, four waves of 64 x BN/2.  Both operands go through LDS in 128-byte slabs of the summed
-// axis; W is the A operand, so that a lane ends with four neighbouring columns of one row and stores them together.
-template <typename T, int MODE, int BN>
-__global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
-    constexpr int CE = kChunk<T>, BK = kSlabBytes / (int)sizeof(T);
-    constexpr int NT = BN / 32, MT = 4;
-    constexpr int XL = kBM * 8 / 256, WL = BN * 8 / 256;  // chunks per thread and slab
-    __shared__ Chunk xs[kBM * 8], ws[BN * 8];
-    const T *x = (const T *)a.x, *w = (const T *)a.w;
+// A lane's 8 columns (of 32) of fp32 dz, summed over the 16 lanes that hold different rows.
+__device__ __forceinline__ void sum_rows(float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] += dpp_f<0xB1>(v[e]);
+        v[e] += dpp_f<0x4E>(v[e]);
+        v[e] += dpp_f<0x141>(v[e]);
+        v[e] += dpp_f<0x140>(v[e]);
+    }
+}
+// ... and the column of each among the 32.
+template <typename T>
+__device__ __forceinline__ int held_column(int lg, int e) {
+    return sizeof(T) == 2 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3);
+}
+
+// Workgroups in dispatch order go round the 8 XCDs, each with an L2 of its own: neighbouring tiles, which share rows of x, are
+// given to one XCD.
+__device__ __forceinline__ int64_t xcd_tile(int64_t id, int64_t n) {
+    const int64_t per = (n + 7) / 8, t = (id & 7) * per + (id >> 3);
+    return t < n && (id >> 3) < per ? t : -1;
+}
+
+// Columns go by groups of 32 (two A tiles): in the half-width types tile t holds the rows of W with
+// column = 8 (r / 4) + 4 t + r % 4 of the group, so that a lane ends with 8 neighbouring columns of one row, 16 bytes.
+template <typename T>
+__device__ __forceinline__ int group_column(int t, int r) {
+    return sizeof(T) == 2 ? (r >> 2) * 8 + t * 4 + (r & 3) : t * 16 + r;
+}
+
+// The first n (at least one) elements of a chunk.
+template <typename T>
+__device__ __forceinline__ void put_chunk(T *to, const Chunk &c, int n, bool stream) {
+    if (n >= kChunk<T>) {
+        if (stream) store_streaming(to, c);
+        else __builtin_memcpy(to, &c, sizeof(Chunk));
+    } else {
+        T t[kChunk<T>];
+        __builtin_memcpy(t, &c, sizeof(Chunk));
+#pragma unroll
+        for (int e = 0; e < kChunk<T>; ++e)
+            if (e < n) to[e] = t[e];
+    }
+}
+
+// ---- general tile: 32 MT rows x BN columns, four waves of 16 MT x BN/2 ---------------------------------------------------
+// Both operands go through LDS in 128-byte slabs of the summed axis (the next slab is under way in registers); W is the A
+// operand, so that a lane ends with neighbouring columns of one row.  Slab rows are two to the 64 banks: chunk c of row r lies
+// at c ^ key(r), with a key that gives the 16 rows of either operand 16 different bank quads.
+template <typename T, int MODE, int BN, int MT>
+__global__ __launch_bounds__(256, 2) void linear_tile_kernel(LinArgs a) {
+    constexpr int CE = kChunk<T>, BK = kSlabBytes / (int)sizeof(T), BM = 32 * MT;
+    constexpr int NT = BN / 32;
+    constexpr int XL = BM * 8 / 256, WL = BN * 8 / 256;  // chunks per thread and slab
+    constexpr int CPG = sizeof(T) == 2 ? 1 : 2;          // 16-byte pieces of a row that a lane holds of 32 columns
+    __shared__ Chunk xs[BM * 8], ws[BN * 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int ntiles_n = (a.N + BN - 1) / BN;
-    const int64_t tile = blockIdx.x;
-    const int64_t m0 = (tile / ntiles_n) * kBM;
+    const int64_t tile = xcd_tile(blockIdx.x, (a.rows + BM - 1) / BM * ntiles_n);
+    if (tile < 0) return;
+    const int64_t m0 = tile / ntiles_n * BM;
     const int n0 = (int)(tile % ntiles_n) * BN;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * (BN / 2);
+    const int wm = (wave & 1) * 16 * MT, wn = (wave >> 1) * (BN / 2);
     const int li = lane & 15, lg = lane >> 4;
+    auto xkey = [](int r) { return (r >> 1) & 7; };
+    auto wkey = [](int r) { return sizeof(T) == 2 ? ((r >> 3) & 3) << 1 | ((r >> 1) & 1) : (r >> 1) & 7; };
 
+    const RowReader<T> xr(a.x, a.rows, a.xp, a.K), wr(a.w, a.N, a.K, a.K);
+    const bool end = m0 + BM + kEndRows >= a.rows || n0 + BN + kEndRows >= a.N || a.xp == 0;
     f32x4 acc[NT][MT] = {};
-    Chunk xr[XL], wr[WL];
+    Chunk xc[XL], wc[WL];
+    const int ck = (tid & 7) * CE;
+    auto xrow = [&](int i) { return min(m0 + (tid >> 3) + i * 32, a.rows - 1); };
+    auto wrow = [&](int i) { return (int64_t)min(n0 + (tid >> 3) + i * 32, a.N - 1); };
     auto fetch = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < XL; ++i) {
-            const int c = tid + i * 256, r = c >> 3, k = k0 + (c & 7) * CE;
-            const int64_t m = m0 + r;
-            xr[i] = load_chunk_n(x + m * a.xp + k, m < a.rows ? a.K - k : 0);
-        }
+        for (int i = 0; i < XL; ++i) xc[i] = xr.raw(xrow(i) * a.xp + k0 + ck);
 #pragma unroll
-        for (int i = 0; i < WL; ++i) {
-            const int c = tid + i * 256, r = c >> 3, k = k0 + (c & 7) * CE;
-            const int n = n0 + r;
-            wr[i] = load_chunk_n(w + (int64_t)n * a.K + k, n < a.N ? a.K - k : 0);
-        }
+        for (int i = 0; i < WL; ++i) wc[i] = wr.raw(wrow(i) * a.K + k0 + ck);
     };
     fetch(0);
     for (int k0 = 0; k0 < a.K; k0 += BK) {
-        __syncthreads();
+        if (k0 + BK > a.K || end) {  // (rows behind the last repeat it: their results are not stored)
+#pragma unroll
+            for (int i = 0; i < XL; ++i) xr.fix(xc[i], xrow(i) * a.xp + k0 + ck, a.K - k0 - ck, end);
+#pragma unroll
+            for (int i = 0; i < WL; ++i) wr.fix(wc[i], wrow(i) * a.K + k0 + ck, a.K - k0 - ck, end);
+        }
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
-            const int c = tid + i * 256, r = c >> 3;
-            xs[r * 8 + ((c & 7) ^ (r & 7))] = xr[i];
+            const int r = (tid >> 3) + i * 32;
+            xs[r * 8 + ((tid & 7) ^ xkey(r))] = xc[i];
         }
 #pragma unroll
         for (int i = 0; i < WL; ++i) {
-            const int c = tid + i * 256, r = c >> 3;
-            ws[r * 8 + ((c & 7) ^ (r & 7))] = wr[i];
+            const int r = (tid >> 3) + i * 32;
+            ws[r * 8 + ((tid & 7) ^ wkey(r))] = wc[i];
         }
-        __syncthreads();
+        lds_barrier();
         if (k0 + BK < a.K) fetch(k0 + BK);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             Chunk xf[MT], wf[NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int r = wm + i * 16 + li;
-                xf[i] = xs[r * 8 + ((s * 4 + lg) ^ (r & 7))];
+            for (int i = 0; i < NT; ++i) {
+                const int r = wn + (i >> 1) * 32 + group_column<T>(i & 1, li);
+                wf[i] = ws[r * 8 + ((s * 4 + lg) ^ wkey(r))];
             }
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int r = wn + i * 16 + li;
-                wf[i] = ws[r * 8 + ((s * 4 + lg) ^ (r & 7))];
+            for (int i = 0; i < MT; ++i) {
+                const int r = wm + i * 16 + li;
+                xf[i] = xs[r * 8 + ((s * 4 + lg) ^ xkey(r))];
             }
 #pragma unroll
             for (int i = 0; i < NT; ++i)
@@ -167,50 +221,60 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
     }
 
     const T *bias = (const T *)a.bias;
-    T *y = (T *)a.y;
+    const T *side = (const T *)(MODE == kModeDz ? a.dy : a.res);
+    const int64_t sp = MODE == kModeDz ? a.dyp : a.rp;
+    const bool stream = a.stream;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int n = n0 + wn + i * 16 + lg * 4;
-        const int nv = min(4, a.N - n);
-        if (nv <= 0) continue;
-        float b[4];
+    for (int i = 0; i < NT / 2; ++i) {
+        float b[8], colsum[8] = {};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) b[q] = bias && q < nv ? (float)bias[n + q] : 0.f;
+        for (int e = 0; e < 8; ++e) {
+            const int n = n0 + wn + i * 32 + held_column<T>(lg, e);
+            b[e] = bias && n < a.N ? (float)bias[n] : 0.f;
+        }
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             const int64_t m = m0 + wm + j * 16 + li;
             if (m >= a.rows) continue;
-            const T *side = MODE == kModeDz ? (const T *)a.dy + m * a.dyp + n
-                            : a.res         ? (const T *)a.res + m * a.rp + n
-                                            : nullptr;
-            T sv[4], out[4];
-            if (side) {
-                if (nv == 4) __builtin_memcpy(sv, side, sizeof(sv));
-                else for (int q = 0; q < nv; ++q) sv[q] = side[q];
-            }
-            float z[4];
+            float z[8], sv[8];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) z[q] = acc[i][j][q] + b[q];
+            for (int q = 0; q < CPG; ++q) {
+                const int n = n0 + wn + i * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                if (side) unpack_chunk<T>(load_chunk_n(side + m * sp + n, a.N - n), sv + q * CE);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = acc[2 * i + (e >> 2)][j][e & 3] + b[e];
             if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
             else act_fwd<T>(z, a.act);
+            if (side)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if constexpr (MODE == kModeDz) z[q] *= (float)sv[q];
-                else z[q] += side ? (float)sv[q] : 0.f;
-                out[q] = (T)z[q];
+                for (int e = 0; e < 8; ++e) z[e] = MODE == kModeDz ? z[e] * sv[e] : z[e] + sv[e];
+            if constexpr (MODE == kModeDz)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) colsum[e] += z[e];
+#pragma unroll
+            for (int q = 0; q < CPG; ++q) {
+                const int n = n0 + wn + i * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+                if (n < a.N) put_chunk((T *)a.y + m * a.yp + n, pack_chunk<T>(z + q * CE), a.N - n, stream);
             }
-            T *dst = y + m * a.yp + n;
-            if (nv == 4) __builtin_memcpy(dst, out, sizeof(out));
-            else for (int q = 0; q < nv; ++q) dst[q] = out[q];
         }
+        if constexpr (MODE == kModeDz)
+            if (a.part_b) {
+                sum_rows(colsum);
+                float *to = a.part_b + (m0 / (16 * MT) + (wave & 1)) * a.N;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int n = n0 + wn + i * 32 + held_column<T>(lg, e);
+                    if (li == 0 && n < a.N) to[n] = colsum[e];
+                }
+            }
     }
 }
 
 // ---- short summed axis: rows go straight from memory to the matrix pipe ------------------------------------------------
 // One wave takes 16 rows at a time and all columns of its workgroup's range.  W (its range) lies in LDS for the life of the
 // workgroup, a row of x is read once, 16 bytes per lane, directly in the layout of the B operand: no barrier and no staging
-// in the loop.  Columns go by groups of 32 (two A tiles): in the half-width types tile t holds the rows of W with
-// column = 8 (r / 4) + 4 t + r % 4 of the group, so that a lane ends with 8 neighbouring columns of one row, 16 bytes.
+// in the loop.
 //
 // How y is stored (640 000 rows, 64 -> 128 bf16: plain 77 us, streaming 49; 32 -> 150 fp32: plain 190, streaming 463):
 //   kStorePlain   through the caches: small outputs, which the next kernel finds there
@@ -223,11 +287,6 @@ struct RowsArgs {
     int range;      // columns per workgroup (a multiple of 32)
     int transpose;  // W is given as [K,N] (its element (n,k) at k * N + n)
 };
-
-template <typename T>
-__device__ __forceinline__ int group_column(int t, int r) {
-    return sizeof(T) == 2 ? (r >> 2) * 8 + t * 4 + (r & 3) : t * 16 + r;
-}
 
 template <typename T, int KC>
 constexpr int rows_pitch() { return KC * 4 + 1; }  // chunks between two rows of W in LDS: 16 rows then lie in 16 bank quads
@@ -252,27 +311,11 @@ __device__ __forceinline__ void fill_weights(Chunk *wl, const T *w, int n0, int 
     }
 }
 
-// The first n (at least one) elements of a chunk.
-template <typename T>
-__device__ __forceinline__ void put_chunk(T *to, const Chunk &c, int n, bool stream) {
-    if (n >= kChunk<T>) {
-        if (stream) store_streaming(to, c);
-        else __builtin_memcpy(to, &c, sizeof(Chunk));
-    } else {
-        T t[kChunk<T>];
-        __builtin_memcpy(t, &c, sizeof(Chunk));
-#pragma unroll
-        for (int e = 0; e < kChunk<T>; ++e)
-            if (e < n) to[e] = t[e];
-    }
-}
-
 template <typename T, int MODE, int KC, int STORE>
 __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     constexpr int CE = kChunk<T>, P = rows_pitch<T, KC>();
     extern __shared__ Chunk lds[];
     const LinArgs &a = ra.l;
-    const T *x = (const T *)a.x;
     T *y = (T *)a.y;
     Chunk *wl = lds;
     float *bl = (float *)(lds + ra.range * P);
@@ -282,7 +325,10 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
         bl[n] = a.bias && n < ncols ? (float)((const T *)a.bias)[n0 + n] : 0.f;
     __syncthreads();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+    float *dbl = bl + ra.range + wave * ra.range;                      // (kModeDz with part_b: this wave's column sums)
     char *mine = (char *)(bl + ra.range) + wave * tile_bytes<T>(a.N);  // (kStoreTile)
+    if (MODE == kModeDz && a.part_b)
+        for (int n = lane; n < ra.range; n += 64) dbl[n] = 0.f;
     constexpr int CPG = sizeof(T) == 2 ? 1 : 2;  // 16-byte pieces of a row that a lane holds of a group
     const RowReader<T> xr(a.x, a.rows, a.xp, a.K);
     const bool has_side = MODE == kModeDz || a.res;
@@ -334,7 +380,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
                     mma_chunk<T>(acc[i], wl[(g * 32 + group_column<T>(i, li)) * P + c * 4 + lg], xf[c]);
             float z[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
+            for (int e = 0; e < 8; ++e) z[e] = acc[e >> 2][e & 3] + bl[g * 32 + held_column<T>(lg, e)];
             if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
             else act_fwd<T>(z, a.act);
             if (has_side) {
@@ -346,6 +392,15 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) z[e] = MODE == kModeDz ? z[e] * sv[e] : z[e] + sv[e];
+            }
+            if (MODE == kModeDz && a.part_b) {
+                float c[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) c[e] = m < a.rows ? z[e] : 0.f;
+                sum_rows(c);
+                if (li == 0)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dbl[g * 32 + held_column<T>(lg, e)] += c[e];
             }
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
@@ -371,6 +426,11 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+    }
+    if (MODE == kModeDz && a.part_b) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        float *to = a.part_b + ((int64_t)blockIdx.x * 4 + wave) * a.N + n0;
+        for (int n = lane; n < ncols; n += 64) to[n] = dbl[n];
     }
 }
 
@@ -472,7 +532,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                                      xf[c]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    z[e] = acc[e >> 2][e & 3] + bl[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))];
+                    z[e] = acc[e >> 2][e & 3] + bl[g * 32 + held_column<T>(lg, e)];
             }
             if (ragged_n || end)
 #pragma unroll
@@ -581,15 +641,10 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             if (g >= ng) break;
+            sum_rows(db[g]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float v = db[g][e];
-                v += dpp_f<0xB1>(v);
-                v += dpp_f<0x4E>(v);
-                v += dpp_f<0x141>(v);
-                v += dpp_f<0x140>(v);  // over the 16 rows of the wave
-                if (li == 0) wb[g * 32 + (CPG == 1 ? lg * 8 + e : (e >> 2) * 16 + lg * 4 + (e & 3))] = v;
-            }
+            for (int e = 0; e < 8; ++e)
+                if (li == 0) wb[g * 32 + held_column<T>(lg, e)] = db[g][e];
         }
         __syncthreads();
         const float *all = (const float *)(mem + lay.dz);
@@ -617,77 +672,116 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w,
 
 struct DwArgs {
     const void *dz, *x;
-    float *part_w, *part_b;  // [slices][N*K], [slices][N]
+    float *part_w, *part_b;  // [slices][N*K], [slices][N]; each may be null
     int64_t rows, dzp, xp, slice_rows;
-    int K, N;
+    int K, N, slices;
 };
 
-// dW tile of 64 columns of dz x 64 columns of x over one slice of the rows, db beside it (tiles of k = 0: dz against ones).
+// dW tile of 128 columns of dz x 128 columns of x over one slice of the rows, four waves of 64 x 64.  Slabs of 64 (fp32: 32)
+// rows of both lie in LDS as they come and are read by columns; the next slab is under way in registers.  db beside it, where
+// dz is dy as it stands (tiles of k = 0: dz against ones).  Tiles of one slice, which share rows, go to one XCD.
+constexpr int kDwTile = 128;
+
 template <typename T>
-__global__ __launch_bounds__(256) void linear_dw_kernel(DwArgs a) {
-    constexpr int CE = kChunk<T>, MS = 32, CPR = 64 / CE, L = MS * CPR / 256 > 0 ? MS * CPR / 256 : 1;
-    __shared__ T ds[MS][64 + CE], xs[MS][64 + CE];
-    const T *dz = (const T *)a.dz, *x = (const T *)a.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int k0 = blockIdx.x * 64, n0 = blockIdx.y * 64, slice = blockIdx.z;
-    const int wn = (wave >> 1) * 32, wk = (wave & 1) * 32;
-    const int li = lane & 15, lg = lane >> 4;
+__global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
+    constexpr int CE = kChunk<T>, ROWS = 128 / (int)sizeof(T), CPR = kDwTile / CE, L = ROWS * CPR / 256;
+    constexpr int PITCH = kDwTile * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16), STEP = 4 * CE;
+    __shared__ Chunk ds[ROWS * PITCH / 16], xs[ROWS * PITCH / 16];
+    char *const dm = (char *)ds, *const xm = (char *)xs;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+    const int kts = a.part_w ? (a.K + kDwTile - 1) / kDwTile : 1, nts = (a.N + kDwTile - 1) / kDwTile;
+    const int64_t id = xcd_tile(blockIdx.x, (int64_t)a.slices * kts * nts);
+    if (id < 0) return;
+    const int slice = (int)(id / (kts * nts)), tile = (int)(id % (kts * nts));
+    const int k0 = tile % kts * kDwTile, n0 = tile / kts * kDwTile;
+    const int wn = (wave >> 1) * 64, wk = (wave & 1) * 64;
+    const int nt = min(4, (a.N - n0 - wn + 15) / 16), kt = a.part_w ? min(4, (a.K - k0 - wk + 15) / 16) : 0;  // (may be < 1)
     const int64_t mb = slice * a.slice_rows, me = min(a.rows, mb + a.slice_rows);
     const bool want_b = a.part_b && k0 == 0 && wk == 0;
-    f32x4 acc[2][2] = {}, accb[2] = {};
-    for (int64_t m0 = mb; m0 < me; m0 += MS) {
-        __syncthreads();
+
+    const RowReader<T> dr(a.dz, a.rows, a.dzp, a.N), xr(a.x, a.rows, a.xp, a.K);
+    const bool ragged = n0 + kDwTile > a.N || k0 + kDwTile > a.K;
+    const int crow = tid / CPR, col = tid % CPR * CE;  // this thread's first chunk of a slab
+    Chunk dc[L], xc[L];
+    auto fetch = [&](int64_t m0) {
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int c = tid + i * 256, r = c / CPR, col = (c % CPR) * CE;
-            const int64_t m = m0 + r;
-            const Chunk cd = load_chunk_n(dz + m * a.dzp + n0 + col, m < me ? a.N - n0 - col : 0);
-            const Chunk cx = load_chunk_n(x + m * a.xp + k0 + col, m < me ? a.K - k0 - col : 0);
-            *(Chunk *)&ds[r][col] = cd;
-            *(Chunk *)&xs[r][col] = cx;
+            const int64_t m = min(m0 + crow + i * (256 / CPR), a.rows - 1);
+            dc[i] = dr.raw(m * a.dzp + n0 + col);
+            xc[i] = xr.raw(m * a.xp + k0 + col);
         }
-        __syncthreads();
-        constexpr int STEPS = sizeof(T) == 2 ? 1 : 2;
+    };
+    f32x4 acc[4][4] = {}, accb[4] = {};
+    T one[CE];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            Chunk df[2], xf[2];
+    for (int e = 0; e < CE; ++e) one[e] = (T)1.f;
+    Chunk ones;
+    __builtin_memcpy(&ones, one, sizeof(Chunk));
+    if (mb < me) fetch(mb);
+    for (int64_t m0 = mb; m0 < me; m0 += ROWS) {
+        const bool end = m0 + ROWS + kEndRows >= a.rows;
+        if (ragged || end || m0 + ROWS > me) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                T vd[CE], vx[CE];
-#pragma unroll
-                for (int e = 0; e < CE; ++e) {
-                    const int r = (s * 4 + lg) * CE + e;
-                    vd[e] = ds[r][wn + t * 16 + li];
-                    vx[e] = xs[r][wk + t * 16 + li];
-                }
-                __builtin_memcpy(&df[t], vd, 16);
-                __builtin_memcpy(&xf[t], vx, 16);
+            for (int i = 0; i < L; ++i) {
+                const int64_t mi = m0 + crow + i * (256 / CPR), m = min(mi, a.rows - 1);
+                dr.fix(dc[i], m * a.dzp + n0 + col, mi < me ? a.N - n0 - col : 0, end || a.dzp == 0);
+                xr.fix(xc[i], m * a.xp + k0 + col, mi < me ? a.K - k0 - col : 0, end || a.xp == 0);
             }
+        }
+        lds_barrier();
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < L; ++i) {
+            const int at = (crow + i * (256 / CPR)) * PITCH + col * (int)sizeof(T);
+            *(Chunk *)(dm + at) = dc[i];
+            *(Chunk *)(xm + at) = xc[i];
+        }
+        lds_barrier();
+        if (m0 + ROWS < me) fetch(m0 + ROWS);
+        const int lc = sizeof(T) == 2 ? (li & 3) * 4 : li;
+        if (nt == 4 && kt == 4 && !want_b) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) mma_chunk<T>(acc[i][j], df[i], xf[j]);
-            if (want_b) {
-                T one[CE];
+            for (int s = 0; s < ROWS / STEP; ++s) {
+                const int lo = s * STEP + lg * 4, hi = lo + 16;
+                Chunk df[4], xf[4];
 #pragma unroll
-                for (int e = 0; e < CE; ++e) one[e] = (T)1.f;
-                Chunk of;
-                __builtin_memcpy(&of, one, 16);
+                for (int i = 0; i < 4; ++i) {
+                    df[i] = load_columns<T>(dm, PITCH, lo, hi, wn + i * 16 + lc);
+                    xf[i] = load_columns<T>(xm, PITCH, lo, hi, wk + i * 16 + lc);
+                }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) mma_chunk<T>(accb[i], df[i], of);
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_chunk<T>(acc[i][j], df[i], xf[j]);
+            }
+        } else {
+            for (int s = 0; s < ROWS / STEP; ++s) {
+                const int lo = s * STEP + lg * 4, hi = lo + 16;
+                Chunk xf[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < kt) xf[j] = load_columns<T>(xm, PITCH, lo, hi, wk + j * 16 + lc);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < nt && (kt > 0 || want_b)) {
+                        const Chunk df = load_columns<T>(dm, PITCH, lo, hi, wn + i * 16 + lc);
+                        if (want_b) mma_chunk<T>(accb[i], df, ones);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (j < kt) mma_chunk<T>(acc[i][j], df, xf[j]);
+                    }
             }
         }
     }
     float *pw = a.part_w ? a.part_w + (int64_t)slice * a.N * a.K : nullptr;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int n = n0 + wn + i * 16 + lg * 4 + q;
             if (n >= a.N) continue;
             if (pw)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 4; ++j) {
                     const int k = k0 + wk + j * 16 + li;
                     if (k < a.K) pw[(int64_t)n * a.K + k] = acc[i][j][q];
                 }
@@ -700,13 +794,14 @@ __global__ __launch_bounds__(256) void linear_dw_kernel(DwArgs a) {
 template <typename T>
 __global__ __launch_bounds__(1024) void reduce_slices_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b,
                                                              T *__restrict__ dw, T *__restrict__ db, int64_t nk, int N,
-                                                             int slices) {
+                                                             int slices_w, int slices_b) {
     __shared__ float part[16][64];
     const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
     const int64_t i = (int64_t)blockIdx.x * 64 + c;
     const bool w = i < nk && dw, b = i >= nk && i < nk + N && db;
     const float *from = w ? part_w + i : b ? part_b + (i - nk) : nullptr;
     const int64_t pitch = w ? nk : N;
+    const int slices = w ? slices_w : slices_b;
     float s = 0.f;
     if (from)
         for (int t = r; t < slices; t += 16) s += from[t * pitch];
@@ -720,15 +815,19 @@ __global__ __launch_bounds__(1024) void reduce_slices_kernel(const float *__rest
 }
 
 template <typename T>
-int launch_reduce(const float *part_w, const float *part_b, void *dw, void *db, int K, int N, int slices, hipStream_t s) {
+int launch_reduce(const float *part_w, const float *part_b, void *dw, void *db, int K, int N, int slices_w, int slices_b,
+                  hipStream_t s) {
     const int64_t nk = (int64_t)N * K;
-    reduce_slices_kernel<T><<<(unsigned)((nk + N + 63) / 64), 1024, 0, s>>>(part_w, part_b, (T *)dw, (T *)db, nk, N, slices);
+    reduce_slices_kernel<T><<<(unsigned)((nk + N + 63) / 64), 1024, 0, s>>>(part_w, part_b, (T *)dw, (T *)db, nk, N, slices_w,
+                                                                                  slices_b);
     return check_launch();
 }
 
 // LDS of a workgroup of the rows kernel: weights up to 40 KB, four workgroups per CU; with the waves' output tiles up to 80 KB.
 constexpr int kRowsLds = 40 * 1024;
 constexpr int64_t kStreamBytes = 32 << 20;  // outputs from here on are stored past the caches
+
+unsigned rows_blocks(int64_t rows) { return (unsigned)((rows + 63) / 64 < 1024 ? (rows + 63) / 64 : 1024); }
 
 template <typename T, int MODE, int KC>
 int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
@@ -739,16 +838,16 @@ int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
     const int fit = kRowsLds / row_bytes / 32 * 32, need = (a.N + 31) / 32 * 32;
     r.range = need < fit ? need : fit;
     const int ranges = (a.N + r.range - 1) / r.range;
-    size_t bytes = (size_t)r.range * row_bytes;
-    const int64_t want = (a.rows + 63) / 64;
-    const dim3 grid((unsigned)(want < 1024 ? want : 1024), ranges);
+    const bool sums = MODE == kModeDz && a.part_b;
+    const size_t bytes = (size_t)r.range * (row_bytes + (sums ? 16 : 0));
+    const dim3 grid(rows_blocks(a.rows), ranges);
     if (a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes) {
         if (a.N * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0) {
             linear_rows_kernel<T, MODE, KC, kStoreStream><<<grid, 256, bytes, s>>>(r);
             return check_launch();
         }
         const size_t tiled = bytes + 4 * (size_t)tile_bytes<T>(a.N);
-        if (ranges == 1 && a.yp == a.N && tiled <= 2 * kRowsLds) {
+        if (!sums && ranges == 1 && a.yp == a.N && tiled <= 2 * kRowsLds) {
             const int rc = ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, kStoreTile>>(tiled);
             if (rc != FSGS_OK) return rc;
             linear_rows_kernel<T, MODE, KC, kStoreTile><<<grid, 256, tiled, s>>>(r);
@@ -759,12 +858,8 @@ int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
     return check_launch();
 }
 
-template <typename T, int MODE>
-bool rows_fit(const LinArgs &a) {
-    const bool side = MODE == kModeDz || a.res;
-    return (size_t)a.K * sizeof(T) <= 512 && row_reader_fits<T>(a.rows, a.xp, a.K) &&
-           (!side || row_reader_fits<T>(a.rows, MODE == kModeDz ? a.dyp : a.rp, a.N));
-}
+template <typename T>
+bool rows_fit(int K) { return (size_t)K * sizeof(T) <= 512; }
 
 template <typename T, int MODE>
 int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
@@ -777,19 +872,28 @@ int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
 
 template <typename T, int MODE>
 int launch_tile(const LinArgs &a, hipStream_t s) {
-    if (rows_fit<T, MODE>(a)) return launch_rows<T, MODE>(a, 0, s);
-    const int64_t mt = (a.rows + kBM - 1) / kBM;
+    if (rows_fit<T>(a.K)) return launch_rows<T, MODE>(a, 0, s);
+    constexpr int MT = 4;
     const int bn = a.N > 64 ? 128 : 64;
-    const int64_t tiles = mt * ((a.N + bn - 1) / bn);
-    if (tiles > (int64_t)UINT32_MAX / 256) return FSGS_EINVAL;  // (a grid holds at most 2^32 threads)
-    if (bn == 128) linear_tile_kernel<T, MODE, 128><<<(unsigned)tiles, 256, 0, s>>>(a);
-    else linear_tile_kernel<T, MODE, 64><<<(unsigned)tiles, 256, 0, s>>>(a);
+    const int64_t tiles = (a.rows + 32 * MT - 1) / (32 * MT) * ((a.N + bn - 1) / bn), blocks = (tiles + 7) / 8 * 8;
+    if (blocks > (int64_t)UINT32_MAX / 256) return FSGS_EINVAL;  // (a grid holds at most 2^32 threads)
+    LinArgs b = a;
+    b.stream = a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes && a.yp * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0;
+    if (bn == 128) linear_tile_kernel<T, MODE, 128, MT><<<(unsigned)blocks, 256, 0, s>>>(b);
+    else linear_tile_kernel<T, MODE, 64, MT><<<(unsigned)blocks, 256, 0, s>>>(b);
     return check_launch();
 }
 
+// Rows of partial column sums that launch_tile<kModeDz> leaves in part_b.
+int64_t dz_sum_rows(int64_t rows, int K, size_t e) {
+    return K * e <= 512 ? (int64_t)rows_blocks(rows) * 4 : (rows + 127) / 128 * 2;
+}
+
+int dw_tiles(int n) { return (n + kDwTile - 1) / kDwTile; }
+
+// Slices of the rows: as many workgroups as the card holds (two per CU), but 256 rows each at least.
 int dw_slices(int64_t rows, int K, int N) {
-    const int64_t tiles = (int64_t)((K + 63) / 64) * ((N + 63) / 64);
-    const int64_t want = (1024 + tiles - 1) / tiles, most = (rows + 255) / 256;
+    const int64_t tiles = (int64_t)dw_tiles(K) * dw_tiles(N), want = 512 / tiles, most = (rows + 255) / 256;
     const int64_t s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s);
 }
@@ -810,7 +914,7 @@ template <typename T>
 BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N) {
     BwdRowsPlan p = {0, 0, 0, 0};
     const int row = K * (int)sizeof(T);
-    if (row > 512 || N > 256 || K < kChunk<T> || N < kChunk<T>) return p;
+    if (row > 512 || N > 256) return p;
     const int kc = row <= 64 ? 1 : row <= 128 ? 2 : row <= 256 ? 4 : 8, ng = (N + 63) / 64 * 2;
     p.bytes = BwdRowsLds<T>(kc, N).bytes;
     if (!bwd_rows_fits<T>(kc, ng) || p.bytes > 160 * 1024) return p;
@@ -875,7 +979,8 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
     l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
     l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
     l.part_b = l.part_w + (dw ? up(s * (size_t)K * N * 4) : 0);
-    l.total = l.part_b + (db ? up(s * (size_t)N * 4) : 0);
+    const size_t sums = act != FSGS_ACT_NONE ? (size_t)dz_sum_rows(rows, K, e) : s;
+    l.total = l.part_b + (db ? up(sums * (size_t)N * 4) : 0);
     return l;
 }
 
@@ -891,43 +996,49 @@ int run_bwd(LinArgs a, void *dx, void *dw, void *db, char *scratch, const BwdScr
         b.stream = a.rows * a.K * (int64_t)sizeof(T) >= kStreamBytes && a.K * sizeof(T) % 64 == 0 && (uintptr_t)dx % 64 == 0;
         const int rc = launch_bwd_rows_k<T>(b, p, s);
         if (rc != FSGS_OK || (!dw && !db)) return rc;
-        return launch_reduce<T>(b.part_w, b.part_b, dw, db, a.K, a.N, p.blocks, s);
+        return launch_reduce<T>(b.part_w, b.part_b, dw, db, a.K, a.N, p.blocks, p.blocks, s);
     }
     const void *dz = a.dy;
     int64_t dzp = a.dyp;
+    float *part_w = dw ? (float *)(scratch + l.part_w) : nullptr, *part_b = db ? (float *)(scratch + l.part_b) : nullptr;
+    int rc = FSGS_OK, sum_rows = 0;
     if (a.act != FSGS_ACT_NONE) {
+        // (the sums of db are taken here, before dz is rounded to T)
         LinArgs z = a;
-        z.y = scratch + l.dz;
-        z.yp = a.N;
-        const int rc = launch_tile<T, kModeDz>(z, s);
+        z.y = scratch + l.dz, z.yp = a.N, z.part_b = part_b;
+        rc = launch_tile<T, kModeDz>(z, s);
         if (rc != FSGS_OK) return rc;
-        dz = z.y;
-        dzp = a.N;
+        dz = z.y, dzp = a.N, sum_rows = (int)dz_sum_rows(a.rows, a.K, sizeof(T));
     }
     if (dx) {
-        T *wt = (T *)(scratch + l.wt);
-        transpose_kernel<T><<<dim3((a.K + 31) / 32, (a.N + 31) / 32), 256, 0, s>>>((const T *)a.w, wt, a.N, a.K);
-        int rc = check_launch();
-        if (rc != FSGS_OK) return rc;
         LinArgs g = {};
-        g.x = dz, g.xp = dzp, g.w = wt, g.y = dx, g.yp = a.K, g.rows = a.rows, g.K = a.N, g.N = a.K;
-        rc = launch_tile<T, kModeFwd>(g, s);
+        g.x = dz, g.xp = dzp, g.y = dx, g.yp = a.K, g.rows = a.rows, g.K = a.N, g.N = a.K;
+        if (rows_fit<T>(a.N)) {
+            g.w = a.w;
+            rc = launch_rows<T, kModeFwd>(g, 1, s);
+        } else {
+            T *wt = (T *)(scratch + l.wt);
+            transpose_kernel<T><<<dim3((a.K + 31) / 32, (a.N + 31) / 32), 256, 0, s>>>((const T *)a.w, wt, a.N, a.K);
+            rc = check_launch();
+            if (rc != FSGS_OK) return rc;
+            g.w = wt;
+            rc = launch_tile<T, kModeFwd>(g, s);
+        }
         if (rc != FSGS_OK) return rc;
     }
-    if (dw || db) {
+    if (!dw && !db) return FSGS_OK;
+    const int slices = dw_slices(a.rows, a.K, a.N);
+    if (dw || !sum_rows) {
         DwArgs d = {};
-        const int slices = dw_slices(a.rows, a.K, a.N);
-        d.dz = dz, d.dzp = dzp, d.x = a.x, d.xp = a.xp, d.rows = a.rows, d.K = a.K, d.N = a.N;
-        d.part_w = dw ? (float *)(scratch + l.part_w) : nullptr;
-        d.part_b = db ? (float *)(scratch + l.part_b) : nullptr;
-        d.slice_rows = (((a.rows + slices - 1) / slices) + 31) / 32 * 32;
-        const int kt = dw ? (a.K + 63) / 64 : 1;
-        linear_dw_kernel<T><<<dim3(kt, (a.N + 63) / 64, slices), 256, 0, s>>>(d);
-        int rc = check_launch();
+        d.dz = dz, d.dzp = dzp, d.x = a.x, d.xp = a.xp, d.rows = a.rows, d.K = a.K, d.N = a.N, d.slices = slices;
+        d.part_w = part_w, d.part_b = sum_rows ? nullptr : part_b;
+        d.slice_rows = ((a.rows + slices - 1) / slices + 63) / 64 * 64;
+        const int64_t blocks = ((int64_t)slices * (dw ? dw_tiles(a.K) : 1) * dw_tiles(a.N) + 7) / 8 * 8;
+        linear_dw_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(d);
+        rc = check_launch();
         if (rc != FSGS_OK) return rc;
-        return launch_reduce<T>(d.part_w, d.part_b, dw, db, a.K, a.N, slices, s);
     }
-    return FSGS_OK;
+    return launch_reduce<T>(part_w, part_b, dw, db, a.K, a.N, slices, sum_rows ? sum_rows : slices, s);
 }
 
 bool bad_sizes(int64_t rows, int K, int N, int dtype, int act) {

@@ -1817,7 +1817,11 @@ def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
     t2 = t.reshape(-1, width)
     if width > 1 and t2.stride(1) != 1:
         t2 = t2.contiguous()
-    return t2, (t2.stride(0) if t2.shape[0] > 1 else width)
+    pitch = t2.stride(0) if t2.shape[0] > 1 else width
+    span = (t2.shape[0] - 1) * pitch + width
+    if span * t2.element_size() < 16:  # the kernels read 16 bytes at a time
+        t2 = torch.cat([t2.as_strided((span,), (1,)), t2.new_zeros(16 // t2.element_size())])
+    return t2, pitch
 
 
 class _LinearAct(torch.autograd.Function):
@@ -1834,7 +1838,7 @@ class _LinearAct(torch.autograd.Function):
             x2, xp = _rows(x, K)
             r2, rp = _rows(residual, N) if residual is not None else (None, 0)
             with _on_device(dev):
-                _run(lib.fsgs_linear_fwd, (x2.shape[0], K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), act,
+                _run(lib.fsgs_linear_fwd, (x.numel() // K, K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), act,
                                            r2.data_ptr() if r2 is not None else None, rp, ptr(y), stream_ptr(dev)),
                      "fsgs_linear_fwd")
         ctx.save_for_backward(x, weight, bias)

@@ -1080,7 +1080,8 @@ int64_t fsgs_step_plan_bytes(void); /* sizeof(fsgs_step_plan): a binding checks 
 /* ---- semantic head: one layer, forward and backward -----------------------------------------------------------------
  * y = act(x W^T + b) + r.  x [rows, in] with rows `x_pitch` elements apart (0: one row for all), w [out, in] contiguous,
  * bias [out] nullable, residual [rows, out] (pitch res_pitch) nullable, y [rows, out] contiguous.  All of one element type;
- * products in that type on the matrix cores, sums fp32.  No pointer has to be aligned beyond its element. */
+ * products in that type on the matrix cores, sums fp32.  No pointer has to be aligned beyond its element; x, residual and dy
+ * are read in 16-byte pieces between their first and last element, and a matrix of fewer bytes than that must have 16 readable. */
 #define FSGS_F32 0
 #define FSGS_BF16 1
 #define FSGS_F16 2
