@@ -47,6 +47,12 @@ struct RowReader {
     __device__ RowReader(const void *base, int64_t rows, int64_t pitch_, int width)
         : p((const T *)base), pitch(pitch_), lim(max((rows - 1) * pitch_ + width - kChunk<T>, (int64_t)0)) {}
     __device__ __forceinline__ Chunk raw(int64_t at) const { return load_chunk(p + min(at, lim)); }
+    // A chunk known to lie inside: `from` (the same for the whole wave) plus a byte offset, no address arithmetic per lane.
+    __device__ __forceinline__ Chunk inside(int64_t from, uint32_t offset) const {
+        Chunk c;
+        __builtin_memcpy(&c, (const char *)(p + from) + offset, sizeof(Chunk));
+        return c;
+    }
     // may_end: some lane's chunk may reach the matrix' end (the same for the whole wave)
     __device__ __forceinline__ void fix(Chunk &c, int64_t at, int valid, bool may_end) const {
         constexpr int CE = kChunk<T>;

@@ -149,7 +149,7 @@ __device__ __forceinline__ void put_chunk(T *to, const Chunk &c, int n, bool str
 // operand, so that a lane ends with neighbouring columns of one row.  Slab rows are two to the 64 banks: chunk c of row r lies
 // at c ^ key(r), with a key that gives the 16 rows of either operand 16 different bank quads.
 template <typename T, int MODE, int BN, int MT>
-__global__ __launch_bounds__(256, 2) void linear_tile_kernel(LinArgs a) {
+__global__ __launch_bounds__(256, 3) void linear_tile_kernel(LinArgs a) {
     constexpr int CE = kChunk<T>, BK = kSlabBytes / (int)sizeof(T), BM = 32 * MT;
     constexpr int NT = BN / 32;
     constexpr int XL = BM * 8 / 256, WL = BN * 8 / 256;  // chunks per thread and slab
@@ -163,61 +163,80 @@ __global__ __launch_bounds__(256, 2) void linear_tile_kernel(LinArgs a) {
     const int n0 = (int)(tile % ntiles_n) * BN;
     const int wm = (wave & 1) * 16 * MT, wn = (wave >> 1) * (BN / 2);
     const int li = lane & 15, lg = lane >> 4;
+    // (keys depend on the row modulo 32: one per thread for its stores, one per lane and operand for its reads)
     auto xkey = [](int r) { return (r >> 1) & 7; };
     auto wkey = [](int r) { return sizeof(T) == 2 ? ((r >> 3) & 3) << 1 | ((r >> 1) & 1) : (r >> 1) & 7; };
+    const int trow = tid >> 3, ck = (tid & 7) * CE;
+    Chunk *const xput = xs + trow * 8 + ((tid & 7) ^ xkey(trow)), *const wput = ws + trow * 8 + ((tid & 7) ^ wkey(trow));
+    const int xr0 = wm + li, wr0 = wn + group_column<T>(0, li);
 
     const RowReader<T> xr(a.x, a.rows, a.xp, a.K), wr(a.w, a.N, a.K, a.K);
-    const bool end = m0 + BM + kEndRows >= a.rows || n0 + BN + kEndRows >= a.N || a.xp == 0;
     f32x4 acc[NT][MT] = {};
     Chunk xc[XL], wc[WL];
-    const int ck = (tid & 7) * CE;
-    auto xrow = [&](int i) { return min(m0 + (tid >> 3) + i * 32, a.rows - 1); };
-    auto wrow = [&](int i) { return (int64_t)min(n0 + (tid >> 3) + i * 32, a.N - 1); };
-    auto fetch = [&](int k0) {
+    auto xrow = [&](int i) { return (int)min((int64_t)(trow + i * 32), a.rows - 1 - m0); };  // (rows behind the last repeat it,
+    auto wrow = [&](int i) { return min(trow + i * 32, a.N - 1 - n0); };                     //  unstored)
+    auto stage = [&] {
+        lds_barrier();
 #pragma unroll
-        for (int i = 0; i < XL; ++i) xc[i] = xr.raw(xrow(i) * a.xp + k0 + ck);
+        for (int i = 0; i < XL; ++i) xput[i * 256] = xc[i];
 #pragma unroll
-        for (int i = 0; i < WL; ++i) wc[i] = wr.raw(wrow(i) * a.K + k0 + ck);
+        for (int i = 0; i < WL; ++i) wput[i * 256] = wc[i];
+        lds_barrier();
     };
-    fetch(0);
-    for (int k0 = 0; k0 < a.K; k0 += BK) {
-        if (k0 + BK > a.K || end) {  // (rows behind the last repeat it: their results are not stored)
-#pragma unroll
-            for (int i = 0; i < XL; ++i) xr.fix(xc[i], xrow(i) * a.xp + k0 + ck, a.K - k0 - ck, end);
-#pragma unroll
-            for (int i = 0; i < WL; ++i) wr.fix(wc[i], wrow(i) * a.K + k0 + ck, a.K - k0 - ck, end);
-        }
-        lds_barrier();
-#pragma unroll
-        for (int i = 0; i < XL; ++i) {
-            const int r = (tid >> 3) + i * 32;
-            xs[r * 8 + ((tid & 7) ^ xkey(r))] = xc[i];
-        }
-#pragma unroll
-        for (int i = 0; i < WL; ++i) {
-            const int r = (tid >> 3) + i * 32;
-            ws[r * 8 + ((tid & 7) ^ wkey(r))] = wc[i];
-        }
-        lds_barrier();
-        if (k0 + BK < a.K) fetch(k0 + BK);
+    auto multiply = [&] {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             Chunk xf[MT], wf[NT];
+            const Chunk *const xg = xs + xr0 * 8 + ((s * 4 + lg) ^ xkey(xr0));
+            const Chunk *const wg = ws + wr0 * 8 + ((s * 4 + lg) ^ wkey(wr0));
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int r = wn + (i >> 1) * 32 + group_column<T>(i & 1, li);
-                wf[i] = ws[r * 8 + ((s * 4 + lg) ^ wkey(r))];
-            }
+            for (int i = 0; i < NT; ++i) wf[i] = wg[(i >> 1) * 256 + (i & 1) * (sizeof(T) == 2 ? 32 : 128)];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int r = wm + i * 16 + li;
-                xf[i] = xs[r * 8 + ((s * 4 + lg) ^ xkey(r))];
-            }
+            for (int i = 0; i < MT; ++i) xf[i] = xg[i * 128];
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int j = 0; j < MT; ++j) mma_chunk<T>(acc[i][j], wf[i], xf[j]);
         }
+    };
+    // whole slabs, byte offsets inside the tile in 32 bits; then what is left of the summed axis (or all of it, where rows lie
+    // too far apart for that)
+    const int kfull = a.xp * BM * (int64_t)sizeof(T) > UINT32_MAX ? 0 : a.K / BK * BK;
+    if (kfull > 0) {
+        uint32_t xo[XL], wo[WL];
+#pragma unroll
+        for (int i = 0; i < XL; ++i) xo[i] = (uint32_t)((xrow(i) * a.xp + ck) * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < WL; ++i) wo[i] = (uint32_t)((wrow(i) * (int64_t)a.K + ck) * sizeof(T));
+        auto fetch = [&](int k0) {
+#pragma unroll
+            for (int i = 0; i < XL; ++i) xc[i] = xr.inside(m0 * a.xp + k0, xo[i]);
+#pragma unroll
+            for (int i = 0; i < WL; ++i) wc[i] = wr.inside((int64_t)n0 * a.K + k0, wo[i]);
+        };
+        fetch(0);
+        for (int k0 = 0; k0 < kfull; k0 += BK) {
+            stage();
+            fetch(min(k0 + BK, kfull - BK));
+            multiply();
+        }
+    }
+    for (int k0 = kfull; k0 < a.K; k0 += BK) {
+        const bool end = m0 + BM + kEndRows >= a.rows || n0 + BN + kEndRows >= a.N || a.xp == 0;
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const int64_t at = (m0 + xrow(i)) * a.xp + k0 + ck;
+            xc[i] = xr.raw(at);
+            xr.fix(xc[i], at, a.K - k0 - ck, end);
+        }
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+            const int64_t at = (int64_t)(n0 + wrow(i)) * a.K + k0 + ck;
+            wc[i] = wr.raw(at);
+            wr.fix(wc[i], at, a.K - k0 - ck, end);
+        }
+        stage();
+        multiply();
     }
 
     const T *bias = (const T *)a.bias;
@@ -700,43 +719,26 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
     const bool want_b = a.part_b && k0 == 0 && wk == 0;
 
     const RowReader<T> dr(a.dz, a.rows, a.dzp, a.N), xr(a.x, a.rows, a.xp, a.K);
-    const bool ragged = n0 + kDwTile > a.N || k0 + kDwTile > a.K;
     const int crow = tid / CPR, col = tid % CPR * CE;  // this thread's first chunk of a slab
+    constexpr int RSTEP = 256 / CPR;
     Chunk dc[L], xc[L];
-    auto fetch = [&](int64_t m0) {
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int64_t m = min(m0 + crow + i * (256 / CPR), a.rows - 1);
-            dc[i] = dr.raw(m * a.dzp + n0 + col);
-            xc[i] = xr.raw(m * a.xp + k0 + col);
-        }
-    };
     f32x4 acc[4][4] = {}, accb[4] = {};
     T one[CE];
 #pragma unroll
     for (int e = 0; e < CE; ++e) one[e] = (T)1.f;
     Chunk ones;
     __builtin_memcpy(&ones, one, sizeof(Chunk));
-    if (mb < me) fetch(mb);
-    for (int64_t m0 = mb; m0 < me; m0 += ROWS) {
-        const bool end = m0 + ROWS + kEndRows >= a.rows;
-        if (ragged || end || m0 + ROWS > me) {
-#pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const int64_t mi = m0 + crow + i * (256 / CPR), m = min(mi, a.rows - 1);
-                dr.fix(dc[i], m * a.dzp + n0 + col, mi < me ? a.N - n0 - col : 0, end || a.dzp == 0);
-                xr.fix(xc[i], m * a.xp + k0 + col, mi < me ? a.K - k0 - col : 0, end || a.xp == 0);
-            }
-        }
+    auto stage = [&] {
         lds_barrier();
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int at = (crow + i * (256 / CPR)) * PITCH + col * (int)sizeof(T);
+            const int at = (crow + i * RSTEP) * PITCH + col * (int)sizeof(T);
             *(Chunk *)(dm + at) = dc[i];
             *(Chunk *)(xm + at) = xc[i];
         }
         lds_barrier();
-        if (m0 + ROWS < me) fetch(m0 + ROWS);
+    };
+    auto multiply = [&] {
         const int lc = sizeof(T) == 2 ? (li & 3) * 4 : li;
         if (nt == 4 && kt == 4 && !want_b) {
 #pragma unroll
@@ -771,6 +773,47 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
                     }
             }
         }
+    };
+    // Columns behind N or K read what follows the row; their sums are not stored.  So whole slabs need no care as long as that
+    // still lies in the matrix; the others (the last ones, or all, where rows lie too far apart for 32-bit offsets) do.
+    auto whole = [&](int64_t m1) {  // the slab that ends before row m1
+        return (m1 - 1) * a.dzp + n0 + kDwTile <= dr.lim + CE && (m1 - 1) * a.xp + k0 + kDwTile <= xr.lim + CE;
+    };
+    int64_t mfull = mb + (me - mb) / ROWS * ROWS;
+    if (me <= mb || max(a.dzp, a.xp) * ROWS * (int64_t)sizeof(T) > UINT32_MAX) mfull = mb;
+    while (mfull > mb && !whole(mfull)) mfull -= ROWS;
+    if (mfull > mb) {
+        uint32_t dof[L], xof[L];
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            dof[i] = (uint32_t)(((crow + i * RSTEP) * a.dzp + col) * sizeof(T));
+            xof[i] = (uint32_t)(((crow + i * RSTEP) * a.xp + col) * sizeof(T));
+        }
+        auto fetch = [&](int64_t m0) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                dc[i] = dr.inside(m0 * a.dzp + n0, dof[i]);
+                xc[i] = xr.inside(m0 * a.xp + k0, xof[i]);
+            }
+        };
+        fetch(mb);
+        for (int64_t m0 = mb; m0 < mfull; m0 += ROWS) {
+            stage();
+            fetch(min(m0 + ROWS, mfull - ROWS));
+            multiply();
+        }
+    }
+    for (int64_t m0 = mfull; m0 < me; m0 += ROWS) {
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int64_t mi = m0 + crow + i * RSTEP, m = min(mi, a.rows - 1);
+            dc[i] = dr.raw(m * a.dzp + n0 + col);
+            xc[i] = xr.raw(m * a.xp + k0 + col);
+            dr.fix(dc[i], m * a.dzp + n0 + col, mi < me ? a.N - n0 - col : 0, true);
+            xr.fix(xc[i], m * a.xp + k0 + col, mi < me ? a.K - k0 - col : 0, true);
+        }
+        stage();
+        multiply();
     }
     float *pw = a.part_w ? a.part_w + (int64_t)slice * a.N * a.K : nullptr;
 #pragma unroll
