@@ -209,7 +209,8 @@ SIGNATURES = {
     "fsgs_step_plan_bytes": (_i64, []),
     "fsgs_linear_fwd": (_i, [_i64, _i, _i, _i, _p, _i64, _p, _p, _i, _p, _i64, _p, _p]),
     "fsgs_linear_bwd_scratch_bytes": (_i64, [_i64, _i, _i, _i, _i, _i, _i, _i]),
-    "fsgs_linear_bwd": (_i, [_i64, _i, _i, _i, _p, _i64, _p, _p, _i, _p, _i64, _p, _p, _p, _p, _i64, _p]),
+    "fsgs_linear_bwd_uses_output": (_i, [_i64, _i, _i, _i, _i]),
+    "fsgs_linear_bwd": (_i, [_i64, _i, _i, _i, _p, _i64, _p, _p, _i, _p, _p, _i64, _p, _p, _p, _p, _i64, _p]),
     "fsgs_distill_scratch_bytes": (_i64, []),
     "fsgs_distill_fwd": (_i, [_i64, _i, _i, _i, _p, _i64, _i, _p, _i64, _i, _p, _i64, _p, _f, _i, _p, _p, _p, _p, _i64, _p]),
     "fsgs_distill_bwd": (_i, [_i64, _i, _i, _i, _p, _i64, _i, _p, _i64, _i, _p, _i64, _p, _f, _p, _p, _p, _i, _p, _p]),

@@ -676,6 +676,28 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
     }
 }
 
+// dz of a relu layer from its output: dy where y > 0 (exact, no product).  Rows of `width` elements; y and dz without gaps.
+template <typename T>
+__global__ __launch_bounds__(256) void relu_dz_kernel(const T *__restrict__ dy, int64_t dyp, const T *__restrict__ y,
+                                                      T *__restrict__ dz, int64_t rows, int64_t width) {
+    constexpr int CE = kChunk<T>;
+    const int64_t chunks = (width + CE - 1) / CE, total = rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = rows == 1 ? 0 : i / chunks, c = (i - r * chunks) * CE;
+        const int n = (int)min(width - c, (int64_t)CE);
+        const Chunk yc = load_chunk_n(y + r * width + c, n);
+        Chunk g = load_chunk_n(dy + r * dyp + c, n);
+        float yv[CE];
+        unpack_chunk<T>(yc, yv);
+        T gv[CE];
+        __builtin_memcpy(gv, &g, sizeof(Chunk));
+#pragma unroll
+        for (int e = 0; e < CE; ++e) gv[e] = yv[e] > 0.f ? gv[e] : (T)0.f;
+        __builtin_memcpy(&g, gv, sizeof(Chunk));
+        put_chunk(dz + r * width + c, g, n, false);
+    }
+}
+
 // W [N,K] -> W^T [K,N]: the operand of dx = dz W with its summed axis contiguous.
 template <typename T>
 __global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w, T *__restrict__ wt, int N, int K) {
@@ -1022,13 +1044,13 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
     l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
     l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
     l.part_b = l.part_w + (dw ? up(s * (size_t)K * N * 4) : 0);
-    const size_t sums = act != FSGS_ACT_NONE ? (size_t)dz_sum_rows(rows, K, e) : s;
+    const size_t sums = act != FSGS_ACT_NONE ? max((size_t)dz_sum_rows(rows, K, e), s) : s;
     l.total = l.part_b + (db ? up(sums * (size_t)N * 4) : 0);
     return l;
 }
 
 template <typename T>
-int run_bwd(LinArgs a, void *dx, void *dw, void *db, char *scratch, const BwdScratch &l, hipStream_t s) {
+int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratch, const BwdScratch &l, hipStream_t s) {
     const BwdRowsPlan p = bwd_rows_plan<T>(a.rows, a.K, a.N);
     if (p.kc) {
         BwdRowsArgs b = {};
@@ -1045,7 +1067,17 @@ int run_bwd(LinArgs a, void *dx, void *dw, void *db, char *scratch, const BwdScr
     int64_t dzp = a.dyp;
     float *part_w = dw ? (float *)(scratch + l.part_w) : nullptr, *part_b = db ? (float *)(scratch + l.part_b) : nullptr;
     int rc = FSGS_OK, sum_rows = 0;
-    if (a.act != FSGS_ACT_NONE) {
+    if (a.act == FSGS_ACT_RELU && y) {
+        const bool flat = a.dyp == a.N;
+        const int64_t rows = flat ? 1 : a.rows, width = flat ? a.rows * a.N : a.N;
+        const int64_t blocks = (rows * ((width + kChunk<T> - 1) / kChunk<T>) + 255) / 256;
+        T *to = (T *)(scratch + l.dz);
+        relu_dz_kernel<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>((const T *)a.dy, a.dyp, (const T *)y, to, rows,
+                                                                                   width);
+        rc = check_launch();
+        if (rc != FSGS_OK) return rc;
+        dz = to, dzp = a.N;
+    } else if (a.act != FSGS_ACT_NONE) {
         // (the sums of db are taken here, before dz is rounded to T)
         LinArgs z = a;
         z.y = scratch + l.dz, z.yp = a.N, z.part_b = part_b;
@@ -1110,6 +1142,11 @@ extern "C" int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype,
     }
 }
 
+extern "C" int fsgs_linear_bwd_uses_output(int64_t rows, int in_dim, int out_dim, int dtype, int act) {
+    if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
+    return act == FSGS_ACT_RELU && bwd_rows_plan(rows, in_dim, out_dim, dtype == FSGS_F32 ? 4 : 2).kc == 0;
+}
+
 extern "C" int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int act, int want_dx,
                                                  int want_dw, int want_db) {
     if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
@@ -1117,8 +1154,8 @@ extern "C" int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int o
 }
 
 extern "C" int fsgs_linear_bwd(int64_t rows, int in_dim, int out_dim, int dtype, const void *x, int64_t x_pitch, const void *w,
-                               const void *bias, int act, const void *dy, int64_t dy_pitch, void *dx, void *dw, void *db,
-                               void *scratch, int64_t scratch_bytes, fsgs_stream_t stream) {
+                               const void *bias, int act, const void *y, const void *dy, int64_t dy_pitch, void *dx, void *dw,
+                               void *db, void *scratch, int64_t scratch_bytes, fsgs_stream_t stream) {
     if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
     if (rows == 0 || (!dx && !dw && !db)) return FSGS_OK;
     if (!x || !w || !dy || x_pitch < 0 || dy_pitch < 0) return FSGS_EINVAL;
@@ -1128,8 +1165,8 @@ extern "C" int fsgs_linear_bwd(int64_t rows, int in_dim, int out_dim, int dtype,
     a.x = x, a.xp = x_pitch, a.w = w, a.bias = bias, a.dy = dy, a.dyp = dy_pitch;
     a.rows = rows, a.K = in_dim, a.N = out_dim, a.act = act;
     switch (dtype) {
-        case FSGS_F32: return run_bwd<float>(a, dx, dw, db, (char *)scratch, l, as_stream(stream));
-        case FSGS_BF16: return run_bwd<__bf16>(a, dx, dw, db, (char *)scratch, l, as_stream(stream));
-        default: return run_bwd<_Float16>(a, dx, dw, db, (char *)scratch, l, as_stream(stream));
+        case FSGS_F32: return run_bwd<float>(a, y, dx, dw, db, (char *)scratch, l, as_stream(stream));
+        case FSGS_BF16: return run_bwd<__bf16>(a, y, dx, dw, db, (char *)scratch, l, as_stream(stream));
+        default: return run_bwd<_Float16>(a, y, dx, dw, db, (char *)scratch, l, as_stream(stream));
     }
 }

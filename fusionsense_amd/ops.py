@@ -1841,14 +1841,17 @@ class _LinearAct(torch.autograd.Function):
                 _run(lib.fsgs_linear_fwd, (x.numel() // K, K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), act,
                                            r2.data_ptr() if r2 is not None else None, rp, ptr(y), stream_ptr(dev)),
                      "fsgs_linear_fwd")
-        ctx.save_for_backward(x, weight, bias)
+        # (a wide relu layer takes its slope from the output's sign instead of forming the pre-activation again)
+        keep = (act == ACTIVATIONS["relu"] and residual is None and any(ctx.needs_input_grad[:3])
+                and lib.fsgs_linear_bwd_uses_output(x.numel() // K, K, N, DTYPES[x.dtype], act) == 1)
+        ctx.save_for_backward(x, weight, bias, y if keep else None)
         ctx.act = act
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors
+        x, weight, bias, y = ctx.saved_tensors
         lib = load()
         dev = x.device
         N, K = weight.shape
@@ -1867,7 +1870,7 @@ class _LinearAct(torch.autograd.Function):
                                                            int(need_b))
                 scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
                 _run(lib.fsgs_linear_bwd, (rows, K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), ctx.act,
-                                           g2.data_ptr(), gp, ptr(dx), ptr(dw), ptr(db), ptr(scratch), nbytes,
+                                           ptr(y), g2.data_ptr(), gp, ptr(dx), ptr(dw), ptr(db), ptr(scratch), nbytes,
                                            stream_ptr(dev)), "fsgs_linear_bwd")
         return dx, dw, db, (dy if need_r else None), None
 

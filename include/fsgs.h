@@ -1093,12 +1093,15 @@ int64_t fsgs_step_plan_bytes(void); /* sizeof(fsgs_step_plan): a binding checks 
 int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype, const void *x, int64_t x_pitch, const void *w,
                     const void *bias, int act, const void *residual, int64_t res_pitch, void *y, fsgs_stream_t stream);
 /* VJP.  dx [rows, in], dw [out, in], db [out]: contiguous, written, each nullable (rows == 0 writes nothing: dw and db are
- * the caller's to clear).  The pre-activation is formed again from x, w and bias.  The residual's gradient is dy itself. */
+ * the caller's to clear).  The pre-activation is formed again from x, w and bias.  The residual's gradient is dy itself.
+ * y: nullable; the forward's output [rows, out] (contiguous) of a layer WITHOUT residual.  Where
+ * fsgs_linear_bwd_uses_output says 1 (relu layers too wide for the one-pass kernel) its sign saves that product. */
+int fsgs_linear_bwd_uses_output(int64_t rows, int in_dim, int out_dim, int dtype, int act);
 int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int act, int want_dx, int want_dw,
                                       int want_db);
 int fsgs_linear_bwd(int64_t rows, int in_dim, int out_dim, int dtype, const void *x, int64_t x_pitch, const void *w,
-                    const void *bias, int act, const void *dy, int64_t dy_pitch, void *dx, void *dw, void *db, void *scratch,
-                    int64_t scratch_bytes, fsgs_stream_t stream);
+                    const void *bias, int act, const void *y, const void *dy, int64_t dy_pitch, void *dx, void *dw, void *db,
+                    void *scratch, int64_t scratch_bytes, fsgs_stream_t stream);
 
 /* ---- distillation from a teacher's top-K scores ---------------------------------------------------------------------
  * p = softmax over the row's K entries of teacher / T, q = softmax over all classes of logits / T,

@@ -57,16 +57,19 @@ def test_linear_fwd_entry_refuses(kw):
 
 def test_linear_entries_without_rows_return_at_once():
     assert _fwd(rows=0, x=None, w=None, y=None) == 0
-    assert _lib.load().fsgs_linear_bwd(0, 8, 8, 0, None, 8, None, None, 0, None, 8, None, None, None, None, 0, None) == 0
+    assert _lib.load().fsgs_linear_bwd(0, 8, 8, 0, None, 8, None, None, 0, None, None, 8, None, None, None, None, 0, None) == 0
 
 
 def test_linear_bwd_entry_refuses():
     lib = _lib.load()
 
     def bwd(rows=4, k=8, n=8, dt=0, x=ONE, act=1, dy=ONE, dyp=8, scratch=ONE, nbytes=1 << 40):
-        return lib.fsgs_linear_bwd(rows, k, n, dt, x, 8, ONE, None, act, dy, dyp, ONE, ONE, ONE, scratch, nbytes, None)
+        return lib.fsgs_linear_bwd(rows, k, n, dt, x, 8, ONE, None, act, None, dy, dyp, ONE, ONE, ONE, scratch, nbytes, None)
     for kw in (dict(rows=-1), dict(k=0), dict(dt=7), dict(act=9), dict(x=None), dict(dy=None), dict(dyp=-1), dict(rows=1 << 40)):
         assert bwd(**kw) == -1, kw
+    assert lib.fsgs_linear_bwd_uses_output(4, 0, 8, 0, 1) == -1
+    assert lib.fsgs_linear_bwd_uses_output(4, 8, 8, 0, 1) == 0 and lib.fsgs_linear_bwd_uses_output(4, 600, 700, 1, 1) == 1
+    assert lib.fsgs_linear_bwd_uses_output(4, 600, 700, 1, 2) == 0
     need = lib.fsgs_linear_bwd_scratch_bytes(4, 8, 8, 0, 1, 1, 1, 1)
     assert need > 0
     assert bwd(nbytes=need - 1) == -3 and bwd(scratch=None) == -3
