@@ -7,7 +7,6 @@ all arithmetic happens in libfsgs.so.  There is no CPU fallback.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
 import os
@@ -1802,26 +1801,45 @@ DISTILL_MAX_CLASSES = 524288
 DISTILL_T_RANGE = (1e-6, 1e6)
 
 
-def _on_device(dev: torch.device):
-    """The tensors' device as the current one: a launch on another device's stream is an error.  (No cost where it is.)"""
+def _run_on(dev: torch.device, fn, args, what: str) -> None:
+    """_run with the tensors' device as the current one: a launch on another device's stream is an error."""
     if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+        _run(fn, args, what)
+    else:
+        with torch.cuda.device(dev):
+            _run(fn, args, what)
 
 
 def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
     """``t`` [..., width] -> (tensor whose storage the kernels read, elements between two rows).  A tensor whose rows lie at
     one pitch (a slice of a wider plane, an expanded row) is read in place, any other is copied once."""
-    if t.numel() == 0:
-        return t, width
-    t2 = t.reshape(-1, width)
-    if width > 1 and t2.stride(1) != 1:
-        t2 = t2.contiguous()
-    pitch = t2.stride(0) if t2.shape[0] > 1 else width
-    span = (t2.shape[0] - 1) * pitch + width
-    if span * t2.element_size() < 16:  # the kernels read 16 bytes at a time
-        t2 = torch.cat([t2.as_strided((span,), (1,)), t2.new_zeros(16 // t2.element_size())])
-    return t2, pitch
+    if t.dim() != 2:
+        t = t.reshape(-1, width) if t.numel() > 0 else t.new_empty(0, width)
+    if width > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else width)
+
+
+def _rows16(t: Tensor, width: int) -> Tuple[Tensor, int]:
+    """_rows for the layer kernels, which read 16 bytes at a time: a matrix of less is copied to where that many are readable."""
+    t, pitch = _rows(t, width)
+    span = (t.shape[0] - 1) * pitch + width
+    if span * t.element_size() < 16:
+        t = torch.cat([t.as_strided((span,), (1,)), t.new_zeros(16 // t.element_size())])
+    return t, pitch
+
+
+def _linear_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], act: int) -> Tensor:
+    N, K = weight.shape
+    dev = x.device
+    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
+    if y.numel() > 0:
+        x2, xp = _rows16(x, K)
+        r2, rp = _rows16(residual, N) if residual is not None else (None, 0)
+        _run_on(dev, load().fsgs_linear_fwd, (x.numel() // K, K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias),
+                                              act, r2.data_ptr() if r2 is not None else None, rp, y.data_ptr(),
+                                              stream_ptr(dev)), "fsgs_linear_fwd")
+    return y
 
 
 class _LinearAct(torch.autograd.Function):
@@ -1829,21 +1847,11 @@ class _LinearAct(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        lib = load()
-        dev = x.device
-        N, K = weight.shape
-        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
-        weight, bias = _c(weight), _c(bias)
-        if y.numel() > 0:
-            x2, xp = _rows(x, K)
-            r2, rp = _rows(residual, N) if residual is not None else (None, 0)
-            with _on_device(dev):
-                _run(lib.fsgs_linear_fwd, (x.numel() // K, K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), act,
-                                           r2.data_ptr() if r2 is not None else None, rp, ptr(y), stream_ptr(dev)),
-                     "fsgs_linear_fwd")
+        y = _linear_fwd(x, weight, bias, residual, act)
         # (a wide relu layer takes its slope from the output's sign instead of forming the pre-activation again)
+        N, K = weight.shape
         keep = (act == ACTIVATIONS["relu"] and residual is None and any(ctx.needs_input_grad[:3])
-                and lib.fsgs_linear_bwd_uses_output(x.numel() // K, K, N, DTYPES[x.dtype], act) == 1)
+                and load().fsgs_linear_bwd_uses_output(x.numel() // K, K, N, DTYPES[x.dtype], act) == 1)
         ctx.save_for_backward(x, weight, bias, y if keep else None)
         ctx.act = act
         return y
@@ -1863,15 +1871,14 @@ class _LinearAct(torch.autograd.Function):
         dw = new(N, K, dtype=x.dtype, device=dev) if need_w else None
         db = new(N, dtype=x.dtype, device=dev) if need_b else None
         if rows > 0 and (need_x or need_w or need_b):
-            x2, xp = _rows(x, K)
-            g2, gp = _rows(dy, N)
-            with _on_device(dev):
-                nbytes = lib.fsgs_linear_bwd_scratch_bytes(rows, K, N, DTYPES[x.dtype], ctx.act, int(need_x), int(need_w),
-                                                           int(need_b))
-                scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-                _run(lib.fsgs_linear_bwd, (rows, K, N, DTYPES[x.dtype], x2.data_ptr(), xp, ptr(weight), ptr(bias), ctx.act,
-                                           ptr(y), g2.data_ptr(), gp, ptr(dx), ptr(dw), ptr(db), ptr(scratch), nbytes,
-                                           stream_ptr(dev)), "fsgs_linear_bwd")
+            x2, xp = _rows16(x, K)
+            g2, gp = _rows16(dy, N)
+            dt = DTYPES[x.dtype]
+            nbytes = lib.fsgs_linear_bwd_scratch_bytes(rows, K, N, dt, ctx.act, need_x, need_w, need_b)
+            scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+            _run_on(dev, lib.fsgs_linear_bwd, (rows, K, N, dt, x2.data_ptr(), xp, ptr(weight), ptr(bias), ctx.act, ptr(y),
+                                               g2.data_ptr(), gp, ptr(dx), ptr(dw), ptr(db), scratch.data_ptr(), nbytes,
+                                               stream_ptr(dev)), "fsgs_linear_bwd")
         return dx, dw, db, (dy if need_r else None), None
 
 
@@ -1912,56 +1919,67 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
         raise ValueError(f"residual must be {tuple(x.shape[:-1] + (N,))}, got {tuple(residual.shape)}")
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
-    return _LinearAct.apply(x, weight, bias, residual, ACTIVATIONS[act])
+    weight, bias = weight.contiguous(), _c(bias)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _LinearAct.apply(x, weight, bias, residual, ACTIVATIONS[act])
+    return _linear_fwd(x, weight, bias, residual, ACTIVATIONS[act])
+
+
+def _distill_fwd(logits, idx, teacher, weight, temperature: float, reduction: int, grad: bool):
+    """(loss, what the backward needs: idx, teacher, weight as they were read and the row statistics)."""
+    lib = load()
+    dev = logits.device
+    V, K = logits.shape[-1], idx.shape[-1]
+    rows = idx.numel() // K
+    per_row = reduction == 0
+    loss = torch.empty(logits.shape[:-1] if per_row else (), dtype=torch.float32, device=dev)
+    s2, sp = _rows(logits, V)
+    i2, ip = _rows(idx, K)
+    t2, tp = _rows(teacher, K)
+    if weight is not None:
+        weight = weight.reshape(-1).contiguous()
+    # one buffer: what the backward needs (row statistics, then 1 / sum of the weights), and behind it the reduction's scratch
+    keep = 4 * rows + 4 if grad else 0
+    nbytes = 0 if per_row else lib.fsgs_distill_scratch_bytes()
+    buf = torch.empty(keep + nbytes // 4, dtype=torch.float32, device=dev)
+    at = buf.data_ptr()
+    stat, inv_w = (at, None if per_row else at + 16 * rows) if keep else (None, None)
+    _run_on(dev, lib.fsgs_distill_fwd, (rows, V, K, DTYPES[logits.dtype], s2.data_ptr(), sp,
+                                        64 if idx.dtype == torch.int64 else 32, i2.data_ptr(), ip, DTYPES[teacher.dtype],
+                                        t2.data_ptr(), tp, ptr(weight), temperature, reduction, loss.data_ptr(), stat, inv_w,
+                                        at + 4 * keep if nbytes else None, nbytes, stream_ptr(dev)), "fsgs_distill_fwd")
+    return loss, (i2, t2, weight, buf[:keep])
 
 
 class _TopkDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, idx, teacher, weight, temperature, reduction):
-        lib = load()
-        dev = logits.device
-        V, K = logits.shape[-1], idx.shape[-1]
-        rows = idx.numel() // K
-        per_row = reduction == REDUCTIONS["none"]
-        loss = torch.empty(logits.shape[:-1] if per_row else (), dtype=torch.float32, device=dev)
-        need = ctx.needs_input_grad[0]
-        stat = torch.empty(rows, 4, dtype=torch.float32, device=dev) if need else None
-        inv_w = torch.empty(1, dtype=torch.float32, device=dev) if need and not per_row else None
-        s2, sp = _rows(logits, V)
-        i2, ip = _rows(idx, K)
-        t2, tp = _rows(teacher, K)
-        w1 = weight.reshape(-1).contiguous() if weight is not None else None
-        with _on_device(dev):
-            nbytes = 0 if per_row else lib.fsgs_distill_scratch_bytes()
-            scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-            _run(lib.fsgs_distill_fwd, (rows, V, K, DTYPES[logits.dtype], s2.data_ptr(), sp, 64 if idx.dtype == torch.int64 else 32,
-                                        i2.data_ptr(), ip, DTYPES[teacher.dtype], t2.data_ptr(), tp, ptr(w1), temperature,
-                                        reduction, loss.data_ptr(), ptr(stat), ptr(inv_w), ptr(scratch), nbytes,
-                                        stream_ptr(dev)), "fsgs_distill_fwd")
-        ctx.save_for_backward(logits, idx, teacher, w1, stat, inv_w)
-        ctx.cfg = (temperature, per_row)
+        loss, keep = _distill_fwd(logits, idx, teacher, weight, temperature, reduction, True)
+        ctx.save_for_backward(logits, *keep)
+        ctx.cfg = temperature, reduction == 0
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        logits, idx, teacher, w1, stat, inv_w = ctx.saved_tensors
+        logits, idx, teacher, weight, buf = ctx.saved_tensors
         temperature, per_row = ctx.cfg
-        lib = load()
         dev = logits.device
-        V, K = logits.shape[-1], idx.shape[-1]
-        rows = idx.numel() // K
+        (rows, K), V = idx.shape, logits.shape[-1]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         if rows > 0:
             s2, sp = _rows(logits, V)
             i2, ip = _rows(idx, K)
             t2, tp = _rows(teacher, K)
-            g1 = g.reshape(-1).contiguous()
-            with _on_device(dev):
-                _run(lib.fsgs_distill_bwd, (rows, V, K, DTYPES[logits.dtype], s2.data_ptr(), sp,
-                                            64 if idx.dtype == torch.int64 else 32, i2.data_ptr(), ip, DTYPES[teacher.dtype],
-                                            t2.data_ptr(), tp, ptr(w1), temperature, ptr(stat), ptr(inv_w), ptr(g1),
-                                            int(per_row), ptr(grad), stream_ptr(dev)), "fsgs_distill_bwd")
+            if per_row:
+                g = g.reshape(-1).contiguous()
+            at = buf.data_ptr()
+            _run_on(dev, load().fsgs_distill_bwd, (rows, V, K, DTYPES[logits.dtype], s2.data_ptr(), sp,
+                                                   64 if idx.dtype == torch.int64 else 32, i2.data_ptr(), ip,
+                                                   DTYPES[teacher.dtype], t2.data_ptr(), tp, ptr(weight), temperature, at,
+                                                   None if per_row else at + 16 * rows, g.data_ptr(), int(per_row),
+                                                   grad.data_ptr(), stream_ptr(dev)), "fsgs_distill_bwd")
         return grad, None, None, None, None, None
 
 
@@ -1994,4 +2012,5 @@ def topk_distill(logits: Tensor, teacher_idx: Tensor, teacher_logits: Tensor, te
         raise ValueError(f"temperature must lie in {DISTILL_T_RANGE}, got {temperature}")
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(REDUCTIONS)}, got {reduction!r}")
-    return _TopkDistill.apply(logits, teacher_idx, teacher_logits, weight, temperature, REDUCTIONS[reduction])
+    args = logits, teacher_idx, teacher_logits, weight, temperature, REDUCTIONS[reduction]
+    return _TopkDistill.apply(*args) if torch.is_grad_enabled() and logits.requires_grad else _distill_fwd(*args, False)[0]

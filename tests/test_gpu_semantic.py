@@ -508,6 +508,21 @@ def test_head_and_loss_captured_and_on_another_stream(dev, dtype):
     assert all(torch.equal(x, y) for x, y in zip(got, [loss.detach()] + list(grads)))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_head_and_loss_with_saved_tensors_kept_on_the_host(dev, dtype):
+    """What the backward needs may come back in other storage and with other strides: the same bits."""
+    head = SemanticHead(32, 150, hidden=64, dtype=dtype, device=dev, generator=torch.Generator().manual_seed(0))
+    wide = _randn(dev, 333, 35, seed=1, dtype=dtype)
+    _, idx, top = _record(dev, 333, 150, 8, torch.float32, seed=2)
+    out = []
+    for hooks in (False, True):
+        feats = wide.clone().requires_grad_(True)
+        with torch.autograd.graph.save_on_cpu(pin_memory=False) if hooks else torch.enable_grad():
+            loss = losses.topk_distill_loss(head(feats[:, 1:33]), idx, top, 2.0)
+        out.append(torch.autograd.grad(loss, [feats] + list(head.parameters())))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
 def test_semantics_through_the_renderer(dev):
     """render_fusionsense with a head: the plane is the features' composite, the scores are the head's, the loss's gradient
     reaches the feature rows and the head and stops at the geometry; images are what they are without the head."""
