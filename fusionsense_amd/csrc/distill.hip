@@ -90,7 +90,8 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // shifted back to end with the row, its doubled elements masked: no element-wise reads, nothing behind the row.
 constexpr int kStep = 5;
 constexpr int kFullSteps = 2;  // with several lanes per row every row has more than kStep / 2 chunks a lane
-constexpr int kHeld = 2;  // entries per lane kept in registers; further ones are read again where they are needed
+template <int STEPS>
+constexpr int kHeldOf = STEPS == kStep ? 2 : 4;  // entries per lane kept in registers; further ones are read again where needed
 
 template <typename T, int L, int STEPS>
 __device__ __forceinline__ void load_step(Chunk (&c)[STEPS], const T *s, int c0, int V) {
@@ -163,7 +164,7 @@ struct RowExp {
 
 template <typename T, int L, int STEPS>
 __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel(DistillArgs a) {
-    constexpr int CE = kChunk<T>, ROWS = 256 / L;
+    constexpr int CE = kChunk<T>, ROWS = 256 / L, kHeld = kHeldOf<STEPS>;
     const int sub = threadIdx.x & (L - 1);
     const int chunks = (a.V + CE - 1) / CE;
     double sum_l = 0.0, sum_w = 0.0;
@@ -325,7 +326,7 @@ struct BwdLds {
 // class.  A row's lanes are one wave's, and LDS runs in a wave's order: no barrier.
 template <typename T, int L, int STEPS>
 __global__ __launch_bounds__(256, 5) void distill_bwd_kernel(DistillArgs a) {
-    constexpr int CE = kChunk<T>, ROWS = kWave / L;
+    constexpr int CE = kChunk<T>, ROWS = kWave / L, kHeld = kHeldOf<STEPS>;
     extern __shared__ Chunk lds[];
     const int lane = threadIdx.x & 63, sub = lane & (L - 1), group = lane / L;
     const BwdLds<T, L> lay(a.V);

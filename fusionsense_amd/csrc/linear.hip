@@ -902,6 +902,9 @@ int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
     const int row_bytes = rows_pitch<T, KC>() * 16 + 4;
     const int fit = kRowsLds / row_bytes / 32 * 32, need = (a.N + 31) / 32 * 32;
     r.range = need < fit ? need : fit;
+    // few rows: more, narrower ranges, whose weights are fetched side by side (one row, 64 -> 150 fp32: 7.0 -> 4.9 us)
+    while (r.range > 32 && (int64_t)rows_blocks(a.rows) * ((a.N + r.range - 1) / r.range) < 256)
+        r.range = (r.range / 2 + 31) / 32 * 32;
     const int ranges = (a.N + r.range - 1) / r.range;
     const bool sums = MODE == kModeDz && a.part_b;
     const size_t bytes = (size_t)r.range * (row_bytes + (sums ? 16 : 0));
