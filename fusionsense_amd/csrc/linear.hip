@@ -6,6 +6,8 @@
 //
 // Products run on the matrix cores in the tensors' own type, sums are fp32 throughout (fp32 tensors use the fp32 matrix
 // instructions: no reduced-precision product).
+#include <type_traits>
+
 #include "half_types.h"
 
 namespace fsgs {
@@ -536,7 +538,26 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
 #pragma unroll
             for (int c = 0; c < KC; ++c)
                 xr.fix(xf[c], mr * a.xp + (c * 4 + lg) * CE, m < a.rows ? a.K - (c * 4 + lg) * CE : 0, end || a.xp == 0);
-        f32x4 accx[KT] = {};
+        // dx^T tiles: rows k of a pair of tiles are 8 neighbours per lane in half width, 4 of one tile in fp32
+        auto add_dx = [&](f32x4 &acc, int kt, int g, const Chunk (&dz)[CPG]) {
+            const int col = CPG == 1 ? (kt >> 1) * 32 + (li & 3) * 8 + (kt & 1) * 4 : kt * 16 + li;
+#pragma unroll
+            for (int q = 0; q < CPG; ++q) {
+                const int n = column(g, q);
+                mma_chunk<T>(acc, load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col), dz[q]);
+            }
+        };
+        auto store_dx = [&](int kt, const f32x4 *acc) {
+            const int k = kt * 16 + lg * CE;
+            float v[CE];
+#pragma unroll
+            for (int e = 0; e < CE; ++e) v[e] = acc[e >> 2][e & 3];
+            if (m < a.rows && k < a.K) put_chunk((T *)a.dx + m * a.K + k, pack_chunk<T>(v), a.K - k, a.stream);
+        };
+        // whichever holds fewer registers meanwhile: dx summed group by group, or the groups' dz kept and dx done at the end
+        constexpr bool kKeepDz = KT > NG * CPG;
+        f32x4 accx[kKeepDz ? 1 : KT] = {};
+        Chunk dzc[kKeepDz ? NG : 1][CPG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             if (g >= ng) break;
@@ -568,33 +589,32 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
             if constexpr (kRegDb)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) db[g][e] += d[e];
-            Chunk dzc[CPG];
+            Chunk (&dz)[CPG] = dzc[kKeepDz ? g : 0];
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
-                dzc[q] = pack_chunk<T>(d + q * CE);
-                *(Chunk *)(mem + lay.dz + row * lay.pn + column(g, q) * (int)sizeof(T)) = dzc[q];
+                dz[q] = pack_chunk<T>(d + q * CE);
+                *(Chunk *)(mem + lay.dz + row * lay.pn + column(g, q) * (int)sizeof(T)) = dz[q];
             }
-            if (a.dx) {
+            if constexpr (!kKeepDz)
+                if (a.dx)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int q = 0; q < CPG; ++q) {
-                        // rows k of the tile: by pairs of tiles 8 neighbours per lane in half width, 4 in fp32
-                        const int col = CPG == 1 ? (kt >> 1) * 32 + (li & 3) * 8 + (kt & 1) * 4 : kt * 16 + li;
-                        const int n = column(g, q);
-                        mma_chunk<T>(accx[kt], load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col), dzc[q]);
-                    }
-            }
+                    for (int kt = 0; kt < KT; ++kt) add_dx(accx[kt], kt, g, dz);
         }
-        if (a.dx && m < a.rows) {
-            T *dst = (T *)a.dx + m * a.K;
+        if (a.dx) {
+            if constexpr (!kKeepDz) {
 #pragma unroll
-            for (int kt = 0; kt < KT; kt += 3 - CPG) {
-                const int k = kt * 16 + lg * CE;
-                float v[CE];
+                for (int kt = 0; kt < KT; kt += 3 - CPG) store_dx(kt, accx + kt);
+            } else {
 #pragma unroll
-                for (int e = 0; e < CE; ++e) v[e] = accx[kt + (e >> 2)][e & 3];
-                if (k < a.K) put_chunk(dst + k, pack_chunk<T>(v), a.K - k, a.stream);
+                for (int kt = 0; kt < KT; kt += 3 - CPG) {
+                    f32x4 acc[3 - CPG] = {};
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+                        if (g < ng)
+#pragma unroll
+                            for (int i = 0; i < 3 - CPG; ++i) add_dx(acc[i], kt + i, g, dzc[g]);
+                    store_dx(kt, acc);
+                }
             }
         }
         if (a.part_w) {
@@ -605,28 +625,35 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
         load_x(xf, nr);
         if (tiles) {
             lds_barrier();
-            constexpr int STEP = 4 * CE;  // rows per matrix instruction: 32, or 16 by four instructions
+            // (the wave's number of tiles compiled in: no branch between the steps)
+            auto add_dw = [&](auto tiles_of_wave) {
+                constexpr int STEP = 4 * CE;  // rows per matrix instruction: 32, or 16 by four instructions
 #pragma unroll
-            for (int s = 0; s < kBwdRows / STEP; ++s) {
-                const int lo = s * STEP + lg * 4, hi = lo + 16;
-                Chunk xc[KTW];
+                for (int s = 0; s < kBwdRows / STEP; ++s) {
+                    const int lo = s * STEP + lg * 4, hi = lo + 16;
+                    Chunk xc[KTW];
 #pragma unroll
-                for (int j = 0; j < KTW; ++j)
-                    xc[j] = load_columns<T>(mem + lay.x, lay.pk, lo, hi, (wk * KTW + j) * 16 + (CPG == 1 ? (li & 3) * 4 : li));
+                    for (int j = 0; j < KTW; ++j)
+                        xc[j] = load_columns<T>(mem + lay.x, lay.pk, lo, hi, (wk * KTW + j) * 16 + (CPG == 1 ? (li & 3) * 4 : li));
 #pragma unroll
-                for (int i = 0; i < NTW; ++i) {
-                    const int n = (i * WN + wn) * 16;
-                    if (n >= cols) break;
-                    const Chunk zc = load_columns<T>(mem + lay.dz, lay.pn, lo, hi, n + (CPG == 1 ? (li & 3) * 4 : li));
-                    if constexpr (!kRegDb) {
-                        float v[4];
-                        __builtin_memcpy(v, &zc, sizeof(v));
-                        accb[i] += (v[0] + v[1]) + (v[2] + v[3]);
+                    for (int i = 0; i < decltype(tiles_of_wave)::value; ++i) {
+                        const int n = (i * WN + wn) * 16;
+                        const Chunk zc = load_columns<T>(mem + lay.dz, lay.pn, lo, hi, n + (CPG == 1 ? (li & 3) * 4 : li));
+                        if constexpr (!kRegDb) {
+                            float v[4];
+                            __builtin_memcpy(v, &zc, sizeof(v));
+                            accb[i] += (v[0] + v[1]) + (v[2] + v[3]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < KTW; ++j) mma_chunk<T>(accw[i][j], zc, xc[j]);
                     }
-#pragma unroll
-                    for (int j = 0; j < KTW; ++j) mma_chunk<T>(accw[i][j], zc, xc[j]);
                 }
-            }
+            };
+            const int mine = (cols / 16 - wn + WN - 1) / WN;
+            if (mine >= NTW) add_dw(std::integral_constant<int, NTW>());
+            else if (NTW > 1 && mine == NTW - 1) add_dw(std::integral_constant<int, (NTW > 1 ? NTW - 1 : 0)>());
+            else if (NTW > 2 && mine == NTW - 2) add_dw(std::integral_constant<int, (NTW > 2 ? NTW - 2 : 0)>());
+            else if (NTW > 3 && mine == NTW - 3) add_dw(std::integral_constant<int, (NTW > 3 ? NTW - 3 : 0)>());
             lds_barrier();
         }
     }
