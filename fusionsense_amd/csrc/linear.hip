@@ -745,32 +745,32 @@ struct DwArgs {
     int K, N, slices;
 };
 
-// dW tile of 128 columns of dz x 128 columns of x over one slice of the rows, four waves of 64 x 64.  Slabs of 64 (fp32: 32)
+// dW tile over one slice of the rows: WN x WK waves (four) of 64 columns of dz x 64 columns of x.  Slabs of 64 (fp32: 32)
 // rows of both lie in LDS as they come and are read by columns; the next slab is under way in registers.  db beside it, where
 // dz is dy as it stands (tiles of k = 0: dz against ones).  Tiles of one slice, which share rows, go to one XCD.
-constexpr int kDwTile = 128;
-
-template <typename T>
+template <typename T, int WN, int WK>
 __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
-    constexpr int CE = kChunk<T>, ROWS = 128 / (int)sizeof(T), CPR = kDwTile / CE, L = ROWS * CPR / 256;
-    constexpr int PITCH = kDwTile * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16), STEP = 4 * CE;
-    __shared__ Chunk ds[ROWS * PITCH / 16], xs[ROWS * PITCH / 16];
+    static_assert(WN * WK == 4, "four waves");
+    constexpr int CE = kChunk<T>, ROWS = 128 / (int)sizeof(T), STEP = 4 * CE, BN = 64 * WN, BK = 64 * WK;
+    constexpr int DCPR = BN / CE, XCPR = BK / CE, DL = ROWS * DCPR / 256, XLD = ROWS * XCPR / 256;  // chunks a row, a thread
+    constexpr int PAD = sizeof(T) == 2 ? 32 : 16, DP = BN * (int)sizeof(T) + PAD, XP = BK * (int)sizeof(T) + PAD;
+    __shared__ Chunk ds[ROWS * DP / 16], xs[ROWS * XP / 16];
     char *const dm = (char *)ds, *const xm = (char *)xs;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
-    const int kts = a.part_w ? (a.K + kDwTile - 1) / kDwTile : 1, nts = (a.N + kDwTile - 1) / kDwTile;
+    const int kts = a.part_w ? (a.K + BK - 1) / BK : 1, nts = (a.N + BN - 1) / BN;
     const int64_t id = xcd_tile(blockIdx.x, (int64_t)a.slices * kts * nts);
     if (id < 0) return;
     const int slice = (int)(id / (kts * nts)), tile = (int)(id % (kts * nts));
-    const int k0 = tile % kts * kDwTile, n0 = tile / kts * kDwTile;
-    const int wn = (wave >> 1) * 64, wk = (wave & 1) * 64;
+    const int k0 = tile % kts * BK, n0 = tile / kts * BN;
+    const int wn = wave / WK * 64, wk = wave % WK * 64;
     const int nt = min(4, (a.N - n0 - wn + 15) / 16), kt = a.part_w ? min(4, (a.K - k0 - wk + 15) / 16) : 0;  // (may be < 1)
     const int64_t mb = slice * a.slice_rows, me = min(a.rows, mb + a.slice_rows);
     const bool want_b = a.part_b && k0 == 0 && wk == 0;
 
     const RowReader<T> dr(a.dz, a.rows, a.dzp, a.N), xr(a.x, a.rows, a.xp, a.K);
-    const int crow = tid / CPR, col = tid % CPR * CE;  // this thread's first chunk of a slab
-    constexpr int RSTEP = 256 / CPR;
-    Chunk dc[L], xc[L];
+    const int drow = tid / DCPR, dcol = tid % DCPR * CE, xrow = tid / XCPR, xcol = tid % XCPR * CE;  // first chunks of a slab
+    constexpr int DSTEP = 256 / DCPR, XSTEP = 256 / XCPR;
+    Chunk dc[DL], xc[XLD];
     f32x4 acc[4][4] = {}, accb[4] = {};
     T one[CE];
 #pragma unroll
@@ -780,11 +780,9 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
     auto stage = [&] {
         lds_barrier();
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int at = (crow + i * RSTEP) * PITCH + col * (int)sizeof(T);
-            *(Chunk *)(dm + at) = dc[i];
-            *(Chunk *)(xm + at) = xc[i];
-        }
+        for (int i = 0; i < DL; ++i) *(Chunk *)(dm + (drow + i * DSTEP) * DP + dcol * (int)sizeof(T)) = dc[i];
+#pragma unroll
+        for (int i = 0; i < XLD; ++i) *(Chunk *)(xm + (xrow + i * XSTEP) * XP + xcol * (int)sizeof(T)) = xc[i];
         lds_barrier();
     };
     auto multiply = [&] {
@@ -796,8 +794,8 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
                 Chunk df[4], xf[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    df[i] = load_columns<T>(dm, PITCH, lo, hi, wn + i * 16 + lc);
-                    xf[i] = load_columns<T>(xm, PITCH, lo, hi, wk + i * 16 + lc);
+                    df[i] = load_columns<T>(dm, DP, lo, hi, wn + i * 16 + lc);
+                    xf[i] = load_columns<T>(xm, XP, lo, hi, wk + i * 16 + lc);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -810,11 +808,11 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
                 Chunk xf[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (j < kt) xf[j] = load_columns<T>(xm, PITCH, lo, hi, wk + j * 16 + lc);
+                    if (j < kt) xf[j] = load_columns<T>(xm, XP, lo, hi, wk + j * 16 + lc);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (i < nt && (kt > 0 || want_b)) {
-                        const Chunk df = load_columns<T>(dm, PITCH, lo, hi, wn + i * 16 + lc);
+                        const Chunk df = load_columns<T>(dm, DP, lo, hi, wn + i * 16 + lc);
                         if (want_b) mma_chunk<T>(accb[i], df, ones);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
@@ -826,24 +824,22 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
     // Columns behind N or K read what follows the row; their sums are not stored.  So whole slabs need no care as long as that
     // still lies in the matrix; the others (the last ones, or all, where rows lie too far apart for 32-bit offsets) do.
     auto whole = [&](int64_t m1) {  // the slab that ends before row m1
-        return (m1 - 1) * a.dzp + n0 + kDwTile <= dr.lim + CE && (m1 - 1) * a.xp + k0 + kDwTile <= xr.lim + CE;
+        return (m1 - 1) * a.dzp + n0 + BN <= dr.lim + CE && (m1 - 1) * a.xp + k0 + BK <= xr.lim + CE;
     };
     int64_t mfull = mb + (me - mb) / ROWS * ROWS;
     if (me <= mb || max(a.dzp, a.xp) * ROWS * (int64_t)sizeof(T) > UINT32_MAX) mfull = mb;
     while (mfull > mb && !whole(mfull)) mfull -= ROWS;
     if (mfull > mb) {
-        uint32_t dof[L], xof[L];
+        uint32_t dof[DL], xof[XLD];
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            dof[i] = (uint32_t)(((crow + i * RSTEP) * a.dzp + col) * sizeof(T));
-            xof[i] = (uint32_t)(((crow + i * RSTEP) * a.xp + col) * sizeof(T));
-        }
+        for (int i = 0; i < DL; ++i) dof[i] = (uint32_t)(((drow + i * DSTEP) * a.dzp + dcol) * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < XLD; ++i) xof[i] = (uint32_t)(((xrow + i * XSTEP) * a.xp + xcol) * sizeof(T));
         auto fetch = [&](int64_t m0) {
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                dc[i] = dr.inside(m0 * a.dzp + n0, dof[i]);
-                xc[i] = xr.inside(m0 * a.xp + k0, xof[i]);
-            }
+            for (int i = 0; i < DL; ++i) dc[i] = dr.inside(m0 * a.dzp + n0, dof[i]);
+#pragma unroll
+            for (int i = 0; i < XLD; ++i) xc[i] = xr.inside(m0 * a.xp + k0, xof[i]);
         };
         fetch(mb);
         for (int64_t m0 = mb; m0 < mfull; m0 += ROWS) {
@@ -853,14 +849,15 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
         }
     }
     for (int64_t m0 = mfull; m0 < me; m0 += ROWS) {
+        auto fetch = [&](const RowReader<T> &r, Chunk &c, int64_t mi, int at, int width) {
+            const int64_t e = min(mi, a.rows - 1) * r.pitch + at;
+            c = r.raw(e);
+            r.fix(c, e, mi < me ? width - at : 0, true);
+        };
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int64_t mi = m0 + crow + i * RSTEP, m = min(mi, a.rows - 1);
-            dc[i] = dr.raw(m * a.dzp + n0 + col);
-            xc[i] = xr.raw(m * a.xp + k0 + col);
-            dr.fix(dc[i], m * a.dzp + n0 + col, mi < me ? a.N - n0 - col : 0, true);
-            xr.fix(xc[i], m * a.xp + k0 + col, mi < me ? a.K - k0 - col : 0, true);
-        }
+        for (int i = 0; i < DL; ++i) fetch(dr, dc[i], m0 + drow + i * DSTEP, n0 + dcol, a.N);
+#pragma unroll
+        for (int i = 0; i < XLD; ++i) fetch(xr, xc[i], m0 + xrow + i * XSTEP, k0 + xcol, a.K);
         stage();
         multiply();
     }
@@ -984,13 +981,31 @@ int64_t dz_sum_rows(int64_t rows, int K, size_t e) {
     return K * e <= 512 ? (int64_t)rows_blocks(rows) * 4 : (rows + 127) / 128 * 2;
 }
 
-int dw_tiles(int n) { return (n + kDwTile - 1) / kDwTile; }
+// dW's tiles: 128 x 128, or 256 along the other axis where one has 64 columns at most (320 000 rows, 64 -> 192 fp32: half of the
+// waves of a square tile would be idle).
+struct DwShape {
+    int wn, wk, tiles;  // waves along N and K; tiles of [N,K]
+    int64_t slices;
+};
 
-// Slices of the rows: as many workgroups as the card holds (two per CU), but 256 rows each at least.
-int dw_slices(int64_t rows, int K, int N) {
-    const int64_t tiles = (int64_t)dw_tiles(K) * dw_tiles(N), want = 512 / tiles, most = (rows + 255) / 256;
-    const int64_t s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s);
+DwShape dw_shape(int64_t rows, int K, int N, bool weights) {
+    DwShape p;
+    p.wk = K <= 64 ? 1 : N <= 64 ? 4 : 2, p.wn = 4 / p.wk;
+    p.tiles = (weights ? (K + 64 * p.wk - 1) / (64 * p.wk) : 1) * ((N + 64 * p.wn - 1) / (64 * p.wn));
+    // slices of the rows: as many workgroups as the card holds (two per CU), but 256 rows each at least
+    const int64_t want = 512 / p.tiles, most = (rows + 255) / 256;
+    p.slices = want < most ? want : most;
+    if (p.slices < 1) p.slices = 1;
+    return p;
+}
+
+template <typename T>
+int launch_dw(const DwArgs &d, const DwShape &p, hipStream_t s) {
+    const unsigned blocks = (unsigned)((p.slices * p.tiles + 7) / 8 * 8);
+    if (p.wk == 1) linear_dw_kernel<T, 4, 1><<<blocks, 256, 0, s>>>(d);
+    else if (p.wk == 4) linear_dw_kernel<T, 1, 4><<<blocks, 256, 0, s>>>(d);
+    else linear_dw_kernel<T, 2, 2><<<blocks, 256, 0, s>>>(d);
+    return check_launch();
 }
 
 // The one-pass backward takes a layer whose weights, and the tiles of 128 rows, fit LDS, and whose accumulators (dW, dx, db)
@@ -1069,7 +1084,7 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
         l.total = l.part_b + (db ? up((size_t)p.blocks * N * 4) : 0);
         return l;
     }
-    const size_t s = (size_t)dw_slices(rows, K, N);
+    const size_t s = (size_t)dw_shape(rows, K, N, dw).slices;
     l.dz = 0;
     l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
     l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
@@ -1132,15 +1147,14 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         if (rc != FSGS_OK) return rc;
     }
     if (!dw && !db) return FSGS_OK;
-    const int slices = dw_slices(a.rows, a.K, a.N);
+    const DwShape shape = dw_shape(a.rows, a.K, a.N, dw);
+    const int slices = (int)shape.slices;
     if (dw || !sum_rows) {
         DwArgs d = {};
         d.dz = dz, d.dzp = dzp, d.x = a.x, d.xp = a.xp, d.rows = a.rows, d.K = a.K, d.N = a.N, d.slices = slices;
         d.part_w = part_w, d.part_b = sum_rows ? nullptr : part_b;
         d.slice_rows = ((a.rows + slices - 1) / slices + 63) / 64 * 64;
-        const int64_t blocks = ((int64_t)slices * (dw ? dw_tiles(a.K) : 1) * dw_tiles(a.N) + 7) / 8 * 8;
-        linear_dw_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(d);
-        rc = check_launch();
+        rc = launch_dw<T>(d, shape, s);
         if (rc != FSGS_OK) return rc;
     }
     return launch_reduce<T>(part_w, part_b, dw, db, a.K, a.N, slices, sum_rows ? sum_rows : slices, s);
