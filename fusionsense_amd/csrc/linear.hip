@@ -292,6 +292,88 @@ __global__ __launch_bounds__(256, 3) void linear_tile_kernel(LinArgs a) {
     }
 }
 
+// ---- few rows, long summed axis: 16 rows x 32 columns per workgroup, the summed axis over its eight waves --------------------
+// A wave takes every eighth 64-byte step of x and W straight from memory (four steps under way), the waves' sums meet in LDS.
+constexpr int kFewWaves = 8;
+
+template <typename T, int MODE>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinArgs a) {
+    constexpr int CE = kChunk<T>, CPG = sizeof(T) == 2 ? 1 : 2, U = 4;
+    __shared__ f32x4 part[kFewWaves][2][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+    const int64_t m0 = (int64_t)blockIdx.y * 16, m = m0 + li;
+    const int n0 = blockIdx.x * 32;
+    const RowReader<T> xr(a.x, a.rows, a.xp, a.K), wr(a.w, a.N, a.K, a.K);
+    const int64_t xa = min(m, a.rows - 1) * a.xp;  // (rows behind the last repeat it, unstored)
+    const int64_t wa[2] = {(int64_t)min(n0 + group_column<T>(0, li), a.N - 1) * a.K,
+                           (int64_t)min(n0 + group_column<T>(1, li), a.N - 1) * a.K};
+    const int steps = (a.K + 4 * CE - 1) / (4 * CE);
+    f32x4 acc[2] = {};
+    for (int s0 = wave; s0 < steps; s0 += kFewWaves * U) {
+        Chunk xc[U], wc[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = ((s0 + u * kFewWaves) * 4 + lg) * CE;
+            xc[u] = xr.raw(xa + k);
+            wc[u][0] = wr.raw(wa[0] + k), wc[u][1] = wr.raw(wa[1] + k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + u * kFewWaves, k = (s * 4 + lg) * CE;
+            if (s >= steps) break;
+            if ((s + 1) * 4 * CE > a.K) {
+                xr.fix(xc[u], xa + k, a.K - k, true);
+                wr.fix(wc[u][0], wa[0] + k, a.K - k, true);
+                wr.fix(wc[u][1], wa[1] + k, a.K - k, true);
+            }
+            mma_chunk<T>(acc[0], wc[u][0], xc[u]);
+            mma_chunk<T>(acc[1], wc[u][1], xc[u]);
+        }
+    }
+    part[wave][0][lane] = acc[0], part[wave][1][lane] = acc[1];
+    __syncthreads();
+    if (wave != 0) return;
+    float z[8], c[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f32x4 v = part[0][i][lane];
+        for (int w = 1; w < kFewWaves; ++w) v += part[w][i][lane];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[i * 4 + q] = v[q];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int n = n0 + held_column<T>(lg, e);
+        if (a.bias && n < a.N) z[e] += (float)((const T *)a.bias)[n];
+    }
+    if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
+    else act_fwd<T>(z, a.act);
+    const T *side = (const T *)(MODE == kModeDz ? a.dy : a.res);
+    const int64_t sp = MODE == kModeDz ? a.dyp : a.rp;
+    const bool here = m < a.rows;
+#pragma unroll
+    for (int q = 0; q < CPG; ++q) {
+        const int n = n0 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+        if (side) {
+            float sv[CE];
+            unpack_chunk<T>(load_chunk_n(side + (here ? m : 0) * sp + n, a.N - n), sv);
+#pragma unroll
+            for (int e = 0; e < CE; ++e) z[q * CE + e] = MODE == kModeDz ? z[q * CE + e] * sv[e] : z[q * CE + e] + sv[e];
+        }
+        if (here && n < a.N) put_chunk((T *)a.y + m * a.yp + n, pack_chunk<T>(z + q * CE), a.N - n, false);
+    }
+    if (MODE == kModeDz && a.part_b) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = here ? z[e] : 0.f;
+        sum_rows(c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int n = n0 + held_column<T>(lg, e);
+            if (li == 0 && n < a.N) a.part_b[(int64_t)blockIdx.y * a.N + n] = c[e];
+        }
+    }
+}
+
 // ---- short summed axis: rows go straight from memory to the matrix pipe ------------------------------------------------
 // One wave takes 16 rows at a time and all columns of its workgroup's range.  W (its range) lies in LDS for the life of the
 // workgroup, a row of x is read once, 16 bytes per lane, directly in the layout of the B operand: no barrier and no staging
@@ -962,9 +1044,17 @@ int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
     return launch_rows_kc<T, MODE, 8>(a, transpose, s);
 }
 
+// Too few tiles of 128 x 128 for the card (16 rows, 1024 -> 1500 fp32: 72 us in 12 workgroups): the few-rows kernel.
+bool few_tiles(int64_t rows, int N) { return (rows + 127) / 128 * ((N + 127) / 128) <= 64; }
+
 template <typename T, int MODE>
 int launch_tile(const LinArgs &a, hipStream_t s) {
     if (rows_fit<T>(a.K)) return launch_rows<T, MODE>(a, 0, s);
+    if (few_tiles(a.rows, a.N)) {
+        const dim3 grid((a.N + 31) / 32, (unsigned)((a.rows + 15) / 16));
+        linear_few_kernel<T, MODE><<<grid, 64 * kFewWaves, 0, s>>>(a);
+        return check_launch();
+    }
     constexpr int MT = 4;
     const int bn = a.N > 64 ? 128 : 64;
     const int64_t tiles = (a.rows + 32 * MT - 1) / (32 * MT) * ((a.N + bn - 1) / bn), blocks = (tiles + 7) / 8 * 8;
@@ -977,8 +1067,8 @@ int launch_tile(const LinArgs &a, hipStream_t s) {
 }
 
 // Rows of partial column sums that launch_tile<kModeDz> leaves in part_b.
-int64_t dz_sum_rows(int64_t rows, int K, size_t e) {
-    return K * e <= 512 ? (int64_t)rows_blocks(rows) * 4 : (rows + 127) / 128 * 2;
+int64_t dz_sum_rows(int64_t rows, int K, int N, size_t e) {
+    return K * e <= 512 ? (int64_t)rows_blocks(rows) * 4 : few_tiles(rows, N) ? (rows + 15) / 16 : (rows + 127) / 128 * 2;
 }
 
 // dW's tiles: 128 x 128, or 256 along the other axis where one has 64 columns at most (320 000 rows, 64 -> 192 fp32: half of the
@@ -1089,7 +1179,7 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
     l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
     l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
     l.part_b = l.part_w + (dw ? up(s * (size_t)K * N * 4) : 0);
-    const size_t sums = act != FSGS_ACT_NONE ? max((size_t)dz_sum_rows(rows, K, e), s) : s;
+    const size_t sums = act != FSGS_ACT_NONE ? max((size_t)dz_sum_rows(rows, K, N, e), s) : s;
     l.total = l.part_b + (db ? up(sums * (size_t)N * 4) : 0);
     return l;
 }
@@ -1128,7 +1218,7 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         z.y = scratch + l.dz, z.yp = a.N, z.part_b = part_b;
         rc = launch_tile<T, kModeDz>(z, s);
         if (rc != FSGS_OK) return rc;
-        dz = z.y, dzp = a.N, sum_rows = (int)dz_sum_rows(a.rows, a.K, sizeof(T));
+        dz = z.y, dzp = a.N, sum_rows = (int)dz_sum_rows(a.rows, a.K, a.N, sizeof(T));
     }
     if (dx) {
         LinArgs g = {};
