@@ -531,9 +531,11 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
         }
     }
     if (MODE == kModeDz && a.part_b) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        float *to = a.part_b + ((int64_t)blockIdx.x * 4 + wave) * a.N + n0;
-        for (int n = lane; n < ncols; n += 64) to[n] = dbl[n];
+        __syncthreads();
+        float *to = a.part_b + (int64_t)blockIdx.x * a.N + n0;
+        const float *all = bl + ra.range;
+        for (int n = threadIdx.x; n < ncols; n += 256)
+            to[n] = (all[n] + all[ra.range + n]) + (all[2 * ra.range + n] + all[3 * ra.range + n]);
     }
 }
 
@@ -616,102 +618,107 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
         const int row = wave * 16 + li;
         const int64_t mr = min(m, a.rows - 1), nr = min(next, a.rows - 1);
         const bool end = (blk + 1) * kBwdRows + kEndRows >= a.rows;
-        if (ragged_x || end)
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-                xr.fix(xf[c], mr * a.xp + (c * 4 + lg) * CE, m < a.rows ? a.K - (c * 4 + lg) * CE : 0, end || a.xp == 0);
-        // dx^T tiles: rows k of a pair of tiles are 8 neighbours per lane in half width, 4 of one tile in fp32
-        auto add_dx = [&](f32x4 &acc, int kt, int g, const Chunk (&dz)[CPG]) {
-            const int col = CPG == 1 ? (kt >> 1) * 32 + (li & 3) * 8 + (kt & 1) * 4 : kt * 16 + li;
-#pragma unroll
-            for (int q = 0; q < CPG; ++q) {
-                const int n = column(g, q);
-                mma_chunk<T>(acc, load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col), dz[q]);
-            }
-        };
-        auto store_dx = [&](int kt, const f32x4 *acc) {
-            const int k = kt * 16 + lg * CE;
-            float v[CE];
-#pragma unroll
-            for (int e = 0; e < CE; ++e) v[e] = acc[e >> 2][e & 3];
-            if (m < a.rows && k < a.K) put_chunk((T *)a.dx + m * a.K + k, pack_chunk<T>(v), a.K - k, a.stream);
-        };
-        // whichever holds fewer registers meanwhile: dx summed group by group, or the groups' dz kept and dx done at the end
-        constexpr bool kKeepDz = KT > NG * CPG;
-        f32x4 accx[kKeepDz ? 1 : KT] = {};
-        Chunk dzc[kKeepDz ? NG : 1][CPG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (g >= ng) break;
-            float z[8], d[8];
-            if (a.act != FSGS_ACT_NONE) {
-                f32x4 acc[2] = {};
+        const int held = (int)min((int64_t)kBwdRows, a.rows - blk * kBwdRows);  // rows of this block
+        constexpr int STEP = 4 * CE;  // rows per matrix instruction of dW: 32, or 16 by four instructions
+        const bool idle = wave * 16 >= (held + STEP - 1) / STEP * STEP;  // (a whole wave without rows, in the last block)
+        if (!idle) {
+            if (ragged_x || end)
 #pragma unroll
                 for (int c = 0; c < KC; ++c)
+                    xr.fix(xf[c], mr * a.xp + (c * 4 + lg) * CE, m < a.rows ? a.K - (c * 4 + lg) * CE : 0, end || a.xp == 0);
+            // dx^T tiles: rows k of a pair of tiles are 8 neighbours per lane in half width, 4 of one tile in fp32
+            auto add_dx = [&](f32x4 &acc, int kt, int g, const Chunk (&dz)[CPG]) {
+                const int col = CPG == 1 ? (kt >> 1) * 32 + (li & 3) * 8 + (kt & 1) * 4 : kt * 16 + li;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        mma_chunk<T>(acc[i], *(const Chunk *)(mem + lay.w + (g * 32 + group_column<T>(i, li)) * lay.pk + (c * 4 + lg) * 16),
-                                     xf[c]);
+                for (int q = 0; q < CPG; ++q) {
+                    const int n = column(g, q);
+                    mma_chunk<T>(acc, load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col), dz[q]);
+                }
+            };
+            auto store_dx = [&](int kt, const f32x4 *acc) {
+                const int k = kt * 16 + lg * CE;
+                float v[CE];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    z[e] = acc[e >> 2][e & 3] + bl[g * 32 + held_column<T>(lg, e)];
+                for (int e = 0; e < CE; ++e) v[e] = acc[e >> 2][e & 3];
+                if (m < a.rows && k < a.K) put_chunk((T *)a.dx + m * a.K + k, pack_chunk<T>(v), a.K - k, a.stream);
+            };
+            // whichever holds fewer registers meanwhile: dx summed group by group, or the groups' dz kept and dx done at the end
+            constexpr bool kKeepDz = KT > NG * CPG;
+            f32x4 accx[kKeepDz ? 1 : KT] = {};
+            Chunk dzc[kKeepDz ? NG : 1][CPG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if (g >= ng) break;
+                float z[8], d[8];
+                if (a.act != FSGS_ACT_NONE) {
+                    f32x4 acc[2] = {};
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            mma_chunk<T>(acc[i], *(const Chunk *)(mem + lay.w + (g * 32 + group_column<T>(i, li)) * lay.pk + (c * 4 + lg) * 16),
+                                         xf[c]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        z[e] = acc[e >> 2][e & 3] + bl[g * 32 + held_column<T>(lg, e)];
+                }
+                if (ragged_n || end)
+#pragma unroll
+                    for (int q = 0; q < CPG; ++q)
+                        gr.fix(dyc[g][q], mr * a.dyp + column(g, q), m < a.rows ? a.N - column(g, q) : 0, end || a.dyp == 0);
+#pragma unroll
+                for (int q = 0; q < CPG; ++q) unpack_chunk<T>(dyc[g][q], d + q * CE);
+                load_dy(dyc[g], nr, g);
+                if (a.act != FSGS_ACT_NONE) {
+                    act_slope<T>(z, a.act);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) d[e] *= z[e];
+                }
+                if constexpr (kRegDb)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) db[g][e] += d[e];
+                Chunk (&dz)[CPG] = dzc[kKeepDz ? g : 0];
+#pragma unroll
+                for (int q = 0; q < CPG; ++q) {
+                    dz[q] = pack_chunk<T>(d + q * CE);
+                    *(Chunk *)(mem + lay.dz + row * lay.pn + column(g, q) * (int)sizeof(T)) = dz[q];
+                }
+                if constexpr (!kKeepDz)
+                    if (a.dx)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) add_dx(accx[kt], kt, g, dz);
             }
-            if (ragged_n || end)
+            if (a.dx) {
+                if constexpr (!kKeepDz) {
 #pragma unroll
-                for (int q = 0; q < CPG; ++q)
-                    gr.fix(dyc[g][q], mr * a.dyp + column(g, q), m < a.rows ? a.N - column(g, q) : 0, end || a.dyp == 0);
+                    for (int kt = 0; kt < KT; kt += 3 - CPG) store_dx(kt, accx + kt);
+                } else {
 #pragma unroll
-            for (int q = 0; q < CPG; ++q) unpack_chunk<T>(dyc[g][q], d + q * CE);
-            load_dy(dyc[g], nr, g);
-            if (a.act != FSGS_ACT_NONE) {
-                act_slope<T>(z, a.act);
+                    for (int kt = 0; kt < KT; kt += 3 - CPG) {
+                        f32x4 acc[3 - CPG] = {};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] *= z[e];
-            }
-            if constexpr (kRegDb)
+                        for (int g = 0; g < NG; ++g)
+                            if (g < ng)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) db[g][e] += d[e];
-            Chunk (&dz)[CPG] = dzc[kKeepDz ? g : 0];
-#pragma unroll
-            for (int q = 0; q < CPG; ++q) {
-                dz[q] = pack_chunk<T>(d + q * CE);
-                *(Chunk *)(mem + lay.dz + row * lay.pn + column(g, q) * (int)sizeof(T)) = dz[q];
-            }
-            if constexpr (!kKeepDz)
-                if (a.dx)
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) add_dx(accx[kt], kt, g, dz);
-        }
-        if (a.dx) {
-            if constexpr (!kKeepDz) {
-#pragma unroll
-                for (int kt = 0; kt < KT; kt += 3 - CPG) store_dx(kt, accx + kt);
-            } else {
-#pragma unroll
-                for (int kt = 0; kt < KT; kt += 3 - CPG) {
-                    f32x4 acc[3 - CPG] = {};
-#pragma unroll
-                    for (int g = 0; g < NG; ++g)
-                        if (g < ng)
-#pragma unroll
-                            for (int i = 0; i < 3 - CPG; ++i) add_dx(acc[i], kt + i, g, dzc[g]);
-                    store_dx(kt, acc);
+                                for (int i = 0; i < 3 - CPG; ++i) add_dx(acc[i], kt + i, g, dzc[g]);
+                        store_dx(kt, acc);
+                    }
                 }
             }
-        }
-        if (a.part_w) {
+            if (a.part_w) {
 #pragma unroll
-            for (int c = 0; c < KC; ++c) *(Chunk *)(mem + lay.x + row * lay.pk + (c * 4 + lg) * 16) = xf[c];
+                for (int c = 0; c < KC; ++c) *(Chunk *)(mem + lay.x + row * lay.pk + (c * 4 + lg) * 16) = xf[c];
+            }
         }
         m = next;
         load_x(xf, nr);
         if (tiles) {
             lds_barrier();
             // (the wave's number of tiles compiled in: no branch between the steps)
-            auto add_dw = [&](auto tiles_of_wave) {
-                constexpr int STEP = 4 * CE;  // rows per matrix instruction: 32, or 16 by four instructions
+            auto add_dw = [&](auto tiles_of_wave, auto all_rows) {
 #pragma unroll
                 for (int s = 0; s < kBwdRows / STEP; ++s) {
+                    if (!decltype(all_rows)::value && s * STEP >= held) break;
                     const int lo = s * STEP + lg * 4, hi = lo + 16;
                     Chunk xc[KTW];
 #pragma unroll
@@ -720,6 +727,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
 #pragma unroll
                     for (int i = 0; i < decltype(tiles_of_wave)::value; ++i) {
                         const int n = (i * WN + wn) * 16;
+                        if (!decltype(all_rows)::value && n >= cols) break;
                         const Chunk zc = load_columns<T>(mem + lay.dz, lay.pn, lo, hi, n + (CPG == 1 ? (li & 3) * 4 : li));
                         if constexpr (!kRegDb) {
                             float v[4];
@@ -732,10 +740,12 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                 }
             };
             const int mine = (cols / 16 - wn + WN - 1) / WN;
-            if (mine >= NTW) add_dw(std::integral_constant<int, NTW>());
-            else if (NTW > 1 && mine == NTW - 1) add_dw(std::integral_constant<int, (NTW > 1 ? NTW - 1 : 0)>());
-            else if (NTW > 2 && mine == NTW - 2) add_dw(std::integral_constant<int, (NTW > 2 ? NTW - 2 : 0)>());
-            else if (NTW > 3 && mine == NTW - 3) add_dw(std::integral_constant<int, (NTW > 3 ? NTW - 3 : 0)>());
+            const std::true_type all;
+            if (held < kBwdRows) add_dw(std::integral_constant<int, NTW>(), std::false_type());  // (the last block, with branches)
+            else if (mine >= NTW) add_dw(std::integral_constant<int, NTW>(), all);
+            else if (NTW > 1 && mine == NTW - 1) add_dw(std::integral_constant<int, (NTW > 1 ? NTW - 1 : 0)>(), all);
+            else if (NTW > 2 && mine == NTW - 2) add_dw(std::integral_constant<int, (NTW > 2 ? NTW - 2 : 0)>(), all);
+            else if (NTW > 3 && mine == NTW - 3) add_dw(std::integral_constant<int, (NTW > 3 ? NTW - 3 : 0)>(), all);
             lds_barrier();
         }
     }
@@ -823,6 +833,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w,
 struct DwArgs {
     const void *dz, *x;
     float *part_w, *part_b;  // [slices][N*K], [slices][N]; each may be null
+    void *dw, *db;           // one slice: the outputs themselves, in place of the partial sums
     int64_t rows, dzp, xp, slice_rows;
     int K, N, slices;
 };
@@ -954,43 +965,60 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int k = k0 + wk + j * 16 + li;
-                    if (k < a.K) pw[(int64_t)n * a.K + k] = acc[i][j][q];
+                    if (k >= a.K) continue;
+                    if (a.slices == 1) ((T *)a.dw)[(int64_t)n * a.K + k] = (T)acc[i][j][q];
+                    else pw[(int64_t)n * a.K + k] = acc[i][j][q];
                 }
-            if (want_b && li == 0) a.part_b[(int64_t)slice * a.N + n] = accb[i][q];
+            if (want_b && li == 0) {
+                if (a.slices == 1) ((T *)a.db)[n] = (T)accb[i][q];
+                else a.part_b[(int64_t)slice * a.N + n] = accb[i][q];
+            }
         }
 }
 
-// Sum of the slices' partial gradients: 64 neighbouring values per workgroup, 16 threads take every 16th slice of a value, in
-// an order that the sizes alone fix.  Values behind N*K are those of db.
-template <typename T>
-__global__ __launch_bounds__(1024) void reduce_slices_kernel(const float *__restrict__ part_w, const float *__restrict__ part_b,
-                                                             T *__restrict__ dw, T *__restrict__ db, int64_t nk, int N,
-                                                             int slices_w, int slices_b) {
-    __shared__ float part[16][64];
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-    const int64_t i = (int64_t)blockIdx.x * 64 + c;
-    const bool w = i < nk && dw, b = i >= nk && i < nk + N && db;
-    const float *from = w ? part_w + i : b ? part_b + (i - nk) : nullptr;
-    const int64_t pitch = w ? nk : N;
-    const int slices = w ? slices_w : slices_b;
+// Sum of partial gradients over their slices: C neighbouring values per workgroup, R threads take every R-th slice of a value
+// (eight loads under way), in an order that the sizes alone fix.  Values behind n1 are those of a second array of n2.
+template <typename T, int C, int R>
+__global__ __launch_bounds__(C * R) void reduce_slices_kernel(const float *__restrict__ p1, int64_t n1, T *__restrict__ out1,
+                                                              const float *__restrict__ p2, int64_t n2, T *__restrict__ out2,
+                                                              int slices) {
+    __shared__ float part[R][C];
+    const int c = threadIdx.x % C, r = threadIdx.x / C;
+    const int64_t i = (int64_t)blockIdx.x * C + c;
+    const bool first = i < n1, second = !first && i < n1 + n2;
+    const float *from = first ? p1 + i : p2 + (i - n1);
+    const int64_t pitch = first ? n1 : n2;
     float s = 0.f;
-    if (from)
-        for (int t = r; t < slices; t += 16) s += from[t * pitch];
+    if (first || second) {
+        int t = r;
+        for (; t + 7 * R < slices; t += 8 * R) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = from[(t + u * R) * pitch];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; t < slices; t += R) s += from[t * pitch];
+    }
     part[r][c] = s;
     __syncthreads();
-    if (r == 0 && from) {
-        for (int t = 1; t < 16; ++t) s += part[t][c];
-        if (w) dw[i] = (T)s;
-        else db[i - nk] = (T)s;
+    if (r == 0 && (first || second)) {
+        for (int t = 1; t < R; ++t) s += part[t][c];
+        if (first) out1[i] = (T)s;
+        else out2[i - n1] = (T)s;
     }
 }
 
+// One or two arrays with the same number of slices.  Few values with many slices (db of a long layer: 1024 x 256) take 64 threads
+// each: 5.9 us.  (16 threads each over 4096 slices, a row per wave of the kernel before it, took 110 us.)
 template <typename T>
-int launch_reduce(const float *part_w, const float *part_b, void *dw, void *db, int K, int N, int slices_w, int slices_b,
-                  hipStream_t s) {
-    const int64_t nk = (int64_t)N * K;
-    reduce_slices_kernel<T><<<(unsigned)((nk + N + 63) / 64), 1024, 0, s>>>(part_w, part_b, (T *)dw, (T *)db, nk, N, slices_w,
-                                                                                  slices_b);
+int launch_reduce(const float *p1, int64_t n1, void *out1, const float *p2, int64_t n2, void *out2, int slices, hipStream_t s) {
+    if (!out1) p1 = p2, n1 = n2, out1 = out2, n2 = 0;
+    if (!out2) n2 = 0;
+    const int64_t n = n1 + n2;
+    T *const o1 = (T *)out1, *const o2 = (T *)out2;
+    if (slices > 512) reduce_slices_kernel<T, 16, 64><<<(unsigned)((n + 15) / 16), 1024, 0, s>>>(p1, n1, o1, p2, n2, o2, slices);
+    else reduce_slices_kernel<T, 64, 16><<<(unsigned)((n + 63) / 64), 1024, 0, s>>>(p1, n1, o1, p2, n2, o2, slices);
     return check_launch();
 }
 
@@ -1068,7 +1096,7 @@ int launch_tile(const LinArgs &a, hipStream_t s) {
 
 // Rows of partial column sums that launch_tile<kModeDz> leaves in part_b.
 int64_t dz_sum_rows(int64_t rows, int K, int N, size_t e) {
-    return K * e <= 512 ? (int64_t)rows_blocks(rows) * 4 : few_tiles(rows, N) ? (rows + 15) / 16 : (rows + 127) / 128 * 2;
+    return K * e <= 512 ? (int64_t)rows_blocks(rows) : few_tiles(rows, N) ? (rows + 15) / 16 : (rows + 127) / 128 * 2;
 }
 
 // dW's tiles: 128 x 128, or 256 along the other axis where one has 64 columns at most (320 000 rows, 64 -> 192 fp32: half of the
@@ -1196,7 +1224,7 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         b.stream = a.rows * a.K * (int64_t)sizeof(T) >= kStreamBytes && a.K * sizeof(T) % 64 == 0 && (uintptr_t)dx % 64 == 0;
         const int rc = launch_bwd_rows_k<T>(b, p, s);
         if (rc != FSGS_OK || (!dw && !db)) return rc;
-        return launch_reduce<T>(b.part_w, b.part_b, dw, db, a.K, a.N, p.blocks, p.blocks, s);
+        return launch_reduce<T>(b.part_w, (int64_t)a.N * a.K, dw, b.part_b, a.N, db, p.blocks, s);
     }
     const void *dz = a.dy;
     int64_t dzp = a.dyp;
@@ -1242,12 +1270,19 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
     if (dw || !sum_rows) {
         DwArgs d = {};
         d.dz = dz, d.dzp = dzp, d.x = a.x, d.xp = a.xp, d.rows = a.rows, d.K = a.K, d.N = a.N, d.slices = slices;
-        d.part_w = part_w, d.part_b = sum_rows ? nullptr : part_b;
+        d.part_w = part_w, d.part_b = sum_rows ? nullptr : part_b, d.dw = dw, d.db = db;
         d.slice_rows = ((a.rows + slices - 1) / slices + 63) / 64 * 64;
         rc = launch_dw<T>(d, shape, s);
         if (rc != FSGS_OK) return rc;
     }
-    return launch_reduce<T>(part_w, part_b, dw, db, a.K, a.N, slices, sum_rows ? sum_rows : slices, s);
+    const int64_t nk = (int64_t)a.N * a.K;
+    if (sum_rows && db) {
+        rc = launch_reduce<T>(part_b, a.N, db, nullptr, 0, nullptr, sum_rows, s);
+        if (rc != FSGS_OK) return rc;
+        db = nullptr;
+    }
+    if (slices == 1 || (!dw && !db)) return FSGS_OK;
+    return launch_reduce<T>(part_w, nk, dw, part_b, a.N, db, slices, s);
 }
 
 bool bad_sizes(int64_t rows, int K, int N, int dtype, int act) {
