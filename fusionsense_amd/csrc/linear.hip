@@ -185,20 +185,45 @@ __global__ __launch_bounds__(256, 3) void linear_tile_kernel(LinArgs a) {
         for (int i = 0; i < WL; ++i) wput[i * 256] = wc[i];
         lds_barrier();
     };
-    auto multiply = [&] {
+    // (a last tile of few columns, and the last slab of the summed axis, leave out what holds nothing: N = 513 has a fifth tile of
+    // one column, K = 513 a ninth slab of one)
+    const int nt = min(NT, (a.N - n0 - wn + 31) / 32 * 2);
+    auto multiply = [&](int left) {
+        const Chunk *xg[2], *wg[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            Chunk xf[MT], wf[NT];
-            const Chunk *const xg = xs + xr0 * 8 + ((s * 4 + lg) ^ xkey(xr0));
-            const Chunk *const wg = ws + wr0 * 8 + ((s * 4 + lg) ^ wkey(wr0));
+            xg[s] = xs + xr0 * 8 + ((s * 4 + lg) ^ xkey(xr0));
+            wg[s] = ws + wr0 * 8 + ((s * 4 + lg) ^ wkey(wr0));
+        }
+        auto wat = [](int i) { return (i >> 1) * 256 + (i & 1) * (sizeof(T) == 2 ? 32 : 128); };
+        if (nt == NT && left > BK / 2) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) wf[i] = wg[(i >> 1) * 256 + (i & 1) * (sizeof(T) == 2 ? 32 : 128)];
+            for (int s = 0; s < 2; ++s) {
+                Chunk xf[MT], wf[NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xf[i] = xg[i * 128];
+                for (int i = 0; i < NT; ++i) wf[i] = wg[s][wat(i)];
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+                for (int i = 0; i < MT; ++i) xf[i] = xg[s][i * 128];
 #pragma unroll
-                for (int j = 0; j < MT; ++j) mma_chunk<T>(acc[i][j], wf[i], xf[j]);
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) mma_chunk<T>(acc[i][j], wf[i], xf[j]);
+            }
+        } else if (nt > 0) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s * (BK / 2) >= left) break;
+                Chunk xf[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) xf[i] = xg[s][i * 128];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    if (i >= nt) break;
+                    const Chunk wf = wg[s][wat(i)];
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) mma_chunk<T>(acc[i][j], wf, xf[j]);
+                }
+            }
         }
     };
     // whole slabs, byte offsets inside the tile in 32 bits; then what is left of the summed axis (or all of it, where rows lie
@@ -220,7 +245,7 @@ __global__ __launch_bounds__(256, 3) void linear_tile_kernel(LinArgs a) {
         for (int k0 = 0; k0 < kfull; k0 += BK) {
             stage();
             fetch(min(k0 + BK, kfull - BK));
-            multiply();
+            multiply(BK);
         }
     }
     for (int k0 = kfull; k0 < a.K; k0 += BK) {
@@ -238,7 +263,7 @@ __global__ __launch_bounds__(256, 3) void linear_tile_kernel(LinArgs a) {
             wr.fix(wc[i], at, a.K - k0 - ck, end);
         }
         stage();
-        multiply();
+        multiply(a.K - k0);
     }
 
     const T *bias = (const T *)a.bias;
@@ -1060,25 +1085,32 @@ int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
     return check_launch();
 }
 
-template <typename T>
-bool rows_fit(int K) { return (size_t)K * sizeof(T) <= 512; }
+// Which kernel a product takes.  A wave of the rows kernel reads all of W from LDS for its 16 rows, a tile's waves a 16th of that,
+// but x goes through LDS too there (300 001 rows, none | gelu with a residual; rows / tile in us):
+//   bf16 128 -> 128  32/36 | 45/53      bf16 256 -> 128  70/45 | 81/62      fp32 128 -> 128  109/115 | 134/152
+//   bf16 128 -> 1024 210/208 | 387/498  bf16 256 -> 1024 452/255 | 612/563  fp32 64 -> 256   107/142 | 156/216
+bool rows_fit(int K, size_t e) { return K * e <= (e == 2 ? 256 : 512); }
 
 template <typename T, int MODE>
 int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
     const int bytes = a.K * (int)sizeof(T);
     if (bytes <= 64) return launch_rows_kc<T, MODE, 1>(a, transpose, s);
     if (bytes <= 128) return launch_rows_kc<T, MODE, 2>(a, transpose, s);
-    if (bytes <= 256) return launch_rows_kc<T, MODE, 4>(a, transpose, s);
-    return launch_rows_kc<T, MODE, 8>(a, transpose, s);
+    if constexpr (sizeof(T) == 4)
+        if (bytes > 256) return launch_rows_kc<T, MODE, 8>(a, transpose, s);
+    return launch_rows_kc<T, MODE, 4>(a, transpose, s);
 }
 
-// Too few tiles of 128 x 128 for the card (16 rows, 1024 -> 1500 fp32: 72 us in 12 workgroups): the few-rows kernel.
-bool few_tiles(int64_t rows, int N) { return (rows + 127) / 128 * ((N + 127) / 128) <= 64; }
+// Too few tiles of 128 x 128 for the card: the few-rows kernel, which splits the summed axis (few rows / tile in us):
+//   bf16 1024 -> 1500: 16 rows (12 tiles) 5.3/14.7, 256 (24) 12.8/16.0, 512 (48) 24/16;  bf16 256 -> 256: 512 rows (8) 5.4/7.2,
+//   1024 (16) 8.7/7.2, 2500 (40) 19/7.4;  fp32 1024 -> 1500: 16 rows 8.3/74, 512 (48) 44/77;  fp32 256 -> 256: 2500 (40) 20/24,
+//   4096 (64) 31/24
+bool few_tiles(int64_t rows, int N, size_t e) { return (rows + 127) / 128 * ((N + 127) / 128) <= (e == 2 ? 16 : 48); }
 
 template <typename T, int MODE>
 int launch_tile(const LinArgs &a, hipStream_t s) {
-    if (rows_fit<T>(a.K)) return launch_rows<T, MODE>(a, 0, s);
-    if (few_tiles(a.rows, a.N)) {
+    if (rows_fit(a.K, sizeof(T))) return launch_rows<T, MODE>(a, 0, s);
+    if (few_tiles(a.rows, a.N, sizeof(T))) {
         const dim3 grid((a.N + 31) / 32, (unsigned)((a.rows + 15) / 16));
         linear_few_kernel<T, MODE><<<grid, 64 * kFewWaves, 0, s>>>(a);
         return check_launch();
@@ -1096,7 +1128,7 @@ int launch_tile(const LinArgs &a, hipStream_t s) {
 
 // Rows of partial column sums that launch_tile<kModeDz> leaves in part_b.
 int64_t dz_sum_rows(int64_t rows, int K, int N, size_t e) {
-    return K * e <= 512 ? (int64_t)rows_blocks(rows) : few_tiles(rows, N) ? (rows + 15) / 16 : (rows + 127) / 128 * 2;
+    return rows_fit(K, e) ? (int64_t)rows_blocks(rows) : few_tiles(rows, N, e) ? (rows + 15) / 16 : (rows + 127) / 128 * 2;
 }
 
 // dW's tiles: 128 x 128, or 256 along the other axis where one has 64 columns at most (320 000 rows, 64 -> 192 fp32: half of the
@@ -1251,7 +1283,7 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
     if (dx) {
         LinArgs g = {};
         g.x = dz, g.xp = dzp, g.y = dx, g.yp = a.K, g.rows = a.rows, g.K = a.N, g.N = a.K;
-        if (rows_fit<T>(a.N)) {
+        if (rows_fit(a.N, sizeof(T))) {
             g.w = a.w;
             rc = launch_rows<T, kModeFwd>(g, 1, s);
         } else {
