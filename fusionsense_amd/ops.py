@@ -1998,7 +1998,9 @@ def topk_distill(logits: Tensor, teacher_idx: Tensor, teacher_logits: Tensor, te
     if teacher_logits.shape != teacher_idx.shape:
         raise ValueError(f"teacher_logits must be {tuple(teacher_idx.shape)} like teacher_idx, got {tuple(teacher_logits.shape)}")
     for name, t in (("teacher_idx", teacher_idx), ("teacher_logits", teacher_logits), ("weight", weight)):
-        if t is not None and isinstance(t, torch.Tensor) and t.device != logits.device:
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t is not None and t.device != logits.device:
             raise ValueError(f"{name} must be on {logits.device} like logits, got {t.device}")
     if teacher_logits.requires_grad or (weight is not None and weight.requires_grad):
         raise ValueError("the teacher's scores and the weights are constants: detach them")

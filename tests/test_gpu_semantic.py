@@ -202,6 +202,79 @@ def test_linear_offsets_beyond_32_bits(dev, dtype):
         assert torch.equal(blk, first.repeat((n + 4095) // 4096, 1)[:n]), m0
 
 
+# Sizes at which the product, its dz, dx and dW take other kernels or tiles than above: many tiles of 128 and of 64 columns, a last
+# tile of two columns, a last slab of a few entries, few rows of a long sum, more than 256 outputs of a short one, dW tiles of
+# either shape, several slices and a single one.
+WIDE = [(3000, 300, 70), (7000, 200, 50), (2200, 600, 130), (1290, 161, 513), (130, 48, 300), (1500, 200, 64), (16, 1100, 33),
+        (1100, 8, 400), (40, 2000, 1100), (129, 64, 257), (3000, 96, 900)]
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("size", WIDE, ids=lambda s: "x".join(map(str, s)))
+def test_linear_wide_sizes(dev, size, dtype, act):
+    i = WIDE.index(size)
+    x, w, b, r, dy = _layer(dev, *size, dtype, bias=i % 3 != 1, res=act == "silu", seed=30 + i)
+    _check_layer(x, w, b, r, act, dy, f"{size} {act}")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("size", [(300, 600, 130), (2500, 300, 140), (200, 40, 300)], ids=lambda s: "x".join(map(str, s)))
+def test_linear_wide_layouts(dev, size, dtype):
+    """One row for all, slices with an odd start and pitch, gradients with a pitch, of wide layers: what the plain copies give."""
+    M, K, N = size
+    x, w, b, r, dy = _layer(dev, M, K, N, dtype, seed=60)
+    y0, g0 = _check_layer(x, w, b, None, "relu", dy)
+    wide = torch.full((M, K + 3), float("nan"), dtype=dtype, device=dev)
+    wide[:, 1:K + 1] = x
+    gw = torch.full((M, N + 5), float("nan"), dtype=dtype, device=dev)
+    gw[:, 3:N + 3] = dy
+    y, g = _check_layer(wide[:, 1:K + 1], w, b, None, "relu", gw[:, 3:N + 3], "slices")
+    assert torch.equal(y, y0) and all(torch.equal(g[k], g0[k]) for k in g0)
+    one = x[:1].expand(M, K)
+    y, _ = _check_layer(one, w, b, r[:1].expand(M, N), "gelu", dy[:1].expand(M, N), "one row for all")
+    assert torch.equal(y, y[:1].expand(M, N))
+
+
+def test_linear_rows_too_far_apart_for_32_bit_offsets(dev):
+    """Tiles whose 128 rows span more than 4 GiB: the same bits as with the rows side by side."""
+    M, K, N, pitch, dtype = 130, 600, 1100, 17_000_000, torch.bfloat16
+    assert pitch * 2 * 128 > 2 ** 32
+    x0, w, b, _, dy0 = _layer(dev, M, K, N, dtype, seed=61)
+    big = torch.zeros(M * pitch, dtype=dtype, device=dev)
+    x = big.as_strided((M, K), (pitch, 1))
+    x.copy_(x0)
+    dy = big.as_strided((M, N), (pitch, 1), 10_000)
+    dy.copy_(dy0)
+    y0, g0 = _check_layer(x0, w, b, None, "none", dy0)
+    y, g = _check_layer(x, w, b, None, "none", dy, "far rows")
+    assert torch.equal(y, y0) and all(torch.equal(g[k], g0[k]) for k in g0)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_writes_its_outputs_only(dev, dtype):
+    """Outputs at unaligned places between guard values, through the C entries: nothing around them changes."""
+    from fusionsense_amd._lib import load, ptr, stream_ptr
+    for M, K, N in ((70, 40, 24), (300, 300, 130), (3, 7, 5), (130, 48, 300)):
+        x, w, b, _, dy = _layer(dev, M, K, N, dtype, seed=62)
+        want, g0 = _check_layer(x, w, b, None, "gelu", dy)
+        lib, dt, act = load(), ops.DTYPES[dtype], ops.ACTIVATIONS["gelu"]
+        n = lib.fsgs_linear_bwd_scratch_bytes(M, K, N, dt, act, 1, 1, 1)
+        scratch = torch.full((n + 256,), 0x5A, dtype=torch.uint8, device=dev)
+        room = [torch.full((t.numel() + 9,), 3.0, dtype=dtype, device=dev) for t in (want, x, w, b)]
+        outs = [t[3:-6] for t in room]
+        at = [t.data_ptr() for t in outs]
+        assert lib.fsgs_linear_fwd(M, K, N, dt, ptr(x), K, ptr(w), ptr(b), act, None, 0, at[0], stream_ptr(dev)) == 0
+        assert lib.fsgs_linear_bwd(M, K, N, dt, ptr(x), K, ptr(w), ptr(b), act, None, ptr(dy), N, at[1], at[2], at[3], ptr(scratch),
+                                   n, stream_ptr(dev)) == 0
+        for t, o, v in zip(room, outs, (want, g0["x"], g0["w"], g0["b"])):
+            assert torch.equal(o.reshape(v.shape), v)
+            assert (t[:3] == 3).all() and (t[-6:] == 3).all()
+        assert (scratch[n:] == 0x5A).all()
+        assert lib.fsgs_linear_bwd(M, K, N, dt, ptr(x), K, ptr(w), ptr(b), act, None, ptr(dy), N, at[1], at[2], at[3], ptr(scratch),
+                                   n - 1, stream_ptr(dev)) < 0  # (a workspace one byte short is refused)
+
+
 # ---- distillation -------------------------------------------------------------------------------------------------
 def _record(dev, R, V, K, dtype, tdtype=torch.float32, idx_dtype=torch.int64, seed=0, ragged=True):
     g = torch.Generator().manual_seed(seed)
@@ -249,6 +322,51 @@ def test_distill_sizes(dev, size, dtype):
     weight = torch.rand(size[0], generator=torch.Generator().manual_seed(i)).to(dev) if i % 2 else None
     for reduction in ops.REDUCTIONS:
         _check_distill(logits, idx, top, (1.0, 2.0, 0.5)[i % 3], weight, reduction, what=f"{size} {reduction}")
+
+
+# Rows at the boundaries between lanes per row, steps per lane and a workgroup per row: L lanes hold 3 or 5 chunks of 4 or 8 classes.
+EDGES = sorted({v + d for v in (12, 20, 24, 40, 48, 80, 96, 160, 320, 640, 768, 1280, 1536, 2560) for d in (-1, 0, 1)})
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_distill_sizes_at_the_boundaries(dev, dtype):
+    for V in EDGES:
+        logits, idx, top = _record(dev, 37, V, min(V, 11), dtype, seed=V)
+        _check_distill(logits, idx, top, 2.0, None, "mean", what=str(V))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [7, 21, 150, 1203, 9001])
+def test_distill_writes_its_outputs_only(dev, dtype, V):
+    """A gradient at an unaligned place between guard values, through the C entries: nothing around it changes."""
+    from fusionsense_amd._lib import load, ptr, stream_ptr
+    R, K = 45, 6
+    logits, idx, top = _record(dev, R, V, K, dtype, seed=70)
+    leaf = logits.clone().requires_grad_(True)
+    loss = losses.topk_distill_loss(leaf, idx, top, 2.0, None, "none")
+    up = _randn(dev, R, seed=71)
+    want, = torch.autograd.grad(loss, [leaf], up)
+    lib, dt = load(), ops.DTYPES[dtype]
+    common = (64, ptr(idx), K, ops.DTYPES[torch.float32], ptr(top), K, None, 2.0)
+    for off in (1, 3, 8):
+        rows, stat = torch.full((R + 2,), 3.0, device=dev), torch.full((4 * R + 4,), 3.0, device=dev)
+        room = torch.full((R * V + 16,), 3.0, dtype=dtype, device=dev)
+        out = room[off:off + R * V]
+        assert lib.fsgs_distill_fwd(R, V, K, dt, ptr(logits), V, *common, 0, rows[1:].data_ptr(), ptr(stat), None, None, 0,
+                                    stream_ptr(dev)) == 0
+        assert lib.fsgs_distill_bwd(R, V, K, dt, ptr(logits), V, *common, ptr(stat), None, ptr(up), 1, out.data_ptr(),
+                                    stream_ptr(dev)) == 0
+        assert torch.equal(rows[1:-1], loss) and torch.equal(out.reshape(R, V), want)
+        assert rows[0] == 3 and rows[-1] == 3 and (stat[4 * R:] == 3).all()
+        assert (room[:off] == 3).all() and (room[off + R * V:] == 3).all()
+        # the scores as a slice of a wider plane: the rest of it has no gradient
+        wide = torch.full((R, V + 3), float("nan"), dtype=dtype, device=dev)
+        wide[:, 2:V + 2] = logits
+        wide.requires_grad_(True)
+        l = losses.topk_distill_loss(wide[:, 2:V + 2], idx, top, 2.0, None, "none")
+        g, = torch.autograd.grad(l, [wide], up)
+        assert torch.equal(l, loss) and torch.equal(g[:, 2:V + 2], want)
+        assert not g[:, :2].any() and not g[:, V + 2:].any()
 
 
 @pytest.mark.parametrize("tdtype", TYPES, ids=IDS)
