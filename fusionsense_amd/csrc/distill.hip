@@ -558,8 +558,8 @@ int launch(const DistillArgs &a, int dtype, bool bwd, hipStream_t st) {
 }
 
 bool bad_args(int64_t rows, int V, int K, int dtype, int tdtype, int idx_bits, float T) {
-    return rows < 0 || rows > INT32_MAX || V < 1 || V > FSGS_DISTILL_MAX_CLASSES || K < 1 || K > FSGS_DISTILL_MAX_K || !known_dtype(dtype) || !known_dtype(tdtype) ||
-           (idx_bits != 32 && idx_bits != 64) || !(T >= FSGS_DISTILL_MIN_T) || !(T <= FSGS_DISTILL_MAX_T);
+    return rows < 0 || rows > INT32_MAX || V < 1 || V > FSGS_DISTILL_MAX_CLASSES || K < 1 || K > FSGS_DISTILL_MAX_K ||
+           !known_dtype(dtype) || !known_dtype(tdtype) || (idx_bits != 32 && idx_bits != 64) || !(T >= FSGS_DISTILL_MIN_T) || !(T <= FSGS_DISTILL_MAX_T);
 }
 
 }  // namespace
@@ -593,8 +593,8 @@ extern "C" int fsgs_distill_fwd(int64_t rows, int classes, int top_k, int dtype,
         if (rc != FSGS_OK) return rc;
     }
     if (reduction == FSGS_REDUCE_NONE) return FSGS_OK;
-    distill_reduce_kernel<<<1, 256, 0, st>>>((const double2 *)scratch, rows > 0 ? row_blocks(rows, lanes_per_row(classes, dtype)) : 0, reduction == FSGS_REDUCE_MEAN,
-                                             loss, inv_weight);
+    const int blocks = rows > 0 ? row_blocks(rows, lanes_per_row(classes, dtype)) : 0;
+    distill_reduce_kernel<<<1, 256, 0, st>>>((const double2 *)scratch, blocks, reduction == FSGS_REDUCE_MEAN, loss, inv_weight);
     return check_launch();
 }
 

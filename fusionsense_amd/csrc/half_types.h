@@ -38,8 +38,8 @@ __device__ __forceinline__ Chunk load_chunk_n(const T *p, int n) {
 }
 
 // Rows of a matrix read in chunks that need not end with the row: raw() reads 16 bytes wherever they start (held back only at
-// the matrix' last element, so nothing outside it is read; a matrix of less than 16 bytes is read from its start) and has no branch, so it can be under way long before it is used;
-// fix() then moves what was held back to its place and zeroes what lies behind `valid` elements.
+// the matrix' last element, so nothing outside it is read; a matrix of less than 16 bytes is read from its start) and has no
+// branch, so it can be under way long before it is used; fix() then moves what was held back to its place and zeroes what lies behind `valid` elements.
 template <typename T>
 struct RowReader {
     const T *p;

@@ -61,7 +61,8 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
         for (int i = 0; i < N; ++i) {
             float e;
             const float p = normal_tail<T>(z[i], e);
-            z[i] = fmaf(-fabsf(z[i]), p * e, fmaxf(z[i], 0.f));  // z >= 0: z - z h; z < 0: -|z| h
+            // z >= 0: z - z h; z < 0: -|z| h  (+inf, where h is zero, stays; -inf and NaN give NaN, as z Phi(z) does)
+            z[i] = fmaf(-fabsf(fminf(z[i], 1e30f)), p * e, fmaxf(z[i], 0.f));
         }
     } else if (act == FSGS_ACT_SILU) {
 #pragma unroll
@@ -565,8 +566,8 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
 }
 
 // ---- backward of a layer whose two axes are both short: one pass over x and dy -----------------------------------------
-// A workgroup of eight waves takes 128 rows at a time, a wave 16 of them.  Per 32 columns: z from W (LDS) and the wave's rows of x, dz =
-// dy act'(z) in fp32 registers (db is summed from these), rounded once to T and used twice: as it stands it is the B operand
+// A workgroup of eight waves takes 128 rows at a time, a wave 16 of them.  Per 32 columns: z from W (LDS) and the wave's rows of
+// x, dz = dy act'(z) in fp32 registers (db is summed from these), rounded once to T and used twice: as it stands it is the B operand
 // of dx^T = W^T dz^T, and through LDS it meets x again in dW = dz^T x, whose whole [N,K] lies in the workgroup's registers for
 // the life of the workgroup.  x and dy are read once, dx is written once; W is held once, read along its rows for z and along
 // its columns for dx.
@@ -766,7 +767,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
             };
             const int mine = (cols / 16 - wn + WN - 1) / WN;
             const std::true_type all;
-            if (held < kBwdRows) add_dw(std::integral_constant<int, NTW>(), std::false_type());  // (the last block, with branches)
+            if (held < kBwdRows) add_dw(std::integral_constant<int, NTW>(), std::false_type());  // (the last block: branches)
             else if (mine >= NTW) add_dw(std::integral_constant<int, NTW>(), all);
             else if (NTW > 1 && mine == NTW - 1) add_dw(std::integral_constant<int, (NTW > 1 ? NTW - 1 : 0)>(), all);
             else if (NTW > 2 && mine == NTW - 2) add_dw(std::integral_constant<int, (NTW > 2 ? NTW - 2 : 0)>(), all);
@@ -811,8 +812,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
         }
         __syncthreads();
         const float *all = (const float *)(mem + lay.dz);
-        for (int n = threadIdx.x; n < a.N; n += 64 * kBwdWaves)
-{
+        for (int n = threadIdx.x; n < a.N; n += 64 * kBwdWaves) {
             float v = 0.f;
             for (int w = 0; w < kBwdWaves; ++w) v += all[w * cols + n];
             a.part_b[(int64_t)blockIdx.x * a.N + n] = v;
@@ -1318,8 +1318,8 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
 }
 
 bool bad_sizes(int64_t rows, int K, int N, int dtype, int act) {
-    return rows < 0 || rows > INT32_MAX || K < 1 || N < 1 || K > FSGS_LINEAR_MAX_DIM || N > FSGS_LINEAR_MAX_DIM || !known_dtype(dtype) ||
-           act < FSGS_ACT_NONE || act > FSGS_ACT_SILU;
+    return rows < 0 || rows > INT32_MAX || K < 1 || N < 1 || K > FSGS_LINEAR_MAX_DIM || N > FSGS_LINEAR_MAX_DIM ||
+           !known_dtype(dtype) || act < FSGS_ACT_NONE || act > FSGS_ACT_SILU;
 }
 
 }  // namespace

@@ -149,6 +149,43 @@ def test_linear_keeps_bad_values_in_their_rows(dev, dtype):
     assert torch.equal(y2[130], torch.where(w[:, 60] > 0, torch.full_like(r[130], float("inf")), r[130]))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("K", [64, 700])
+def test_linear_infinite_pre_activations(dev, dtype, act, K):
+    """What z Phi(z) and z sigma(z) give: +inf stays, -inf and NaN become NaN, the largest finite sums stay or vanish."""
+    x = torch.zeros(3000, K, dtype=dtype, device=dev)
+    big = torch.finfo(dtype).max
+    values = [float("inf"), -float("inf"), float("nan"), big, -big]
+    x[40:45, 1] = torch.tensor(values, dtype=dtype, device=dev)
+    w = torch.zeros(70, K, dtype=dtype, device=dev)
+    w[:, 1] = 1
+    y = ops.linear_act(x, w, None, act)
+    want = [float("inf"), float("nan"), float("nan"), big, 0.0]
+    for m, v in enumerate(want):
+        assert torch.equal(y[40 + m].isnan(), torch.full_like(y[0], v).isnan())
+        assert v != v or (y[40 + m].abs() == abs(v)).all()
+    assert not y[:40].any() and not y[45:].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("K", [24, 64, 200, 700])
+@pytest.mark.parametrize("pitch", [1, 3, 8])
+def test_linear_overlapping_rows(dev, dtype, K, pitch):
+    """Sliding windows over one vector (rows closer together than they are long), forward and backward."""
+    M, N = 300, 70
+    v = _randn(dev, (M - 1) * pitch + K, seed=80, dtype=dtype)
+    x = v.as_strided((M, K), (pitch, 1))
+    x0, w, b, r, dy = _layer(dev, M, K, N, dtype, seed=81)
+    y0, g0 = _check_layer(x.clone(), w, b, r, "gelu", dy)
+    g = _randn(dev, (M - 1) * pitch + N, seed=82, dtype=dtype).as_strided((M, N), (pitch, 1))
+    leaves = [t.detach().requires_grad_(True) for t in (w, b)]
+    out = ops.linear_act(x, leaves[0], leaves[1], "gelu", r)
+    got = torch.autograd.grad(out, leaves, dy)
+    assert torch.equal(out, y0) and torch.equal(got[0], g0["w"]) and torch.equal(got[1], g0["b"])
+    _check_layer(x.clone(), w, b, r, "silu", g, "windows of gradients")
+
+
 def test_linear_gradients_against_differences(dev):
     """fp32, central differences of sum(dy * y) along random directions.  y carries (K + 2) U32 of its terms (S.linear's bound);
     with a step h the quotient is off by that over h plus h^2 / 6 times the third derivative along the direction (act''' <= 2
