@@ -1053,82 +1053,123 @@ constexpr int64_t kStreamBytes = 32 << 20;  // outputs from here on are stored p
 
 unsigned rows_blocks(int64_t rows) { return (unsigned)((rows + 63) / 64 < 1024 ? (rows + 63) / 64 : 1024); }
 
-template <typename T, int MODE, int KC>
-int launch_rows_kc(const LinArgs &a, int transpose, hipStream_t s) {
-    RowsArgs r;
-    r.l = a;
-    r.transpose = transpose;
-    const int row_bytes = rows_pitch<T, KC>() * 16 + 4;
+// How the rows kernel would take a product.
+struct RowsPlan {
+    int kc, range, store;
+    size_t bytes;
+};
+
+template <typename T, int MODE>
+RowsPlan rows_plan(const LinArgs &a) {
+    const int row = a.K * (int)sizeof(T);
+    RowsPlan p;
+    p.kc = row <= 64 ? 1 : row <= 128 ? 2 : row <= 256 ? 4 : 8;
+    const int row_bytes = (p.kc * 4 + 1) * 16 + 4;  // (rows_pitch, and a bias)
     const int fit = kRowsLds / row_bytes / 32 * 32, need = (a.N + 31) / 32 * 32;
-    r.range = need < fit ? need : fit;
+    p.range = need < fit ? need : fit;
     // few rows: more, narrower ranges, whose weights are fetched side by side (one row, 64 -> 150 fp32: 7.0 -> 4.9 us)
-    while (r.range > 32 && (int64_t)rows_blocks(a.rows) * ((a.N + r.range - 1) / r.range) < 256)
-        r.range = (r.range / 2 + 31) / 32 * 32;
-    const int ranges = (a.N + r.range - 1) / r.range;
+    while (p.range > 32 && (int64_t)rows_blocks(a.rows) * ((a.N + p.range - 1) / p.range) < 256)
+        p.range = (p.range / 2 + 31) / 32 * 32;
     const bool sums = MODE == kModeDz && a.part_b;
-    const size_t bytes = (size_t)r.range * (row_bytes + (sums ? 16 : 0));
-    const dim3 grid(rows_blocks(a.rows), ranges);
+    p.bytes = (size_t)p.range * (row_bytes + (sums ? 16 : 0));
+    p.store = kStorePlain;
     if (a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes) {
-        if (a.N * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0) {
-            linear_rows_kernel<T, MODE, KC, kStoreStream><<<grid, 256, bytes, s>>>(r);
-            return check_launch();
-        }
-        const size_t tiled = bytes + 4 * (size_t)tile_bytes<T>(a.N);
-        if (!sums && ranges == 1 && a.yp == a.N && tiled <= 2 * kRowsLds) {
-            const int rc = ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, kStoreTile>>(tiled);
-            if (rc != FSGS_OK) return rc;
-            linear_rows_kernel<T, MODE, KC, kStoreTile><<<grid, 256, tiled, s>>>(r);
-            return check_launch();
-        }
+        const size_t tiled = p.bytes + 4 * (size_t)tile_bytes<T>(a.N);
+        if (a.N * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0) p.store = kStoreStream;
+        else if (!sums && p.range >= a.N && a.yp == a.N && tiled <= 2 * kRowsLds) p.store = kStoreTile, p.bytes = tiled;
     }
-    linear_rows_kernel<T, MODE, KC, kStorePlain><<<grid, 256, bytes, s>>>(r);
-    return check_launch();
+    return p;
 }
 
-// Which kernel a product takes.  A wave of the rows kernel reads all of W from LDS for its 16 rows, a tile's waves a 16th of that,
-// but x goes through LDS too there (300 001 rows, none | gelu with a residual; rows / tile in us):
-//   bf16 128 -> 128  32/36 | 45/53      bf16 256 -> 128  70/45 | 81/62      fp32 128 -> 128  109/115 | 134/152
-//   bf16 128 -> 1024 210/208 | 387/498  bf16 256 -> 1024 452/255 | 612/563  fp32 64 -> 256   107/142 | 156/216
-bool rows_fit(int K, size_t e) { return K * e <= (e == 2 ? 256 : 512); }
+template <typename T, int MODE, int KC>
+int launch_rows_kc(const RowsArgs &r, const RowsPlan &p, hipStream_t s) {
+    const dim3 grid(rows_blocks(r.l.rows), (r.l.N + p.range - 1) / p.range);
+    if (p.store == kStoreTile) {
+        const int rc = ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, kStoreTile>>(p.bytes);
+        if (rc != FSGS_OK) return rc;
+        linear_rows_kernel<T, MODE, KC, kStoreTile><<<grid, 256, p.bytes, s>>>(r);
+    } else if (p.store == kStoreStream) {
+        linear_rows_kernel<T, MODE, KC, kStoreStream><<<grid, 256, p.bytes, s>>>(r);
+    } else {
+        linear_rows_kernel<T, MODE, KC, kStorePlain><<<grid, 256, p.bytes, s>>>(r);
+    }
+    return check_launch();
+}
 
 template <typename T, int MODE>
 int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
-    const int bytes = a.K * (int)sizeof(T);
-    if (bytes <= 64) return launch_rows_kc<T, MODE, 1>(a, transpose, s);
-    if (bytes <= 128) return launch_rows_kc<T, MODE, 2>(a, transpose, s);
-    if constexpr (sizeof(T) == 4)
-        if (bytes > 256) return launch_rows_kc<T, MODE, 8>(a, transpose, s);
-    return launch_rows_kc<T, MODE, 4>(a, transpose, s);
+    const RowsPlan p = rows_plan<T, MODE>(a);
+    RowsArgs r;
+    r.l = a, r.range = p.range, r.transpose = transpose;
+    switch (p.kc) {
+        case 1: return launch_rows_kc<T, MODE, 1>(r, p, s);
+        case 2: return launch_rows_kc<T, MODE, 2>(r, p, s);
+        case 4: return launch_rows_kc<T, MODE, 4>(r, p, s);
+        default:
+            if constexpr (sizeof(T) == 4) return launch_rows_kc<T, MODE, 8>(r, p, s);
+            return FSGS_EINVAL;  // (product_kind sends no such product here)
+    }
 }
 
-// Too few tiles of 128 x 128 for the card: the few-rows kernel, which splits the summed axis (few rows / tile in us):
-//   bf16 1024 -> 1500: 16 rows (12 tiles) 5.3/14.7, 256 (24) 12.8/16.0, 512 (48) 24/16;  bf16 256 -> 256: 512 rows (8) 5.4/7.2,
-//   1024 (16) 8.7/7.2, 2500 (40) 19/7.4;  fp32 1024 -> 1500: 16 rows 8.3/74, 512 (48) 44/77;  fp32 256 -> 256: 2500 (40) 20/24,
-//   4096 (64) 31/24
-bool few_tiles(int64_t rows, int N, size_t e) { return (rows + 127) / 128 * ((N + 127) / 128) <= (e == 2 ? 16 : 48); }
+// Which kernel a product takes (times in us; "small" is a tile of 64 x 64, "tile" of 128 x 128).
+//
+// Rows: a wave reads all of W from LDS for its 16 rows, a tile's waves an 8th or a 16th of that, but there x goes through LDS
+// too.  It pays for short rows as long as its stores leave in whole lines, or are few (rows / small / tile):
+//   640 000 rows  bf16 64 -> 128 48/60/54 | gelu 68/80/74     bf16 32 -> 150 48/92/95     fp32 32 -> 128 105/114/120 (gelu)
+//   ... where they cannot  bf16 128 -> 150 227/161/142    fp32 64 -> 150 296/231/264
+//   120 000 rows, outputs below kStreamBytes  bf16 64 -> 128 28/16/19    fp32 32 -> 64 21/17/17    bf16 64 -> 21 9/10/10
+//   16 384 rows  fp32 32 -> 64 5.6/4.4/5.7    bf16 32 -> 64 4.3/4.4/5.3   4096 rows  bf16 32 -> 64 3.4/4.3/5.1
+//   300 001 rows, longer  bf16 256 -> 1024 452/-/255    fp32 128 -> 128 109/-/115
+// Few: the summed axis over a workgroup's waves, for long sums with few tiles (few / small / tile):
+//   bf16 1024 -> 256  512 rows 5.5/7.6/16, 1024 9.1/7.6/16     bf16 512 -> 256  512 rows 5.4/5.2/10
+//   fp32 512 -> 256  1024 rows (16 tiles) 9.9/13.9/41, 2500 (40) 23/14/42
+// Small: until there are tiles enough for the card (small / tile):
+//   bf16 192 -> 256  20 000 rows (314 tiles) 7.7/9.2, 40 000 (626) 13.7/13.7, 80 000 (1250) 23/19; 4096 -> 512  8000 rows 64/54
+//   fp32 192 -> 256  40 000 rows (626) 46/48, 160 000 (2500) 162/152; 1024 -> 256  40 000 rows 205/211, 80 000 (1250) 400/346
+enum { kByRows, kByFew, kBySmall, kByTiles };
+constexpr int64_t kFewBytes = 4 << 20;
 
 template <typename T, int MODE>
-int launch_tile(const LinArgs &a, hipStream_t s) {
-    if (rows_fit(a.K, sizeof(T))) return launch_rows<T, MODE>(a, 0, s);
-    if (few_tiles(a.rows, a.N, sizeof(T))) {
-        const dim3 grid((a.N + 31) / 32, (unsigned)((a.rows + 15) / 16));
-        linear_few_kernel<T, MODE><<<grid, 64 * kFewWaves, 0, s>>>(a);
-        return check_launch();
+int product_kind(const LinArgs &a) {
+    constexpr bool half = sizeof(T) == 2;
+    const int64_t out = a.rows * a.N * (int64_t)sizeof(T), tiles = (a.rows + 127) / 128 * ((a.N + 127) / 128);
+    if (a.K * sizeof(T) <= (half ? 256 : 512) && (a.N <= 32 || out < kFewBytes || rows_plan<T, MODE>(a).store != kStorePlain))
+        return kByRows;
+    if (half ? a.K > 512 && tiles <= 8 : tiles <= 16) return kByFew;
+    if (half ? a.K <= 2048 && tiles <= 512 : tiles <= 1024) return kBySmall;
+    return kByTiles;
+}
+
+// Rows of partial column sums that a dz kernel leaves in part_b.
+int64_t sum_rows_of(int kind, int64_t rows) {
+    switch (kind) {
+        case kByRows: return rows_blocks(rows);
+        case kByFew: return (rows + 15) / 16;
+        case kBySmall: return (rows + 63) / 64 * 2;
+        default: return (rows + 127) / 128 * 2;
     }
-    constexpr int MT = 4;
-    const int bn = a.N > 64 ? 128 : 64;
-    const int64_t tiles = (a.rows + 32 * MT - 1) / (32 * MT) * ((a.N + bn - 1) / bn), blocks = (tiles + 7) / 8 * 8;
+}
+
+template <typename T, int MODE, int BN, int MT>
+int launch_tiles(const LinArgs &a, hipStream_t s) {
+    const int64_t tiles = (a.rows + 32 * MT - 1) / (32 * MT) * ((a.N + BN - 1) / BN), blocks = (tiles + 7) / 8 * 8;
     if (blocks > (int64_t)UINT32_MAX / 256) return FSGS_EINVAL;  // (a grid holds at most 2^32 threads)
     LinArgs b = a;
     b.stream = a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes && a.yp * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0;
-    if (bn == 128) linear_tile_kernel<T, MODE, 128, MT><<<(unsigned)blocks, 256, 0, s>>>(b);
-    else linear_tile_kernel<T, MODE, 64, MT><<<(unsigned)blocks, 256, 0, s>>>(b);
+    linear_tile_kernel<T, MODE, BN, MT><<<(unsigned)blocks, 256, 0, s>>>(b);
     return check_launch();
 }
 
-// Rows of partial column sums that launch_tile<kModeDz> leaves in part_b.
-int64_t dz_sum_rows(int64_t rows, int K, int N, size_t e) {
-    return rows_fit(K, e) ? (int64_t)rows_blocks(rows) : few_tiles(rows, N, e) ? (rows + 15) / 16 : (rows + 127) / 128 * 2;
+template <typename T, int MODE>
+int launch_product(const LinArgs &a, int kind, hipStream_t s) {
+    switch (kind) {
+        case kByRows: return launch_rows<T, MODE>(a, 0, s);
+        case kByFew:
+            linear_few_kernel<T, MODE><<<dim3((a.N + 31) / 32, (unsigned)((a.rows + 15) / 16)), 64 * kFewWaves, 0, s>>>(a);
+            return check_launch();
+        case kBySmall: return launch_tiles<T, MODE, 64, 2>(a, s);
+        default: return a.N > 64 ? launch_tiles<T, MODE, 128, 4>(a, s) : launch_tiles<T, MODE, 64, 4>(a, s);
+    }
 }
 
 // dW's tiles: 128 x 128, or 256 along the other axis where one has 64 columns at most (320 000 rows, 64 -> 192 fp32: half of the
@@ -1239,7 +1280,9 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
     l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
     l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
     l.part_b = l.part_w + (dw ? up(s * (size_t)K * N * 4) : 0);
-    const size_t sums = act != FSGS_ACT_NONE ? max((size_t)dz_sum_rows(rows, K, N, e), s) : s;
+    // (which kernel forms dz depends on where the workspace lies: room for any)
+    const int64_t dz_sums = max(sum_rows_of(kByRows, rows), sum_rows_of(rows <= 16 * 128 ? kByFew : kBySmall, rows));
+    const size_t sums = act != FSGS_ACT_NONE ? max((size_t)dz_sums, s) : s;
     l.total = l.part_b + (db ? up(sums * (size_t)N * 4) : 0);
     return l;
 }
@@ -1276,14 +1319,16 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         // (the sums of db are taken here, before dz is rounded to T)
         LinArgs z = a;
         z.y = scratch + l.dz, z.yp = a.N, z.part_b = part_b;
-        rc = launch_tile<T, kModeDz>(z, s);
+        const int kind = product_kind<T, kModeDz>(z);
+        rc = launch_product<T, kModeDz>(z, kind, s);
         if (rc != FSGS_OK) return rc;
-        dz = z.y, dzp = a.N, sum_rows = (int)dz_sum_rows(a.rows, a.K, a.N, sizeof(T));
+        dz = z.y, dzp = a.N, sum_rows = (int)sum_rows_of(kind, a.rows);
     }
     if (dx) {
         LinArgs g = {};
         g.x = dz, g.xp = dzp, g.y = dx, g.yp = a.K, g.rows = a.rows, g.K = a.N, g.N = a.K;
-        if (rows_fit(a.N, sizeof(T))) {
+        const int kind = product_kind<T, kModeFwd>(g);
+        if (kind == kByRows) {
             g.w = a.w;
             rc = launch_rows<T, kModeFwd>(g, 1, s);
         } else {
@@ -1292,7 +1337,7 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
             rc = check_launch();
             if (rc != FSGS_OK) return rc;
             g.w = wt;
-            rc = launch_tile<T, kModeFwd>(g, s);
+            rc = launch_product<T, kModeFwd>(g, kind, s);
         }
         if (rc != FSGS_OK) return rc;
     }
@@ -1337,9 +1382,9 @@ extern "C" int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype,
     a.x = x, a.xp = x_pitch, a.w = w, a.bias = bias, a.res = residual, a.rp = res_pitch, a.y = y, a.yp = out_dim;
     a.rows = rows, a.K = in_dim, a.N = out_dim, a.act = act;
     switch (dtype) {
-        case FSGS_F32: return launch_tile<float, kModeFwd>(a, as_stream(stream));
-        case FSGS_BF16: return launch_tile<__bf16, kModeFwd>(a, as_stream(stream));
-        default: return launch_tile<_Float16, kModeFwd>(a, as_stream(stream));
+        case FSGS_F32: return launch_product<float, kModeFwd>(a, product_kind<float, kModeFwd>(a), as_stream(stream));
+        case FSGS_BF16: return launch_product<__bf16, kModeFwd>(a, product_kind<__bf16, kModeFwd>(a), as_stream(stream));
+        default: return launch_product<_Float16, kModeFwd>(a, product_kind<_Float16, kModeFwd>(a), as_stream(stream));
     }
 }
 
