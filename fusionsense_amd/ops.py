@@ -1815,6 +1815,8 @@ def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
     one pitch (a slice of a wider plane, an expanded row) is read in place, any other is copied once."""
     if t.dim() != 2:
         t = t.reshape(-1, width) if t.numel() > 0 else t.new_empty(0, width)
+    if t.is_contiguous():
+        return t, width
     if width > 1 and t.stride(1) != 1:
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else width)
@@ -1823,8 +1825,9 @@ def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
 def _rows16(t: Tensor, width: int) -> Tuple[Tensor, int]:
     """_rows for the layer kernels, which read 16 bytes at a time: a matrix of less is copied to where that many are readable."""
     t, pitch = _rows(t, width)
-    span = (t.shape[0] - 1) * pitch + width
-    if span * t.element_size() < 16:
+    rows = t.shape[0]
+    if rows * pitch < 16 and ((rows - 1) * pitch + width) * t.element_size() < 16:
+        span = (rows - 1) * pitch + width
         t = torch.cat([t.as_strided((span,), (1,)), t.new_zeros(16 // t.element_size())])
     return t, pitch
 
@@ -1842,6 +1845,23 @@ def _linear_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Opt
     return y
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_scratch_bytes(*sizes) -> int:
+    """The backward's workspace for these sizes (a call through ctypes costs 2 us, which a small layer's backward would see)."""
+    n = load().fsgs_linear_bwd_scratch_bytes(*sizes)
+    if n < 0:
+        check(n, "fsgs_linear_bwd_scratch_bytes")
+    return n
+
+
+def _once(backward, ctx, g):
+    """A backward that cannot be differentiated again.  Where no graph of it is asked for, the usual case, it needs no guard (3 us
+    of the 110 that a small layer's training call costs the host)."""
+    if torch.is_grad_enabled():
+        return torch.autograd.function.once_differentiable(backward)(ctx, g)
+    return backward(ctx, g)
+
+
 class _LinearAct(torch.autograd.Function):
     """act(x W^T + b) + residual; the backward forms the pre-activation again instead of keeping it."""
 
@@ -1857,27 +1877,30 @@ class _LinearAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        return _once(_LinearAct._backward, ctx, dy)
+
+    @staticmethod
+    def _backward(ctx, dy):
         x, weight, bias, y = ctx.saved_tensors
         lib = load()
         dev = x.device
         N, K = weight.shape
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         need_b = need_b and bias is not None
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         rows = x.numel() // K
-        new = torch.empty if rows > 0 else torch.zeros
-        dw = new(N, K, dtype=x.dtype, device=dev) if need_w else None
-        db = new(N, dtype=x.dtype, device=dev) if need_b else None
+        dx = x.new_empty(x.shape) if need_x else None
+        new = torch.empty_like if rows > 0 else torch.zeros_like
+        dw = new(weight) if need_w else None
+        db = new(bias) if need_b else None
         if rows > 0 and (need_x or need_w or need_b):
             x2, xp = _rows16(x, K)
             g2, gp = _rows16(dy, N)
             dt = DTYPES[x.dtype]
-            nbytes = lib.fsgs_linear_bwd_scratch_bytes(rows, K, N, dt, ctx.act, need_x, need_w, need_b)
-            scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+            nbytes = _linear_scratch_bytes(rows, K, N, dt, ctx.act, need_x, need_w, need_b)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             _run_on(dev, lib.fsgs_linear_bwd, (rows, K, N, dt, x2.data_ptr(), xp, ptr(weight), ptr(bias), ctx.act, ptr(y),
-                                               g2.data_ptr(), gp, ptr(dx), ptr(dw), ptr(db), scratch.data_ptr(), nbytes,
+                                               g2.data_ptr(), gp, ptr(dx), ptr(dw), ptr(db), ptr(scratch), nbytes,
                                                stream_ptr(dev)), "fsgs_linear_bwd")
         return dx, dw, db, (dy if need_r else None), None
 
@@ -1961,13 +1984,16 @@ class _TopkDistill(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        return _once(_TopkDistill._backward, ctx, g)
+
+    @staticmethod
+    def _backward(ctx, g):
         logits, idx, teacher, weight, buf = ctx.saved_tensors
         temperature, per_row = ctx.cfg
         dev = logits.device
         (rows, K), V = idx.shape, logits.shape[-1]
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        grad = logits.new_empty(logits.shape)
         if rows > 0:
             s2, sp = _rows(logits, V)
             i2, ip = _rows(idx, K)
