@@ -440,8 +440,12 @@ __device__ __forceinline__ void fill_weights(Chunk *wl, const T *w, int n0, int 
     }
 }
 
+// Waves of a workgroup: with output tiles six, two workgroups a CU (640 000 rows, 32 -> 150 fp32: 127 us; four waves, also two: 133).
+constexpr int rows_waves(int store) { return store == kStoreTile ? 6 : 4; }
+
 template <typename T, int MODE, int KC, int STORE>
-__global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
+__global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(RowsArgs ra) {
+    constexpr int WAVES = rows_waves(STORE);
     constexpr int CE = kChunk<T>, P = rows_pitch<T, KC>();
     extern __shared__ Chunk lds[];
     const LinArgs &a = ra.l;
@@ -450,7 +454,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     float *bl = (float *)(lds + ra.range * P);
     const int n0 = blockIdx.y * ra.range, ncols = min(ra.range, a.N - n0);
     fill_weights<T, KC>(wl, (const T *)a.w, n0, ra.range, a.N, a.K, ra.transpose);
-    for (int n = threadIdx.x; n < ra.range; n += 256)
+    for (int n = threadIdx.x; n < ra.range; n += 64 * WAVES)
         bl[n] = a.bias && n < ncols ? (float)((const T *)a.bias)[n0 + n] : 0.f;
     __syncthreads();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
@@ -463,7 +467,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
     const bool has_side = MODE == kModeDz || a.res;
     const RowReader<T> sr(MODE == kModeDz ? a.dy : a.res, a.rows, MODE == kModeDz ? a.dyp : a.rp, a.N);
     const bool ragged_x = a.K != KC * 4 * CE, ragged_n = ncols % 32 != 0;
-    const int64_t tiles = (a.rows + 15) / 16, step = (int64_t)gridDim.x * 4;
+    const int64_t tiles = (a.rows + 15) / 16, step = (int64_t)gridDim.x * WAVES;
     auto column = [&](int g, int q) { return g * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4); };
     auto load_x = [&](Chunk (&f)[KC], int64_t row) {
 #pragma unroll
@@ -473,7 +477,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
 #pragma unroll
         for (int q = 0; q < CPG; ++q) f[q] = sr.raw(row * sr.pitch + n0 + column(g, q));
     };
-    int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    int64_t t = (int64_t)blockIdx.x * WAVES + wave;
     // the next tile's rows, and of the side input the next group, are under way while this one is worked on
     Chunk xn[KC], sn[CPG];
     if (t < tiles) {
@@ -531,13 +535,17 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dbl[g * 32 + held_column<T>(lg, e)] += c[e];
             }
+            const bool whole = (g + 1) * 32 <= ncols;
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
                 const int n = column(g, q);
                 const Chunk o = pack_chunk<T>(z + q * CE);
-                if (m < a.rows && n < ncols) {
-                    if constexpr (STORE == kStoreTile) put_chunk((T *)mine + off + li * a.N + n, o, ncols - n, false);
-                    else put_chunk(y + m * a.yp + n0 + n, o, ncols - n, STORE == kStoreStream);
+                if constexpr (STORE == kStoreTile) {  // (rows behind the last stay in the wave's LDS)
+                    T *at = (T *)mine + off + li * a.N + n;
+                    if (whole) __builtin_memcpy(at, &o, sizeof(Chunk));
+                    else if (n < ncols) put_chunk(at, o, ncols - n, false);
+                } else if (m < a.rows && n < ncols) {
+                    put_chunk(y + m * a.yp + n0 + n, o, ncols - n, STORE == kStoreStream);
                 }
             }
         }
@@ -560,7 +568,7 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(RowsArgs ra) {
         __syncthreads();
         float *to = a.part_b + (int64_t)blockIdx.x * a.N + n0;
         const float *all = bl + ra.range;
-        for (int n = threadIdx.x; n < ncols; n += 256)
+        for (int n = threadIdx.x; n < ncols; n += 64 * WAVES)
             to[n] = (all[n] + all[ra.range + n]) + (all[2 * ra.range + n] + all[3 * ra.range + n]);
     }
 }
@@ -1074,7 +1082,7 @@ RowsPlan rows_plan(const LinArgs &a) {
     p.bytes = (size_t)p.range * (row_bytes + (sums ? 16 : 0));
     p.store = kStorePlain;
     if (a.rows * a.N * (int64_t)sizeof(T) >= kStreamBytes) {
-        const size_t tiled = p.bytes + 4 * (size_t)tile_bytes<T>(a.N);
+        const size_t tiled = p.bytes + rows_waves(kStoreTile) * (size_t)tile_bytes<T>(a.N);
         if (a.N * sizeof(T) % 64 == 0 && (uintptr_t)a.y % 64 == 0) p.store = kStoreStream;
         else if (!sums && p.range >= a.N && a.yp == a.N && tiled <= 2 * kRowsLds) p.store = kStoreTile, p.bytes = tiled;
     }
@@ -1087,7 +1095,8 @@ int launch_rows_kc(const RowsArgs &r, const RowsPlan &p, hipStream_t s) {
     if (p.store == kStoreTile) {
         const int rc = ensure_dynamic_lds<linear_rows_kernel<T, MODE, KC, kStoreTile>>(p.bytes);
         if (rc != FSGS_OK) return rc;
-        linear_rows_kernel<T, MODE, KC, kStoreTile><<<grid, 256, p.bytes, s>>>(r);
+        constexpr unsigned rows_tile_blocks = 512;  // (what the card holds at once; such an output is long enough for all)
+        linear_rows_kernel<T, MODE, KC, kStoreTile><<<rows_tile_blocks, 64 * rows_waves(kStoreTile), p.bytes, s>>>(r);
     } else if (p.store == kStoreStream) {
         linear_rows_kernel<T, MODE, KC, kStoreStream><<<grid, 256, p.bytes, s>>>(r);
     } else {
