@@ -50,6 +50,24 @@ __device__ __forceinline__ float normal_tail(float z, float &e) {
     return p * t;
 }
 
+// The tail at |z| for the half-width types' forward as one exponential: 2^Q(|z|), Q a polynomial of degree 9 fitted here to
+// log2 of the tail on [0, 13.2] and falling on from there.  The relative error stays below 5e-6 at |z| < 1, 3e-5 < 2, 1e-4
+// everywhere, so that |z| h is off by 1.4e-6 at most: under a hundredth of an fp16 step at 1, a fifth of its half step far out.
+// (640 000 rows, 64 -> 128 bf16: 61.5 us; by the form above, with its reciprocal, 64.8.)
+__device__ __forceinline__ float normal_tail_half(float z) {
+    const float a = fabsf(z);
+    float q = fmaf(-1.56790725e-09f, a, 1.2192244e-07f);
+    q = fmaf(q, a, -4.12213922e-06f);
+    q = fmaf(q, a, 8.01530987e-05f);
+    q = fmaf(q, a, -0.00100325886f);
+    q = fmaf(q, a, 0.00863550697f);
+    q = fmaf(q, a, -0.0540182889f);
+    q = fmaf(q, a, -0.458512872f);
+    q = fmaf(q, a, -1.15121996f);
+    q = fmaf(q, a, -0.999997079f);
+    return __builtin_amdgcn_exp2f(q);
+}
+
 // z -> act(z) for N values (one uniform branch for all of them).
 template <typename T, int N>
 __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
@@ -59,10 +77,16 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
     } else if (act == FSGS_ACT_GELU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            float e;
-            const float p = normal_tail<T>(z[i], e);
+            float h;
+            if constexpr (sizeof(T) == 2) {
+                h = normal_tail_half(z[i]);
+            } else {
+                float e;
+                h = normal_tail<T>(z[i], e);
+                h *= e;
+            }
             // z >= 0: z - z h; z < 0: -|z| h  (+inf, where h is zero, stays; -inf and NaN give NaN, as z Phi(z) does)
-            z[i] = fmaf(-fabsf(fminf(z[i], 1e30f)), p * e, fmaxf(z[i], 0.f));
+            z[i] = fmaf(-fabsf(fminf(z[i], 1e30f)), h, fmaxf(z[i], 0.f));
         }
     } else if (act == FSGS_ACT_SILU) {
 #pragma unroll
