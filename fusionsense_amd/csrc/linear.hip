@@ -156,18 +156,22 @@ __device__ __forceinline__ int group_column(int t, int r) {
     return sizeof(T) == 2 ? (r >> 2) * 8 + t * 4 + (r & 3) : t * 16 + r;
 }
 
-// The first n (at least one) elements of a chunk.
+// The first n (at least one) elements of a chunk.  The two branches end apart (two empty instructions that differ): their stores
+// are the same instructions at other places, and the compiler, left to join them, has given lanes of the one the values of the
+// other.
 template <typename T>
 __device__ __forceinline__ void put_chunk(T *to, const Chunk &c, int n, bool stream) {
     if (n >= kChunk<T>) {
         if (stream) store_streaming(to, c);
         else __builtin_memcpy(to, &c, sizeof(Chunk));
+        asm volatile("; whole chunk" ::: "memory");
     } else {
         T t[kChunk<T>];
         __builtin_memcpy(t, &c, sizeof(Chunk));
 #pragma unroll
         for (int e = 0; e < kChunk<T>; ++e)
             if (e < n) to[e] = t[e];
+        asm volatile("; part of a chunk" ::: "memory");
     }
 }
 
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinArgs a) {
 //   kStoreStream  past the caches; rows must start at 64-byte boundaries, which a store instruction then covers whole
 //   kStoreTile    the wave's 16 rows (neighbours in y) are put together in LDS and leave it as aligned streaming stores
 // Bound by memory where the activation is cheap (921 600 rows, 64 -> 64 fp32, silu and a residual: 139 us, 708 MB at 5.1 TB/s;
-// a 4 GiB copy reaches 4.8), by gelu's vector instructions at 640 000 rows, 64 -> 128 bf16 (61.5 us, 48 without it), and with
+// a 4 GiB copy reaches 4.8), by gelu's vector instructions at 640 000 rows, 64 -> 128 bf16 (59 us, 48 without it), and with
 // fp32 class scores (640 000 rows, 32 -> 150: 127 us, 466 MB at 3.7 TB/s) by what overlaps between twelve waves a CU.
 enum { kStorePlain = 0, kStoreStream = 1, kStoreTile = 2 };
 
@@ -567,17 +571,13 @@ __global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(Row
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dbl[g * 32 + held_column<T>(lg, e)] += c[e];
             }
-            const bool whole = (g + 1) * 32 <= ncols;
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
                 const int n = column(g, q);
                 const Chunk o = pack_chunk<T>(z + q * CE);
-                if constexpr (STORE == kStoreTile) {  // (rows behind the last stay in the wave's LDS)
-                    T *at = (T *)mine + off + li * a.N + n;
-                    if (whole) __builtin_memcpy(at, &o, sizeof(Chunk));
-                    else if (n < ncols) put_chunk(at, o, ncols - n, false);
-                } else if (m < a.rows && n < ncols) {
-                    put_chunk(y + m * a.yp + n0 + n, o, ncols - n, STORE == kStoreStream);
+                if (m < a.rows && n < ncols) {
+                    if constexpr (STORE == kStoreTile) put_chunk((T *)mine + off + li * a.N + n, o, ncols - n, false);
+                    else put_chunk(y + m * a.yp + n0 + n, o, ncols - n, STORE == kStoreStream);
                 }
             }
         }

@@ -273,6 +273,32 @@ def test_linear_wide_layouts(dev, size, dtype):
     assert torch.equal(y, y[:1].expand(M, N))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("K,N", [(32, 150), (16, 21), (24, 35), (40, 43), (32, 64), (20, 9), (64, 147), (128, 150), (300, 129)])
+def test_linear_large_outputs(dev, dtype, K, N):
+    """Outputs beyond 32 MiB, which leave past the caches (in whole lines, through LDS, or plainly, by their rows' length): the
+    first 1000 rows against 64 bits, the others, which repeat them, bit for bit; dx likewise."""
+    M = (33 << 20) // (N * dtype.itemsize) + 5
+    base, w, b, r, _ = _layer(dev, 1000, K, N, dtype, seed=90)
+    x = base.repeat(M // 1000 + 1, 1)[:M]
+    for act, res in (("none", False), ("gelu", True)):
+        rr = r.repeat(M // 1000 + 1, 1)[:M] if res else None
+        v, e = S.linear(base, w, b, r if res else None, act)["y"]
+        y = ops.linear_act(x, w, b, act, rr)
+        S.check(y[:1000], (v, e), f"first rows {act}")
+        for m0 in range(0, M, 1000):
+            blk = y[m0:m0 + 1000]
+            assert torch.equal(blk, y[:blk.shape[0]]), (act, m0)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    dy = torch.ones(1, 1, dtype=dtype, device=dev).expand(M, N)
+    dx, _, _ = torch.autograd.grad(ops.linear_act(*leaves, "silu"), leaves, dy)
+    want = S.linear(base, w, b, None, "silu", torch.ones(1000, N))
+    S.check(dx[:1000], want["dx"], "dx")
+    for m0 in range(0, M, 1000):
+        blk = dx[m0:m0 + 1000]
+        assert torch.equal(blk, dx[:blk.shape[0]]), ("dx", m0)
+
+
 def test_linear_rows_too_far_apart_for_32_bit_offsets(dev):
     """Tiles whose 128 rows span more than 4 GiB: the same bits as with the rows side by side."""
     M, K, N, pitch, dtype = 130, 600, 1100, 17_000_000, torch.bfloat16
