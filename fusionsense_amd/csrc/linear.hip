@@ -864,6 +864,108 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
     }
 }
 
+// ---- backward of a few rows and outputs, half width: one launch, dz never rounded -----------------------------------------
+// In the kernels above and below dz is rounded to T for its two products, up to half a step of each value: over many values that
+// adds two fifths to the error of the gradients' own rounding, but over few it may double it.  Here every workgroup forms all of
+// dz (rows x N) by itself in fp32 LDS and takes 32 columns of dW and dx.  Bound by latency: 16 rows, 64 -> 20 bf16 6.4 us; one row,
+// 64 -> 150 10.8, where four rows take 15 in the one-pass kernel and its sum over slices; one row, 512 -> 512 43.
+constexpr int kSmallDz = 512, kSmallCols = 32, kSmallWaves = 8;
+constexpr int64_t kSmallWeights = 1 << 18;  // every workgroup reads all of W: up to half a megabyte
+
+bool small_bwd(int64_t rows, int K, int N, size_t e) {
+    return e == 2 && rows * N <= kSmallDz && (int64_t)K * N <= kSmallWeights;
+}
+
+struct SmallArgs {
+    const void *x, *w, *bias, *dy;
+    void *dx, *dw, *db;
+    int64_t xp, dyp;
+    int rows, K, N, act;
+};
+
+template <typename T>
+__global__ __launch_bounds__(64 * kSmallWaves) void linear_bwd_small_kernel(SmallArgs a) {
+    constexpr int CE = kChunk<T>, U = 4, THREADS = 64 * kSmallWaves;
+    __shared__ float dz[kSmallDz], part[THREADS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+    const T *x = (const T *)a.x, *w = (const T *)a.w, *bias = (const T *)a.bias, *dy = (const T *)a.dy;
+    const RowReader<T> xr(a.x, a.rows, a.xp, a.K), wr(a.w, a.N, a.K, a.K);
+    const bool tiny = a.N * a.K < CE;  // (of x the caller has 16 bytes to read, not of W)
+    const int nts = (a.N + 15) / 16, tiles = (a.rows + 15) / 16 * nts, steps = (a.K + 4 * CE - 1) / (4 * CE);
+    for (int t = wave; t < tiles; t += kSmallWaves) {  // a wave: 16 rows x 16 columns of z
+        const int m = t / nts * 16 + li, n0 = t % nts * 16;
+        float z[4] = {};
+        if (a.act != FSGS_ACT_NONE) {
+            const int64_t xa = min(m, a.rows - 1) * a.xp, wa = (int64_t)min(n0 + li, a.N - 1) * a.K;
+            f32x4 acc = {};
+            for (int s0 = 0; s0 < steps; s0 += U) {
+                Chunk xc[U], wc[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = ((s0 + u) * 4 + lg) * CE;
+                    xc[u] = xr.raw(xa + k);
+                    if (tiny) wc[u] = load_chunk_n(w + wa + k, a.K - k);
+                    else wc[u] = wr.raw(wa + k);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = ((s0 + u) * 4 + lg) * CE;
+                    xr.fix(xc[u], xa + k, a.K - k, true);
+                    if (!tiny) wr.fix(wc[u], wa + k, a.K - k, true);
+                    mma_chunk<T>(acc, wc[u], xc[u]);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[q] = acc[q] + (bias && n0 + lg * 4 + q < a.N ? (float)bias[n0 + lg * 4 + q] : 0.f);
+        }
+        act_slope<T>(z, a.act);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = n0 + lg * 4 + q;
+            if (m < a.rows && n < a.N) dz[m * a.N + n] = z[q] * (float)dy[m * a.dyp + n];
+        }
+    }
+    __syncthreads();
+    const int k0 = blockIdx.x * kSmallCols, cols = min(kSmallCols, a.K - k0);
+    // out[o][k] = sum over j < len of dz value (o, j) times other's (j, k); where there are threads to spare each takes every S-th j
+    auto product = [&](T *out, int outer, int len, int dzo, int dzj, const T *other, int64_t pitch) {
+        const int items = outer * kSmallCols;
+        int split = 1;
+        while (split < len && items * split * 2 <= THREADS) split *= 2;
+        auto sum = [&](int i, int j0, int step) {
+            const int o = i / kSmallCols, k = i % kSmallCols;
+            float v = 0.f;
+            if (k < cols)
+#pragma unroll 8
+                for (int j = j0; j < len; j += step) v = fmaf(dz[o * dzo + j * dzj], (float)other[j * pitch + k0 + k], v);
+            return v;
+        };
+        auto put = [&](int i, float v) {
+            const int o = i / kSmallCols, k = i % kSmallCols;
+            if (k < cols) out[(int64_t)o * a.K + k0 + k] = (T)v;
+        };
+        if (split == 1) {
+            for (int i = tid; i < items; i += THREADS) put(i, sum(i, 0, 1));
+            return;
+        }
+        if (tid < items * split) part[tid] = sum(tid % items, tid / items, split);
+        __syncthreads();
+        if (tid < items) {
+            float v = part[tid];
+            for (int p = 1; p < split; ++p) v += part[tid + p * items];
+            put(tid, v);
+        }
+        __syncthreads();
+    };
+    if (a.dw) product((T *)a.dw, a.N, a.rows, 1, a.N, x, a.xp);
+    if (a.dx) product((T *)a.dx, a.rows, a.N, a.N, 1, w, a.K);
+    if (a.db && blockIdx.x == 0 && tid < a.N) {
+        float v = 0.f;
+        for (int m = 0; m < a.rows; ++m) v += dz[m * a.N + tid];
+        ((T *)a.db)[tid] = (T)v;
+    }
+}
+
 // dz of a relu layer from its output: dy where y > 0 (exact, no product; what the layer's rounding took to zero has no slope).
 // Rows of `width` elements; y and dz without gaps.  Bound by memory: 100 003 x 768 fp16 82 us, 461 MB at 5.6 TB/s.
 template <typename T>
@@ -1337,6 +1439,15 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
 
 template <typename T>
 int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratch, const BwdScratch &l, hipStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (small_bwd(a.rows, a.K, a.N, sizeof(T))) {  // (needs no workspace)
+            SmallArgs b = {};
+            b.x = a.x, b.xp = a.xp, b.w = a.w, b.bias = a.bias, b.dy = a.dy, b.dyp = a.dyp, b.dx = dx, b.dw = dw, b.db = db;
+            b.rows = (int)a.rows, b.K = a.K, b.N = a.N, b.act = a.act;
+            const int blocks = dx || dw ? (a.K + kSmallCols - 1) / kSmallCols : 1;
+            linear_bwd_small_kernel<T><<<blocks, 64 * kSmallWaves, 0, s>>>(b);
+            return check_launch();
+        }
     const BwdRowsPlan p = bwd_rows_plan<T>(a.rows, a.K, a.N);
     if (p.kc) {
         BwdRowsArgs b = {};
@@ -1438,7 +1549,8 @@ extern "C" int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype,
 
 extern "C" int fsgs_linear_bwd_uses_output(int64_t rows, int in_dim, int out_dim, int dtype, int act) {
     if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
-    return act == FSGS_ACT_RELU && bwd_rows_plan(rows, in_dim, out_dim, dtype == FSGS_F32 ? 4 : 2).kc == 0;
+    const size_t e = dtype == FSGS_F32 ? 4 : 2;
+    return act == FSGS_ACT_RELU && bwd_rows_plan(rows, in_dim, out_dim, e).kc == 0 && !small_bwd(rows, in_dim, out_dim, e);
 }
 
 extern "C" int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int act, int want_dx,

@@ -255,6 +255,30 @@ def test_linear_wide_sizes(dev, size, dtype, act):
     _check_layer(x, w, b, r, act, dy, f"{size} {act}")
 
 
+FEW = [(1, 1, 1), (1, 3, 2), (2, 1, 3), (1, 40, 500), (16, 64, 20), (17, 33, 30), (512, 24, 1), (3, 1000, 170), (1, 1024, 512), (100, 7, 5),
+       (8, 65, 64), (9, 64, 64)]
+
+
+@pytest.mark.parametrize("act", list(ops.ACTIVATIONS))
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("size", FEW, ids=lambda s: "x".join(map(str, s)))
+def test_linear_few_values(dev, size, dtype, act):
+    """Few rows and outputs.  Half width, up to 512 values of dz and 2^18 weights: no rounding of dz, so dx, dW and db are off by
+    half a step of their own and the fp32 sums only (the bound of a layer whose dz is exact in fp32)."""
+    i = FEW.index(size)
+    x, w, b, r, dy = _layer(dev, *size, dtype, bias=i % 2 == 0, res=i % 3 == 0, seed=100 + i)
+    _, g = _check_layer(x, w, b, r, act, dy, f"{size} {act}")
+    M, K, N = size
+    if dtype == torch.float32 or M * N > 512 or K * N > 1 << 18:
+        return
+    f = lambda t: t.float() if t is not None else None  # noqa: E731
+    want = S.linear(f(x), f(w), f(b), None, act, f(dy))  # (bounds without the rounding of dz, and with fp32's of the result)
+    for k, n in (("x", "dx"), ("w", "dw"), ("b", "db")):
+        if k in g:
+            v, e = want[n]
+            S.check(g[k], (v, e + S.U[dtype] * (v.abs() + e) + S.TINY[dtype]), f"{size} {act} {n} without a rounding of dz")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("size", [(300, 600, 130), (2500, 300, 140), (200, 40, 300)], ids=lambda s: "x".join(map(str, s)))
 def test_linear_wide_layouts(dev, size, dtype):
