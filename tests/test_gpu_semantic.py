@@ -279,6 +279,29 @@ def test_linear_few_values(dev, size, dtype, act):
             S.check(g[k], (v, e + S.U[dtype] * (v.abs() + e) + S.TINY[dtype]), f"{size} {act} {n} without a rounding of dz")
 
 
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("size", [(5000, 8, 2), (700, 32, 32), (3000, 100, 10), (1000, 250, 4), (2000, 4, 200), (10, 20, 150), (300, 3, 129),
+                                  (128, 8, 200), (129, 12, 60)], ids=lambda s: "x".join(map(str, s)))
+def test_linear_few_gradient_values(dev, size, dtype, act):
+    """Thin layers (128 inputs at most) with a thousand values of dW, or of dx, or fewer: their products take dz as two values of
+    the type, so they are off by half a step of their own, half a step of half a step of dz, and the fp32 sums.  (250 inputs are
+    no thin layer: the bound of every layer.)"""
+    x, w, b, r, dy = _layer(dev, *size, dtype, res=False, seed=120 + size[0])
+    _, g = _check_layer(x, w, b, r, act, dy, f"{size} {act}")
+    if size[1] > 128:
+        return
+    want = S.linear(x.float(), w.float(), b.float(), None, act, dy.float())
+    u = S.U[dtype]
+    dz = (dy.double() * S.slope(x.double() @ w.double().t() + b.double(), act)).abs().cpu()
+    left = {"dx": dz @ w.cpu().double().abs(), "dw": dz.t() @ x.cpu().double().abs()}
+    for k, n in (("x", "dx"), ("w", "dw")):
+        v, e = want[n]
+        # (what the second value leaves: half a step of a number that is half a step of dz at most, or a least subnormal)
+        e = e + u * u * left[n] + S.TINY[dtype] * (x.abs().sum(0).cpu().double() if n == "dw" else w.abs().sum(0).cpu().double())
+        S.check(g[k], (v, e + u * (v.abs() + e) + S.TINY[dtype]), f"{size} {act} {n}")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("size", [(300, 600, 130), (2500, 300, 140), (200, 40, 300)], ids=lambda s: "x".join(map(str, s)))
 def test_linear_wide_layouts(dev, size, dtype):
