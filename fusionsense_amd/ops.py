@@ -1924,7 +1924,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     place).  Differentiable in all four tensors, once; the backward forms the pre-activation again from ``x``.  In the
     half-width types the gradient of the pre-activation is rounded to that type before its two products (the rounding an
     unfused layer makes when it stores that gradient), except where that one rounding could be most of the error: 512 values
-    of it and 2^18 weights at most, or 128 inputs and a thousand values of ``x``'s or the weight's gradient at most.  A wide relu layer takes its slope from the sign of the rounded output."""
+    of it and 2^18 weights at most, or 128 inputs and a thousand values of ``x``'s or the weight's gradient at most.  A wide relu
+    layer takes its slope from the sign of the rounded output."""
     _require_float(x, "x")
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
         if t is None and name != "weight":
