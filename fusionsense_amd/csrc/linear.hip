@@ -442,7 +442,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinArgs a) {
 //   kStoreStream  past the caches; rows must start at 64-byte boundaries, which a store instruction then covers whole
 //   kStoreTile    the wave's 16 rows (neighbours in y) are put together in LDS and leave it as aligned streaming stores
 // Bound by memory where the activation is cheap (921 600 rows, 64 -> 64 fp32, silu and a residual: 139 us, 708 MB at 5.1 TB/s;
-// a 4 GiB copy reaches 4.8), by gelu's vector instructions at 640 000 rows, 64 -> 128 bf16 (59 us, 48 without it), and with
+// a 4 GiB copy reaches 4.8), by gelu's vector instructions at 640 000 rows, 64 -> 128 bf16 (61 us, 48 without it), and with
 // fp32 class scores (640 000 rows, 32 -> 150: 127 us, 466 MB at 3.7 TB/s) by what overlaps between twelve waves a CU.
 enum { kStorePlain = 0, kStoreStream = 1, kStoreTile = 2 };
 
@@ -1423,7 +1423,8 @@ template <typename T, int KC, int NG>
 int launch_bwd_rows(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
     if constexpr (bwd_rows_fits<T>(KC, NG)) {
         if constexpr (bwd_rows_fine<T>(KC, NG))
-            if (p.fine) return launch_bwd_rows_as<T, KC, NG, true>(a, p, s);
+            if (p.fine && (a.act == FSGS_ACT_GELU || a.act == FSGS_ACT_SILU))  // (the others' dz is dy or zero: exact)
+                return launch_bwd_rows_as<T, KC, NG, true>(a, p, s);
         return launch_bwd_rows_as<T, KC, NG, false>(a, p, s);
     } else {
         return FSGS_EINVAL;
