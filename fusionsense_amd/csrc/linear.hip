@@ -1300,6 +1300,7 @@ int launch_rows(const LinArgs &a, int transpose, hipStream_t s) {
 //   fp32 192 -> 256  40 000 rows (626) 46/48, 160 000 (2500) 162/152; 1024 -> 256  40 000 rows 205/211, 80 000 (1250) 400/346
 enum { kByRows, kByFew, kBySmall, kByTiles };
 constexpr int64_t kFewBytes = 4 << 20;
+constexpr int kFewTiles = 16;  // tiles of 128 x 128 up to which the few-rows kernel is asked
 
 template <typename T, int MODE>
 int product_kind(const LinArgs &a) {
@@ -1307,7 +1308,7 @@ int product_kind(const LinArgs &a) {
     const int64_t out = a.rows * a.N * (int64_t)sizeof(T), tiles = (a.rows + 127) / 128 * ((a.N + 127) / 128);
     if (a.K * sizeof(T) <= (half ? 256 : 512) && (a.N <= 32 || out < kFewBytes || rows_plan<T, MODE>(a).store != kStorePlain))
         return kByRows;
-    if (half ? a.K > 512 && tiles <= 8 : tiles <= 16) return kByFew;
+    if (half ? a.K > 512 && tiles <= kFewTiles / 2 : tiles <= kFewTiles) return kByFew;
     if (half ? a.K <= 2048 && tiles <= 512 : tiles <= 1024) return kBySmall;
     return kByTiles;
 }
@@ -1453,14 +1454,24 @@ int launch_bwd_rows_k(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s)
 
 struct BwdScratch {
     size_t dz, wt, part_w, part_b, total;
+    int64_t sums;  // rows of partial column sums that part_b holds
 };
+
+// Room for the partial column sums of dz, whichever kernel forms it (that depends on where the workspace lies too).  The tile
+// kernels leave two rows per tile, also for a single row of dz.
+int64_t most_sum_rows(int64_t rows, int N) {
+    const int64_t tiles = (rows + 127) / 128 * ((N + 127) / 128);
+    int64_t most = max(max(sum_rows_of(kByRows, rows), sum_rows_of(kBySmall, rows)), sum_rows_of(kByTiles, rows));
+    if (tiles <= kFewTiles) most = max(most, sum_rows_of(kByFew, rows));
+    return most;
+}
 
 BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bool dw, bool db) {
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     BwdScratch l;
     const BwdRowsPlan p = bwd_rows_plan(rows, K, N, e);
     if (p.kc) {
-        l.dz = l.wt = l.part_w = 0;
+        l.dz = l.wt = l.part_w = 0, l.sums = p.blocks;
         l.part_b = dw ? up((size_t)p.blocks * K * N * 4) : 0;
         l.total = l.part_b + (db ? up((size_t)p.blocks * N * 4) : 0);
         return l;
@@ -1470,10 +1481,8 @@ BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bo
     l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
     l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
     l.part_b = l.part_w + (dw ? up(s * (size_t)K * N * 4) : 0);
-    // (which kernel forms dz depends on where the workspace lies: room for any)
-    const int64_t dz_sums = max(sum_rows_of(kByRows, rows), sum_rows_of(rows <= 16 * 128 ? kByFew : kBySmall, rows));
-    const size_t sums = act != FSGS_ACT_NONE ? max((size_t)dz_sums, s) : s;
-    l.total = l.part_b + (db ? up(sums * (size_t)N * 4) : 0);
+    l.sums = act != FSGS_ACT_NONE ? max(most_sum_rows(rows, N), (int64_t)s) : (int64_t)s;
+    l.total = l.part_b + (db ? up((size_t)l.sums * (size_t)N * 4) : 0);
     return l;
 }
 
@@ -1519,6 +1528,7 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         LinArgs z = a;
         z.y = scratch + l.dz, z.yp = a.N, z.part_b = part_b;
         const int kind = product_kind<T, kModeDz>(z);
+        if (part_b && sum_rows_of(kind, a.rows) > l.sums) return FSGS_ESCRATCH;
         rc = launch_product<T, kModeDz>(z, kind, s);
         if (rc != FSGS_OK) return rc;
         dz = z.y, dzp = a.N, sum_rows = (int)sum_rows_of(kind, a.rows);

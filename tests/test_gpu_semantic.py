@@ -385,6 +385,28 @@ def test_linear_writes_its_outputs_only(dev, dtype):
                                    n - 1, stream_ptr(dev)) < 0  # (a workspace one byte short is refused)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("size", [(1, 256, 1024), (4, 512, 512), (16, 300, 200), (17, 300, 200), (5, 1024, 1500), (1, 256, 4096), (16, 200, 2100),
+                                  (9, 2100, 1100), (33, 130, 600), (64, 129, 300)], ids=lambda s: "x".join(map(str, s)))
+def test_linear_bwd_stays_inside_its_workspace(dev, dtype, act, size):
+    """Few rows of wide layers, whose dz the tile kernels form: nothing behind the workspace changes, and the bias gradient, which
+    is summed from it, is right."""
+    from fusionsense_amd._lib import load, ptr, stream_ptr
+    M, K, N = size
+    x, w, b, r, dy = _layer(dev, M, K, N, dtype, seed=63)
+    want, g0 = _check_layer(x, w, b, r, act, dy)
+    lib, dt, code = load(), ops.DTYPES[dtype], ops.ACTIVATIONS[act]
+    n = lib.fsgs_linear_bwd_scratch_bytes(M, K, N, dt, code, 1, 1, 1)
+    scratch = torch.full((n + 32 * N,), 0x5A, dtype=torch.uint8, device=dev)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    assert lib.fsgs_linear_bwd(M, K, N, dt, ptr(x), K, ptr(w), ptr(b), code, None, ptr(dy), N, ptr(dx), ptr(dw), ptr(db),
+                               ptr(scratch), n, stream_ptr(dev)) == 0
+    assert (scratch[n:] == 0x5A).all()
+    for got, k in ((dx, "x"), (dw, "w"), (db, "b")):
+        assert torch.equal(got, g0[k]), k
+
+
 # ---- distillation -------------------------------------------------------------------------------------------------
 def _record(dev, R, V, K, dtype, tdtype=torch.float32, idx_dtype=torch.int64, seed=0, ragged=True):
     g = torch.Generator().manual_seed(seed)

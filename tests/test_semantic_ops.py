@@ -76,6 +76,29 @@ def test_linear_bwd_entry_refuses():
     assert lib.fsgs_linear_bwd_scratch_bytes(4, 0, 8, 0, 1, 1, 1, 1) == -1
 
 
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [0, 1, 2], ids=["f32", "bf16", "f16"])
+def test_linear_bwd_workspace_holds_every_partial_sum(dtype, act):
+    """Layers too wide for the one-pass kernel (more than 512 bytes a row, or 256 outputs): the column sums of dz take two rows
+    per tile of 64 or of 128 rows, or one per 16 rows where there are 16 tiles of 128 x 128 at most; the workspace has room
+    for any of them, whichever gradients come with db."""
+    lib = _lib.load()
+    code, e = ops.ACTIVATIONS[act], 4 if dtype == 0 else 2
+    for K, N in ((64, 257), (129, 300), (200, 512), (256, 1024), (256, 4096), (300, 200), (512, 512), (768, 2050), (1024, 1500),
+                 (2049, 1025), (4096, 4096), (600, 8), (513, 65536)):
+        if K * e <= 512 and N <= 256:
+            continue
+        for rows in list(range(1, 82)) + [127, 128, 129, 1000, 2047, 2048, 2049, 2112, 5000]:
+            if dtype != 0 and rows * N <= 512 and K * N <= 1 << 18:
+                continue  # (one launch without a workspace)
+            tiles = -(-rows // 128) * -(-N // 128)
+            sums = max(2 * -(-rows // 64), 2 * -(-rows // 128), -(-rows // 16) if tiles <= 16 else 0)
+            for dx, dw in ((1, 1), (0, 0), (1, 0), (0, 1)):
+                room = (lib.fsgs_linear_bwd_scratch_bytes(rows, K, N, dtype, code, dx, dw, 1)
+                        - lib.fsgs_linear_bwd_scratch_bytes(rows, K, N, dtype, code, dx, dw, 0))
+                assert room >= 4 * N * sums, (rows, K, N, dx, dw, room, 4 * N * sums)
+
+
 def _dfwd(rows=4, v=8, k=2, dt=0, s=ONE, sp=8, bits=64, idx=ONE, tdt=0, u=ONE, T=1.0, red=2, loss=ONE, scratch=ONE, nbytes=1 << 30):
     return _lib.load().fsgs_distill_fwd(rows, v, k, dt, s, sp, bits, idx, k, tdt, u, k, None, T, red, loss, None, None, scratch,
                                         nbytes, None)
