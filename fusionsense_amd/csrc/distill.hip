@@ -153,12 +153,13 @@ __device__ __forceinline__ float chunks_max(const Chunk (&c)[STEPS]) {
 }
 
 // Exponents of a row against its maximum m, in base 2: one multiply-add per score, v scale2 - round(m scale2).  The shift's
-// rounding is the same for every score of the row and cancels in the softmax as long as all of its parts use this form; only
-// where m scale2 itself leaves the range (a row of nothing but the type's lowest value) the difference is taken first.
+// rounding is the same for every score of the row and cancels in the softmax as long as all of its parts use this form.  It is
+// 2^-9 at most: from a shift of 2^16 on the difference is taken first (from 2^32 on half a step of the shift alone would leave
+// the exponential's range: a row of nothing but -1e10, or scores of 12 345 at T = 1e-6).
 struct RowExp {
     float m, scale2, shift;
     bool far;
-    __device__ RowExp(float m_, float s) : m(m_ == -INFINITY ? 0.f : m_), scale2(s), shift(m * s), far(!(fabsf(shift) < 1e38f)) {}
+    __device__ RowExp(float m_, float s) : m(m_ == -INFINITY ? 0.f : m_), scale2(s), shift(m * s), far(!(fabsf(shift) < 65536.f)) {}
     __device__ __forceinline__ float of(float v) const { return far ? (v - m) * scale2 : fmaf(v, scale2, -shift); }
 };
 

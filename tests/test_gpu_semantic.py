@@ -564,6 +564,41 @@ def test_distill_masked_student(dev, dtype):
     assert torch.isnan(loss[[4, 5, 6]]).all() and torch.isfinite(loss[[0, 1, 2, 3, 7]]).all()
 
 
+def _far_scores(dev, V, K, dtype, T, seed):
+    """Rows whose maximum lies anywhere in the type's range: (a) every class at one value (a mask that rules all of them out, or a
+    constant), (b) a tenth of the classes around zero and the others at a mask value, (c) N(0, 2) T around an offset."""
+    top = torch.finfo(dtype).max
+    sizes = [s * v for v in (12.0, 345.0, 12345.0, 60000.0, 3e6, 1e9, 1e10, 1e12, 1e20, 1e30, 3e38) if v <= top for s in (1, -1)]
+    g = torch.Generator().manual_seed(seed)
+    rows = [torch.full((V,), v, dtype=torch.float64) for v in sizes]
+    for v in sizes:
+        if v < 0:
+            row = torch.randn(V, generator=g, dtype=torch.float64) * 2 * T
+            row[(torch.arange(V) * 7) % 10 != 0] = v
+            rows.append(row)
+    rows += [torch.randn(V, generator=g, dtype=torch.float64) * 2 * T + v for v in sizes]
+    logits = torch.stack(rows).clamp(-top, top).to(dtype)
+    R = logits.shape[0]
+    # (entries among the classes around zero of (b): a ruled-out class that the teacher wants has a loss beyond fp32)
+    zero = torch.arange(V)[(torch.arange(V) * 7) % 10 == 0]
+    idx = zero[torch.rand(R, zero.numel(), generator=g).topk(min(K, zero.numel()), dim=1).indices]
+    teacher = torch.randn(idx.shape, generator=g) * 2 * T
+    return logits.to(dev), idx.to(dev), teacher.to(dev)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("T", [1e-6, 1e-3, 0.5, 1.0, 30.0, 1e6])
+@pytest.mark.parametrize("V", [11, 21, 150, 1203])
+def test_distill_far_scores(dev, dtype, T, V):
+    """Maxima over the whole range of the type, temperatures at both ends of theirs: finite, and within the bound that only
+    counts differences from the row's maximum.  (A gradient goes up to T: fp16 has 65 504.)"""
+    T = min(T, 1e4) if dtype == torch.float16 else T
+    args = _far_scores(dev, V, 6, dtype, T, seed=91)
+    for reduction in ("none", "mean"):
+        loss, grad = _check_distill(*args, T, None, reduction, what=f"{reduction}")
+        assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("V,K", [(30, 8), (150, 64), (1500, 200), (33000, 70)])
 def test_distill_repeated_classes(dev, dtype, V, K):
