@@ -152,14 +152,19 @@ __device__ __forceinline__ float chunks_max(const Chunk (&c)[STEPS]) {
     }
 }
 
-// Exponents of a row against its maximum m, in base 2: one multiply-add per score, v scale2 - round(m scale2).  The shift's
-// rounding is the same for every score of the row and cancels in the softmax as long as all of its parts use this form.  It is
-// 2^-9 at most: from a shift of 2^16 on the difference is taken first (from 2^32 on half a step of the shift alone would leave
-// the exponential's range: a row of nothing but -1e10, or scores of 12 345 at T = 1e-6).
+// Exponents of a row against its maximum m, in base 2.  A row that its lanes hold whole: one multiply-add per score, v scale2 -
+// round(m scale2).  The shift's rounding is the same for every score of the row and cancels in the softmax, as all of its parts
+// use this form.  It is 2^-9 at most: from a shift of 2^16 on the difference is taken first (from 2^32 on half a step of the
+// shift alone would leave the exponential's range: a row of nothing but -1e10, or scores of 12 345 at T = 1e-6).
+// A row that fills a workgroup always takes the difference first: its lanes sum against maxima of their own, whose shifts'
+// roundings would stay in the sum (4e-6 of it at an offset of 1000, 4e-5 at 1e4).  It costs nothing there (V = 32 003: 200 us
+// either way, forward and backward); held rows would pay for it (800x800 x 150 fp32: 264 against 292).
+template <int L>
 struct RowExp {
     float m, scale2, shift;
     bool far;
-    __device__ RowExp(float m_, float s) : m(m_ == -INFINITY ? 0.f : m_), scale2(s), shift(m * s), far(!(fabsf(shift) < 65536.f)) {}
+    __device__ RowExp(float m_, float s)
+        : m(m_ == -INFINITY ? 0.f : m_), scale2(s), shift(m * s), far(L == kWideRow || !(fabsf(shift) < 65536.f)) {}
     __device__ __forceinline__ float of(float v) const { return far ? (v - m) * scale2 : fmaf(v, scale2, -shift); }
 };
 
@@ -223,7 +228,7 @@ __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel
             const float before = m;
             m = fmaxf(m, chunks_max<T>(c));
             if constexpr (L != kWideRow) row_reduce<L, MaxOp>(m, um, any);
-            const RowExp x(m, a.scale2);
+            const RowExp<L> x(m, a.scale2);
             if constexpr (L == kWideRow) sum *= exp2_hw(x.of(before));
             auto add = [&](auto exponent) {
 #pragma unroll
@@ -245,9 +250,9 @@ __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel
         if constexpr (L == kWideRow) {
             const float lane_m = m;
             row_reduce<L, MaxOp>(m, um, any);
-            sum *= exp2_hw(RowExp(m, a.scale2).of(lane_m));
+            sum *= exp2_hw(RowExp<L>(m, a.scale2).of(lane_m));
         }
-        const RowExp x(m, a.scale2);
+        const RowExp<L> x(m, a.scale2);
         const bool alive = any != 0.f && w != 0.f;
         // sum_k p_k (log p_k - log q_k) = (sum_k e_k y_k) / Z - log Z + log S with e_k = exp((u_k - um) / T), Z their sum,
         // y_k = (u_k - um) / T - (s_k - m) / T; exponents and logarithms in base 2, ln 2 at the end
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(256, 5) void distill_bwd_kernel(DistillArgs a) {
         const float4 st = a.stat[row];
         const bool dead = st.w == 0.f || !here;
         const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * (a.g_per_row ? a.g[row] : up) * inv_w;
-        const RowExp x(st.x, a.scale2);
+        const RowExp<L> x(st.x, a.scale2);
         const float cq = dead ? 0.f : coef * st.y, cp = coef * st.w;
         auto class_of = [&](int k) { return class_at(a.idx, row * a.ip + k, a.idx64, a.V); };
         auto mass_of = [&](int k) { return cp * exp2_hw((teacher_at(a.u, row * a.up + k, a.tdtype) - st.z) * a.scale2); };
@@ -467,7 +472,7 @@ __global__ __launch_bounds__(256) void distill_bwd_wide_kernel(DistillArgs a) {
         const float4 st = a.stat[row];
         const bool dead = st.w == 0.f;
         const float coef = a.T * (a.weight ? a.weight[row] : 1.f) * (a.g_per_row ? a.g[row] : up) * inv_w;
-        const RowExp x(st.x, a.scale2);
+        const RowExp<L> x(st.x, a.scale2);
         const float cq = coef * st.y, cp = coef * st.w;
         // (at most one entry per lane: K <= 256)
         const int cls = sub < a.K && !dead ? class_at(a.idx, row * a.ip + sub, a.idx64, a.V) : -1;

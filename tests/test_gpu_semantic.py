@@ -588,7 +588,7 @@ def _far_scores(dev, V, K, dtype, T, seed):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("T", [1e-6, 1e-3, 0.5, 1.0, 30.0, 1e6])
-@pytest.mark.parametrize("V", [11, 21, 150, 1203])
+@pytest.mark.parametrize("V", [11, 21, 150, 1203, 9001])
 def test_distill_far_scores(dev, dtype, T, V):
     """Maxima over the whole range of the type, temperatures at both ends of theirs: finite, and within the bound that only
     counts differences from the row's maximum.  (A gradient goes up to T: fp16 has 65 504.)"""
@@ -597,6 +597,25 @@ def test_distill_far_scores(dev, dtype, T, V):
     for reduction in ("none", "mean"):
         loss, grad = _check_distill(*args, T, None, reduction, what=f"{reduction}")
         assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("T", [1e-3, 1.0, 7.0])
+@pytest.mark.parametrize("V", [150, 1203, 2561, 9000, 40001])
+def test_distill_offset_scores(dev, dtype, T, V):
+    """N(0, 2) T around a common offset over T of up to 1e6, either sign, and rows whose lanes see rising, falling and far apart
+    scores: the bound counts differences from the row's maximum, not the scores themselves."""
+    g = torch.Generator().manual_seed(92)
+    offsets = [s * v * T for v in (0.0, 50.0, 1e3, 1e4, 1e5, 1e6) for s in (1, -1) if v * T < torch.finfo(dtype).max / 2]
+    ramp = torch.linspace(-40, 0, V, dtype=torch.float64)
+    rows = [torch.randn(V, generator=g, dtype=torch.float64) * 2 * T + o for o in offsets]
+    rows += [r * T + o for o in offsets[-2:] for r in (ramp, ramp.flip(0), ramp[torch.randperm(V, generator=g)])]
+    logits = torch.stack(rows).to(dtype).to(dev)
+    R = len(rows)
+    idx = torch.randint(0, V, (R, 9), generator=g)
+    top = (torch.randn(R, 9, generator=g) * 2 * T + 1e3 * T).to(dev)
+    for reduction in ("none", "sum"):
+        _check_distill(logits, idx.to(dev), top, T, None, reduction, what=reduction)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
