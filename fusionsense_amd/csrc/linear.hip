@@ -95,28 +95,28 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
     }
 }
 
-// z -> act'(z) for N values.
+// z -> dz = d act'(z) for N values.  (relu takes d or nothing: an infinite or NaN gradient of a value that it cut off is gone.)
 template <typename T, int N>
-__device__ __forceinline__ void act_slope(float (&z)[N], int act) {
+__device__ __forceinline__ void act_bwd(float (&z)[N], const float (&d)[N], int act) {
     if (act == FSGS_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? 1.f : 0.f;
+        for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? d[i] : 0.f;
     } else if (act == FSGS_ACT_GELU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float e;
             const float p = normal_tail<T>(z[i], e), r = e * fmaf(-0.39894228040143268f, fabsf(z[i]), p);
-            z[i] = z[i] < 0.f ? r : 1.f - r;  // z < 0: h + z density; z >= 0: 1 - h + z density
+            z[i] = d[i] * (z[i] < 0.f ? r : 1.f - r);  // z < 0: h + z density; z >= 0: 1 - h + z density
         }
     } else if (act == FSGS_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[i] * -1.4426950408889634f));
-            z[i] = s * fmaf(z[i], 1.f - s, 1.f);
+            z[i] = d[i] * (s * fmaf(z[i], 1.f - s, 1.f));
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = 1.f;
+        for (int i = 0; i < N; ++i) z[i] = d[i];
     }
 }
 
@@ -322,11 +322,14 @@ __global__ __launch_bounds__(256, 3) void linear_tile_kernel(LinArgs a) {
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[e] = acc[2 * i + (e >> 2)][j][e & 3] + b[e];
-            if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
-            else act_fwd<T>(z, a.act);
-            if (side)
+            if constexpr (MODE == kModeDz) {
+                act_bwd<T>(z, sv, a.act);
+            } else {
+                act_fwd<T>(z, a.act);
+                if (side)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] = MODE == kModeDz ? z[e] * sv[e] : z[e] + sv[e];
+                    for (int e = 0; e < 8; ++e) z[e] += sv[e];
+            }
             if constexpr (MODE == kModeDz)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) colsum[e] += z[e];
@@ -404,20 +407,27 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinArgs a) {
         const int n = n0 + held_column<T>(lg, e);
         if (a.bias && n < a.N) z[e] += (float)((const T *)a.bias)[n];
     }
-    if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
-    else act_fwd<T>(z, a.act);
     const T *side = (const T *)(MODE == kModeDz ? a.dy : a.res);
     const int64_t sp = MODE == kModeDz ? a.dyp : a.rp;
     const bool here = m < a.rows;
+    float sv[8];
+    if (side)
+#pragma unroll
+        for (int q = 0; q < CPG; ++q) {
+            const int n = n0 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
+            unpack_chunk<T>(load_chunk_n(side + (here ? m : 0) * sp + n, a.N - n), sv + q * CE);
+        }
+    if constexpr (MODE == kModeDz) {
+        act_bwd<T>(z, sv, a.act);
+    } else {
+        act_fwd<T>(z, a.act);
+        if (side)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] += sv[e];
+    }
 #pragma unroll
     for (int q = 0; q < CPG; ++q) {
         const int n = n0 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
-        if (side) {
-            float sv[CE];
-            unpack_chunk<T>(load_chunk_n(side + (here ? m : 0) * sp + n, a.N - n), sv);
-#pragma unroll
-            for (int e = 0; e < CE; ++e) z[q * CE + e] = MODE == kModeDz ? z[q * CE + e] * sv[e] : z[q * CE + e] + sv[e];
-        }
         if (here && n < a.N) put_chunk((T *)a.y + m * a.yp + n, pack_chunk<T>(z + q * CE), a.N - n, false);
     }
     if (MODE == kModeDz && a.part_b) {
@@ -550,8 +560,7 @@ __global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(Row
             float z[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[e] = acc[e >> 2][e & 3] + bl[g * 32 + held_column<T>(lg, e)];
-            if constexpr (MODE == kModeDz) act_slope<T>(z, a.act);
-            else act_fwd<T>(z, a.act);
+            if constexpr (MODE == kModeFwd) act_fwd<T>(z, a.act);
             if (has_side) {
                 float sv[8];
 #pragma unroll
@@ -559,8 +568,12 @@ __global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(Row
                     if (ragged_n) sr.fix(sc[q], mr * sr.pitch + n0 + column(g, q), ncols - column(g, q), end || sr.pitch == 0);
                     unpack_chunk<T>(sc[q], sv + q * CE);
                 }
+                if constexpr (MODE == kModeDz) {
+                    act_bwd<T>(z, sv, a.act);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] = MODE == kModeDz ? z[e] * sv[e] : z[e] + sv[e];
+                    for (int e = 0; e < 8; ++e) z[e] += sv[e];
+                }
             }
             if (MODE == kModeDz && a.part_b) {
                 float c[8];
@@ -742,9 +755,9 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                 for (int q = 0; q < CPG; ++q) unpack_chunk<T>(dyc[g][q], d + q * CE);
                 load_dy(dyc[g], nr, g);
                 if (a.act != FSGS_ACT_NONE) {
-                    act_slope<T>(z, a.act);
+                    act_bwd<T>(z, d, a.act);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) d[e] *= z[e];
+                    for (int e = 0; e < 8; ++e) d[e] = z[e];
                 }
                 if constexpr (kRegDb)
 #pragma unroll
@@ -940,12 +953,13 @@ __global__ __launch_bounds__(64 * kSmallWaves) void linear_bwd_small_kernel(Smal
 #pragma unroll
             for (int q = 0; q < 4; ++q) z[q] = acc[q] + (bias && n0 + lg * 4 + q < a.N ? (float)bias[n0 + lg * 4 + q] : 0.f);
         }
-        act_slope<T>(z, a.act);
+        float d[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int n = n0 + lg * 4 + q;
-            if (m < a.rows && n < a.N) dz[m * a.N + n] = z[q] * (float)dy[m * a.dyp + n];
-        }
+        for (int q = 0; q < 4; ++q) d[q] = m < a.rows && n0 + lg * 4 + q < a.N ? (float)dy[m * a.dyp + n0 + lg * 4 + q] : 0.f;
+        act_bwd<T>(z, d, a.act);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (m < a.rows && n0 + lg * 4 + q < a.N) dz[m * a.N + n0 + lg * 4 + q] = z[q];
     }
     __syncthreads();
     const int k0 = blockIdx.x * kSmallCols, cols = min(kSmallCols, a.K - k0);

@@ -149,6 +149,26 @@ def test_linear_keeps_bad_values_in_their_rows(dev, dtype):
     assert torch.equal(y2[130], torch.where(w[:, 60] > 0, torch.full_like(r[130], float("inf")), r[130]))
 
 
+# A layer per kernel that forms dz: few values, one pass, few rows, rows, tiles of 64 and of 128 rows.
+DZ = [(3, 7, 5), (300, 64, 72), (40, 2000, 1100), (1100, 8, 400), (3000, 300, 70), (2200, 600, 130), (2200, 2100, 1100)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("res", [False, True], ids=["", "residual"])
+@pytest.mark.parametrize("size", DZ, ids=lambda s: "x".join(map(str, s)))
+def test_linear_relu_drops_gradients_of_what_it_cut_off(dev, dtype, res, size):
+    """Infinite and NaN gradients where the pre-activation is clearly negative: the bits that zeros there give."""
+    x, w, b, r, dy = _layer(dev, *size, dtype, res=res, seed=64)
+    z = x.float() @ w.float().t() + b.float()
+    cut = (z < -0.1) & (torch.rand(z.shape, generator=torch.Generator().manual_seed(65)).to(dev) < 0.2)
+    bad = torch.tensor([math.inf, -math.inf, math.nan], device=dev)[torch.arange(z.numel(), device=dev).reshape(z.shape) % 3].to(dtype)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    y = ops.linear_act(*leaves, "relu", r)
+    want = torch.autograd.grad(y, leaves, dy.masked_fill(cut, 0), retain_graph=True)
+    got = torch.autograd.grad(y, leaves, torch.where(cut, bad, dy))
+    assert cut.any() and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("K", [64, 700])
