@@ -1868,7 +1868,7 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         y = _linear_fwd(x, weight, bias, residual, act)
-        # (a wide relu layer takes its slope from the output's sign instead of forming the pre-activation again)
+        # (a wide relu layer takes its slope from the output's bits instead of forming the pre-activation again)
         N, K = weight.shape
         keep = (act == ACTIVATIONS["relu"] and residual is None and any(ctx.needs_input_grad[:3])
                 and load().fsgs_linear_bwd_uses_output(x.numel() // K, K, N, DTYPES[x.dtype], act) == 1)
@@ -1924,8 +1924,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     place).  Differentiable in all four tensors, once; the backward forms the pre-activation again from ``x``.  In the
     half-width types the gradient of the pre-activation is rounded to that type before its two products (the rounding an
     unfused layer makes when it stores that gradient), except where that one rounding could be most of the error: 512 values
-    of it and 2^18 weights at most, or 128 inputs and a thousand values of ``x``'s or the weight's gradient at most.  A wide relu
-    layer takes its slope from the sign of the rounded output."""
+    of it and 2^18 weights at most, or 128 inputs and a thousand values of ``x``'s or the weight's gradient at most.  A relu
+    output that is positive but rounds to zero is -0: a wide relu layer takes its slope from the output's bits."""
     _require_float(x, "x")
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
         if t is None and name != "weight":

@@ -1095,7 +1095,8 @@ int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype, const void
 /* VJP.  dx [rows, in], dw [out, in], db [out]: contiguous, written, each nullable (rows == 0 writes nothing: dw and db are
  * the caller's to clear).  The pre-activation is formed again from x, w and bias.  The residual's gradient is dy itself.
  * y: nullable; the forward's output [rows, out] (contiguous) of a layer WITHOUT residual.  Where
- * fsgs_linear_bwd_uses_output says 1 (relu layers too wide for the one-pass kernel) its sign saves that product. */
+ * fsgs_linear_bwd_uses_output says 1 (relu layers too wide for the one-pass kernel) its bits save that product: the forward
+ * stores a positive value that rounds to zero as -0. */
 int fsgs_linear_bwd_uses_output(int64_t rows, int in_dim, int out_dim, int dtype, int act);
 int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int act, int want_dx, int want_dw,
                                       int want_db);

@@ -169,6 +169,30 @@ def test_linear_relu_drops_gradients_of_what_it_cut_off(dev, dtype, res, size):
     assert cut.any() and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("res", [False, True], ids=["", "residual"])
+@pytest.mark.parametrize("size", DZ, ids=lambda s: "x".join(map(str, s)))
+def test_linear_relu_slope_of_values_that_round_to_zero(dev, size, res):
+    """fp16: a pre-activation of 2^-26 or 2^-25 has slope one though the output is zero, one of 0 or -2^-26 has none; alike in
+    every kernel.  (Column n of x picks row n's weight: one term a sum, exact.)"""
+    M, K, N = size
+    dtype = torch.float16
+    x, w, dy = torch.zeros(M, K, dtype=dtype), torch.zeros(N, K, dtype=dtype), _randn("cpu", M, N, seed=66, dtype=dtype)
+    x[:, 0] = 2.0 ** -13
+    values = torch.tensor([2.0 ** -13, 2.0 ** -12, 0.0, -(2.0 ** -13), 1.5 * 2.0 ** -12, 1.0])
+    w[:, 0] = values[torch.arange(N) % 6].to(dtype)
+    leaves = [t.to(dev).requires_grad_(True) for t in (x, w, torch.zeros(N, dtype=dtype))]
+    r = torch.zeros(M, N, dtype=dtype, device=dev) if res else None
+    y = ops.linear_act(*leaves, "relu", r)
+    z = x[0, 0].double() * w[:, 0].double()
+    assert torch.equal(y.detach().cpu(), z.clamp(min=0).to(dtype).expand(M, N)) and (z > 0).sum() > (y[0] != 0).sum()
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.to(dev))
+    dz = dy.double() * (z > 0)
+    for got, v, mag in ((dx, dz @ w.double(), dz.abs() @ w.double().abs()), (dw, dz.t() @ x.double(), dz.abs().t() @ x.double().abs()),
+                        (db, dz.sum(0), dz.abs().sum(0))):
+        e = (max(M, N) + 2) * S.U32 * mag
+        S.check(got, (v, e + S.U[dtype] * (v.abs() + e) + S.TINY[dtype]), "")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("K", [64, 700])
