@@ -26,35 +26,26 @@ struct LinArgs {
 };
 
 // The normal distribution's tail h = P(t) exp(-z^2 / 2) at |z|, t = 1 / (1 + c |z|), P a polynomial without a constant term
-// fitted to erfc here; P and the exponential apart.  fp32: degree 7, |error of h| < 9e-9, a seventh of half an fp32 step at 1;
-// half width: degree 5, < 4e-7, a six-hundredth of half an fp16 step.
-template <typename T>
+// fitted here to erfc over rounded coefficients; P and the exponential apart.  The fit is off by 1.3e-9 of h at most, a fiftieth
+// of half an fp32 step at 1; its evaluation in fp32 adds 1.5e-7, two and a half of those.  The slopes of every type and the
+// forward of fp32 and fp16 use it (far out an fp16 output's half step is five times the fit's |z| h).
 __device__ __forceinline__ float normal_tail(float z, float &e) {
-    constexpr float c = sizeof(T) == 4 ? 0.34f : 0.35f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(c, fabsf(z), 1.f));
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.32f, fabsf(z), 1.f));
     e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
-    float p;
-    if constexpr (sizeof(T) == 4) {
-        p = fmaf(0.04310445f, t, -0.19278112f);
-        p = fmaf(p, t, 0.24988606f);
-        p = fmaf(p, t, -0.0172307f);
-        p = fmaf(p, t, 0.1495994f);
-        p = fmaf(p, t, 0.13158924f);
-        p = fmaf(p, t, 0.13583268f);
-    } else {
-        p = fmaf(-0.09327425f, t, 0.2608071f);
-        p = fmaf(p, t, 0.03706592f);
-        p = fmaf(p, t, 0.15632539f);
-        p = fmaf(p, t, 0.1390755f);
-    }
+    float p = fmaf(0.04611215f, t, -0.24249351f);
+    p = fmaf(p, t, 0.41171595f);
+    p = fmaf(p, t, -0.16985106f);
+    p = fmaf(p, t, 0.22053833f);
+    p = fmaf(p, t, 0.104102224f);
+    p = fmaf(p, t, 0.12987591f);
     return p * t;
 }
 
-// The tail at |z| for the half-width types' forward as one exponential: 2^Q(|z|), Q a polynomial of degree 9 fitted here to
-// log2 of the tail on [0, 13.2] and falling on from there.  The relative error stays below 5e-6 at |z| < 1, 3e-5 < 2, 1e-4
-// everywhere, so that |z| h is off by 1.4e-6 at most: under a hundredth of an fp16 step at 1, a fifth of its half step far out.
+// The tail at |z| for the bf16 forward as one exponential: 2^Q(|z|), Q a polynomial of degree 9 fitted here to log2 of the tail
+// on [0, 13.2] and falling on from there.  The relative error stays below 5e-6 at |z| < 1, 3.1e-5 < 2, 1e-4 everywhere: a
+// twentieth of a bf16 output's half step or less (of fp16's, two fifths far out: that type takes the form above).
 // (640 000 rows, 64 -> 128 bf16: 61.5 us; by the form above, with its reciprocal, 64.8.)
-__device__ __forceinline__ float normal_tail_half(float z) {
+__device__ __forceinline__ float normal_tail_bf16(float z) {
     const float a = fabsf(z);
     float q = fmaf(-1.56790725e-09f, a, 1.2192244e-07f);
     q = fmaf(q, a, -4.12213922e-06f);
@@ -84,11 +75,11 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float h;
-            if constexpr (sizeof(T) == 2) {
-                h = normal_tail_half(z[i]);
+            if constexpr (std::is_same_v<T, __bf16>) {
+                h = normal_tail_bf16(z[i]);
             } else {
                 float e;
-                h = normal_tail<T>(z[i], e);
+                h = normal_tail(z[i], e);
                 h *= e;
             }
             // z >= 0: z - z h; z < 0: -|z| h  (+inf, where h is zero, stays; -inf and NaN give NaN, as z Phi(z) does)
@@ -111,7 +102,7 @@ __device__ __forceinline__ void act_bwd(float (&z)[N], const float (&d)[N], int 
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float e;
-            const float p = normal_tail<T>(z[i], e), r = e * fmaf(-0.39894228040143268f, fabsf(z[i]), p);
+            const float p = normal_tail(z[i], e), r = e * fmaf(-0.39894228040143268f, fabsf(z[i]), p);
             z[i] = d[i] * (z[i] < 0.f ? r : 1.f - r);  // z < 0: h + z density; z >= 0: 1 - h + z density
         }
     } else if (act == FSGS_ACT_SILU) {

@@ -195,6 +195,39 @@ def test_linear_relu_slope_of_values_that_round_to_zero(dev, size, res):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_linear_activation_over_its_range(dev, dtype, act):
+    """act and its slope of single numbers over [-14, 14] (one term a sum: z is exact).
+
+    gelu's tail h = P(t) exp(-z^2/2) is off by its fit, 1.3e-9, and relatively by the exponent's rounding, z^2 / 2 times two
+    roundings, and by 32 U32 for P (seven steps, magnitudes 2.7 times the sum), the reciprocal and the exponential; bf16's form by
+    1e-4.  y = max(z, 0) - |z| h; the slope is h - |z| phi, or one minus that.  silu's sigma is off by (2 |z| + 8) U32 of itself.
+    The type's rounding comes last; dz enters its product as two values of a half-width type."""
+    z = torch.linspace(-14, 14, 100000).to(dtype)
+    x = z[:, None].to(dev).requires_grad_(True)
+    y = ops.linear_act(x, torch.ones(1, 1, dtype=dtype, device=dev), None, act)
+    dx, = torch.autograd.grad(y, [x], torch.ones_like(y))
+    z = z.double()
+    u, size = S.U[dtype], z.abs()
+    if act == "gelu":
+        h, phi = 0.5 * torch.erfc(size / math.sqrt(2)), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        rel = (z * z + 32) * S.U32
+        # (the exponential instruction gives zero for what lies below 2^-126, bf16's tail from |z| = 13.1 on: off by that at most)
+        ey = size * (1e-4 * h + 2.0 ** -126 if dtype == torch.bfloat16 else 1.3e-9 + rel * h)
+        es = 1.3e-9 + rel * (h + size * phi) + 2 * S.U32
+        low = 0.5 * torch.erfc(-z / math.sqrt(2))  # (1 + erf, as S has it, is 2e-16 off: all of the value at z = -9)
+        vy, vs = z * low, low + z * phi
+    else:
+        rel = (2 * size + 8) * S.U32
+        ey = rel * size * torch.sigmoid(z)
+        es = 2 * rel * torch.sigmoid(z) * (1 + size) + 2 * S.U32
+        vy, vs = S.act(z, act), S.slope(z, act)
+    for got, v, e in ((y, vy, ey), (dx, vs, es)):
+        e = e + 2 * S.U32 * v.abs() + (u * u * v.abs() + S.TINY[dtype] if got is dx and dtype != torch.float32 else 0)
+        S.check(got, (v[:, None], (e + u * (v.abs() + e) + S.TINY[dtype])[:, None]), "y" if got is y else "dx")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("K", [64, 700])
 def test_linear_infinite_pre_activations(dev, dtype, act, K):
     """What z Phi(z) and z sigma(z) give: +inf stays, -inf and NaN become NaN, the largest finite sums stay or vanish."""

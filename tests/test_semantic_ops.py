@@ -136,6 +136,38 @@ def test_semantic_head_refuses(kw):
         SemanticHead(**args)
 
 
+def _coefficients(function):
+    import os
+    import re
+    src = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "linear.hip")).read()
+    body = src[src.index(f"float {function}(") :]
+    body = body[:body.index("\n}")]
+    first, rest = re.search(r"fmaf\(([-\d.e]+)f, [ta], ([-\d.e]+)f\)", body), re.findall(r"fmaf\([pq], [ta], ([-\d.e]+)f\)", body)
+    scale = re.search(r"fmaf\(([\d.]+)f, fabsf", body)
+    f32 = lambda v: float(torch.tensor(float(v), dtype=torch.float32))  # noqa: E731
+    return [f32(v) for v in (*first.groups(), *rest)], f32(scale.group(1)) if scale else None
+
+
+def test_gelu_tails_are_as_close_as_their_comments_say():
+    """The normal tail's two fits, evaluated in 64 bits with the coefficients that the source holds."""
+    z = torch.linspace(0, 13, 400001, dtype=torch.float64)
+    e = torch.exp(-z * z / 2)
+    h = 0.5 * torch.special.erfcx(z / 2 ** 0.5) * e
+    c, scale = _coefficients("normal_tail")
+    assert len(c) == 7
+    t, p = 1 / (1 + scale * z), torch.zeros_like(z)
+    for v in c:
+        p = p * t + v
+    assert (p * t * e - h).abs().max() < 1.3e-9
+    c, _ = _coefficients("normal_tail_bf16")
+    assert len(c) == 10
+    q = torch.zeros_like(z)
+    for v in c:
+        q = q * z + v
+    rel = (torch.exp2(q) / h - 1).abs()
+    assert rel[z < 1].max() < 5e-6 and rel[z < 2].max() < 3.1e-5 and rel.max() < 1e-4
+
+
 def test_semantic_head_parameters():
     g = torch.Generator().manual_seed(0)
     h = SemanticHead(5, 7, hidden=6, blocks=2, generator=g)
