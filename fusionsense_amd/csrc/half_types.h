@@ -1,5 +1,7 @@
 // The three element types of the semantic-head operators (fp32 / bf16 / fp16) and their matrix instructions.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace fsgs {
@@ -97,6 +99,34 @@ __device__ __forceinline__ void unpack_chunk(const Chunk &c, float *v) {
     __builtin_memcpy(t, &c, sizeof(Chunk));
 #pragma unroll
     for (int e = 0; e < kChunk<T>; ++e) v[e] = (float)t[e];
+}
+
+// kChunk floats as the sum of two chunks of a half-width type: hi the rounded values, lo what that left, rounded.  Together 16 bits
+// of a value (bf16) or 22 (fp16, down to the absolute 2^-25 that half of its least number is).  Values of up to twice fp16's
+// largest number are held too; infinities lie in hi alone.
+template <typename T>
+__device__ __forceinline__ Chunk split_chunk(const float *v, Chunk &lo) {
+    static_assert(sizeof(T) == 2);
+    constexpr float kMax = std::is_same_v<T, _Float16> ? 65504.f : 0x1.fep127f;
+    float r[8], m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+    Chunk hi = pack_chunk<T>(v);
+    unpack_chunk<T>(hi, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = v[e] - r[e];
+    if (__any(m > kMax)) {
+        float h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool finite = fabsf(v[e]) < INFINITY;
+            h[e] = finite ? __builtin_amdgcn_fmed3f(v[e], -kMax, kMax) : v[e];
+            r[e] = finite ? v[e] - (float)(T)h[e] : 0.f;
+        }
+        hi = pack_chunk<T>(h);
+    }
+    lo = pack_chunk<T>(r);
+    return hi;
 }
 
 // Past the caches: for outputs that no kernel reads while they could still be there.  16-byte aligned.

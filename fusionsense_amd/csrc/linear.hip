@@ -6,8 +6,6 @@
 //
 // Products run on the matrix cores in the tensors' own type, sums are fp32 throughout (fp32 tensors use the fp32 matrix
 // instructions: no reduced-precision product).
-#include <type_traits>
-
 #include "half_types.h"
 
 namespace fsgs {
@@ -23,12 +21,13 @@ struct LinArgs {
     int K, N, act;
     int stream;     // general tile: store past the caches
     float *part_b;  // dz kernels: partial column sums of dz, or null
+    int lo;         // dz kernels: dz as two values, the second this many columns on; 0: one value
 };
 
 // The normal distribution's tail h = P(t) exp(-z^2 / 2) at |z|, t = 1 / (1 + c |z|), P a polynomial without a constant term
 // fitted here to erfc over rounded coefficients; P and the exponential apart.  The fit is off by 1.3e-9 of h at most, a fiftieth
-// of half an fp32 step at 1; its evaluation in fp32 adds 1.5e-7, two and a half of those.  The slopes of every type and the
-// forward of fp32 and fp16 use it (far out an fp16 output's half step is five times the fit's |z| h).
+// of half an fp32 step at 1; its evaluation in fp32 adds 1.5e-7, two and a half of those.  The slopes of every type and
+// fp32's forward use it.
 __device__ __forceinline__ float normal_tail(float z, float &e) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.32f, fabsf(z), 1.f));
     e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
@@ -41,21 +40,33 @@ __device__ __forceinline__ float normal_tail(float z, float &e) {
     return p * t;
 }
 
-// The tail at |z| for the bf16 forward as one exponential: 2^Q(|z|), Q a polynomial of degree 9 fitted here to log2 of the tail
-// on [0, 13.2] and falling on from there.  The relative error stays below 5e-6 at |z| < 1, 3.1e-5 < 2, 1e-4 everywhere: a
-// twentieth of a bf16 output's half step or less (of fp16's, two fifths far out: that type takes the form above).
-// (640 000 rows, 64 -> 128 bf16: 61.5 us; by the form above, with its reciprocal, 64.8.)
-__device__ __forceinline__ float normal_tail_bf16(float z) {
+// The tail at |z| for the half-width types' forward as one exponential: 2^Q(|z|), Q a polynomial fitted here to log2 of the tail.
+// bf16: degree 9 on [0, 13.2]; relative errors below 5e-6 at |z| < 1, 3.1e-5 < 2, 1e-4 everywhere, a twentieth of an output's
+// half step or less.  fp16: degree 7 on [0, 6], behind which outputs are zero; 5.6e-6, a fortieth.  Both fall on behind
+// their ranges.  (640 000 rows, 64 -> 128: bf16 61 us, fp16 59; by the form above, with its reciprocal, 65 and 72.)
+template <typename T>
+__device__ __forceinline__ float normal_tail_half(float z) {
     const float a = fabsf(z);
-    float q = fmaf(-1.56790725e-09f, a, 1.2192244e-07f);
-    q = fmaf(q, a, -4.12213922e-06f);
-    q = fmaf(q, a, 8.01530987e-05f);
-    q = fmaf(q, a, -0.00100325886f);
-    q = fmaf(q, a, 0.00863550697f);
-    q = fmaf(q, a, -0.0540182889f);
-    q = fmaf(q, a, -0.458512872f);
-    q = fmaf(q, a, -1.15121996f);
-    q = fmaf(q, a, -0.999997079f);
+    float q;
+    if constexpr (std::is_same_v<T, __bf16>) {
+        q = fmaf(-1.56790725e-09f, a, 1.2192244e-07f);
+        q = fmaf(q, a, -4.12213922e-06f);
+        q = fmaf(q, a, 8.01530987e-05f);
+        q = fmaf(q, a, -0.00100325886f);
+        q = fmaf(q, a, 0.00863550697f);
+        q = fmaf(q, a, -0.0540182889f);
+        q = fmaf(q, a, -0.458512872f);
+        q = fmaf(q, a, -1.15121996f);
+        q = fmaf(q, a, -0.999997079f);
+    } else {
+        q = fmaf(-1.8348113e-06f, a, 6.159829e-05f);
+        q = fmaf(q, a, -0.00093052484f);
+        q = fmaf(q, a, 0.008507891f);
+        q = fmaf(q, a, -0.05396007f);
+        q = fmaf(q, a, -0.45846438f);
+        q = fmaf(q, a, -1.1512511f);
+        q = fmaf(q, a, -0.9999953f);
+    }
     return __builtin_amdgcn_exp2f(q);
 }
 
@@ -75,8 +86,8 @@ __device__ __forceinline__ void act_fwd(float (&z)[N], int act) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float h;
-            if constexpr (std::is_same_v<T, __bf16>) {
-                h = normal_tail_bf16(z[i]);
+            if constexpr (sizeof(T) == 2) {
+                h = normal_tail_half<T>(z[i]);
             } else {
                 float e;
                 h = normal_tail(z[i], e);
@@ -170,6 +181,20 @@ __device__ __forceinline__ void put_chunk(T *to, const Chunk &c, int n, bool str
             if (e < n) to[e] = t[e];
         asm volatile("; part of a chunk" ::: "memory");
     }
+}
+
+// A lane's values of a row of the output.
+template <typename T, int MODE>
+__device__ __forceinline__ void put_values(T *to, const float *v, int n, bool stream, int lo) {
+    if constexpr (MODE == kModeDz && sizeof(T) == 2) {
+        if (lo) {
+            Chunk rest;
+            put_chunk(to, split_chunk<T>(v, rest), n, stream);
+            put_chunk(to + lo, rest, n, stream);
+            return;
+        }
+    }
+    put_chunk(to, pack_chunk<T>(v), n, stream);
 }
 
 // ---- general tile: 32 MT rows x BN columns, four waves of 16 MT x BN/2 ---------------------------------------------------
@@ -333,7 +358,7 @@ __global__ __launch_bounds__(256, 3) void linear_tile_kernel(LinArgs a) {
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
                 const int n = n0 + wn + i * 32 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
-                if (n < a.N) put_chunk((T *)a.y + m * a.yp + n, pack_chunk<T>(z + q * CE), a.N - n, stream);
+                if (n < a.N) put_values<T, MODE>((T *)a.y + m * a.yp + n, z + q * CE, a.N - n, stream, a.lo);
             }
         }
         if constexpr (MODE == kModeDz)
@@ -425,7 +450,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinArgs a) {
 #pragma unroll
     for (int q = 0; q < CPG; ++q) {
         const int n = n0 + (CPG == 1 ? lg * 8 : q * 16 + lg * 4);
-        if (here && n < a.N) put_chunk((T *)a.y + m * a.yp + n, pack_chunk<T>(z + q * CE), a.N - n, false);
+        if (here && n < a.N) put_values<T, MODE>((T *)a.y + m * a.yp + n, z + q * CE, a.N - n, false, a.lo);
     }
     if (MODE == kModeDz && a.part_b) {
 #pragma unroll
@@ -456,7 +481,7 @@ enum { kStorePlain = 0, kStoreStream = 1, kStoreTile = 2 };
 struct RowsArgs {
     LinArgs l;
     int range;      // columns per workgroup (a multiple of 32)
-    int transpose;  // W is given as [K,N] (its element (n,k) at k * N + n)
+    int transpose;  // W is given as [transpose,N], its element (n,k) at k * N + n; a longer K runs through it once more
 };
 
 template <typename T, int KC>
@@ -477,7 +502,7 @@ __device__ __forceinline__ void fill_weights(Chunk *wl, const T *w, int n0, int 
     } else {
         for (int c = threadIdx.x; c < range * KC * 4 * CE; c += blockDim.x) {
             const int k = c / range, n = c % range;
-            ((T *)(wl + n * P))[k] = n0 + n < N && k < K ? w[(int64_t)k * N + n0 + n] : (T)0.f;
+            ((T *)(wl + n * P))[k] = n0 + n < N && k < K ? w[(int64_t)(k < transpose ? k : k - transpose) * N + n0 + n] : (T)0.f;
         }
     }
 }
@@ -584,10 +609,9 @@ __global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(Row
 #pragma unroll
             for (int q = 0; q < CPG; ++q) {
                 const int n = column(g, q);
-                const Chunk o = pack_chunk<T>(z + q * CE);
                 if (m < a.rows && n < ncols) {
-                    if constexpr (STORE == kStoreTile) put_chunk((T *)mine + off + li * a.N + n, o, ncols - n, false);
-                    else put_chunk(y + m * a.yp + n0 + n, o, ncols - n, STORE == kStoreStream);
+                    if constexpr (STORE == kStoreTile) put_chunk((T *)mine + off + li * a.N + n, pack_chunk<T>(z + q * CE), ncols - n, false);
+                    else put_values<T, MODE>(y + m * a.yp + n0 + n, z + q * CE, ncols - n, STORE == kStoreStream, a.lo);
                 }
             }
         }
@@ -617,7 +641,7 @@ __global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(Row
 
 // ---- backward of a layer whose two axes are both short: one pass over x and dy -----------------------------------------
 // A workgroup of eight waves takes 128 rows at a time, a wave 16 of them.  Per 32 columns: z from W (LDS) and the wave's rows of
-// x, dz = dy act'(z) in fp32 registers (db is summed from these), rounded once to T and used twice: as it stands it is the B
+// x, dz = dy act'(z) in fp32 registers (db is summed from these), put into T and used twice: as it stands it is the B
 // operand of dx^T = W^T dz^T, and through LDS it meets x again in dW = dz^T x, whose whole [N,K] lies in the workgroup's
 // registers for the life of the workgroup.  x and dy are read once, dx is written once; W is held once, read along its rows for
 // z and along its columns for dx.
@@ -650,7 +674,7 @@ struct BwdRowsLds {
 };
 
 // NG: groups of 32 columns that the registers provide for.  FINE: dz goes into its products as the sum of two values of T, the
-// rounded one and what that left (BwdRowsPlan::fine).
+// rounded one and what that left (split_chunk).
 template <typename T, int KC, int NG, bool FINE>
 __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdRowsArgs a) {
     constexpr int CE = kChunk<T>, CPG = sizeof(T) == 2 ? 1 : 2;
@@ -709,12 +733,14 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                 for (int c = 0; c < KC; ++c)
                     xr.fix(xf[c], mr * a.xp + (c * 4 + lg) * CE, m < a.rows ? a.K - (c * 4 + lg) * CE : 0, end || a.xp == 0);
             // dx^T tiles: rows k of a pair of tiles are 8 neighbours per lane in half width, 4 of one tile in fp32
-            auto add_dx = [&](f32x4 &acc, int kt, int g, const Chunk (&dz)[CPG]) {
+            auto add_dx = [&](f32x4 &acc, int kt, int g, const Chunk (&dz)[CPG], const Chunk (&lo)[CPG]) {
                 const int col = CPG == 1 ? (kt >> 1) * 32 + (li & 3) * 8 + (kt & 1) * 4 : kt * 16 + li;
 #pragma unroll
                 for (int q = 0; q < CPG; ++q) {
                     const int n = column(g, q);
-                    mma_chunk<T>(acc, load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col), dz[q]);
+                    const Chunk wc = load_columns<T>(mem + lay.w, lay.pk, n, n + 4, col);
+                    mma_chunk<T>(acc, wc, dz[q]);
+                    if constexpr (FINE) mma_chunk<T>(acc, wc, lo[q]);
                 }
             };
             auto store_dx = [&](int kt, const f32x4 *acc) {
@@ -725,7 +751,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                 if (m < a.rows && k < a.K) put_chunk((T *)a.dx + m * a.K + k, pack_chunk<T>(v), a.K - k, a.stream);
             };
             // whichever holds fewer registers meanwhile: dx summed group by group, or the groups' dz kept and dx done at the end
-            constexpr bool kKeepDz = KT > NG * CPG;
+            constexpr bool kKeepDz = KT > NG * CPG * (FINE ? 2 : 1);
             f32x4 accx[kKeepDz ? 1 : KT] = {};
             Chunk dzc[kKeepDz ? NG : 1][CPG], loc[FINE && kKeepDz ? NG : 1][CPG];
 #pragma unroll
@@ -759,28 +785,22 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                 if constexpr (kRegDb)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) db[g][e] += d[e];
-                Chunk (&dz)[CPG] = dzc[kKeepDz ? g : 0];
+                Chunk (&dz)[CPG] = dzc[kKeepDz ? g : 0], (&lo)[CPG] = loc[FINE && kKeepDz ? g : 0];
 #pragma unroll
                 for (int q = 0; q < CPG; ++q) {
-                    dz[q] = pack_chunk<T>(d + q * CE);
-                    *(Chunk *)(mem + lay.dz + row * lay.pn + column(g, q) * (int)sizeof(T)) = dz[q];
-                }
-                Chunk (&lo)[CPG] = loc[FINE && kKeepDz ? g : 0];
-                if constexpr (FINE) {
-                    float r[8];
-                    unpack_chunk<T>(dz[0], r);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) r[e] = fabsf(r[e]) <= 3.4028235e38f ? d[e] - r[e] : 0.f;  // (infinities stay)
-                    lo[0] = pack_chunk<T>(r);
-                    *(Chunk *)(mem + lay.lo + row * lay.pn + column(g, 0) * (int)sizeof(T)) = lo[0];
+                    char *const to = mem + lay.dz + row * lay.pn + column(g, q) * (int)sizeof(T);
+                    if constexpr (FINE) {
+                        dz[q] = split_chunk<T>(d + q * CE, lo[q]);
+                        *(Chunk *)(to + (lay.lo - lay.dz)) = lo[q];
+                    } else {
+                        dz[q] = pack_chunk<T>(d + q * CE);
+                    }
+                    *(Chunk *)to = dz[q];
                 }
                 if constexpr (!kKeepDz)
                     if (a.dx)
 #pragma unroll
-                        for (int kt = 0; kt < KT; ++kt) {
-                            add_dx(accx[kt], kt, g, dz);
-                            if constexpr (FINE) add_dx(accx[kt], kt, g, lo);
-                        }
+                        for (int kt = 0; kt < KT; ++kt) add_dx(accx[kt], kt, g, dz, lo);
             }
             if (a.dx) {
                 if constexpr (!kKeepDz) {
@@ -794,10 +814,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
                         for (int g = 0; g < NG; ++g)
                             if (g < ng)
 #pragma unroll
-                                for (int i = 0; i < 3 - CPG; ++i) {
-                                    add_dx(acc[i], kt + i, g, dzc[g]);
-                                    if constexpr (FINE) add_dx(acc[i], kt + i, g, loc[g]);
-                                }
+                                for (int i = 0; i < 3 - CPG; ++i) add_dx(acc[i], kt + i, g, dzc[g], loc[FINE ? g : 0]);
                         store_dx(kt, acc);
                     }
                 }
@@ -896,10 +913,8 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
     }
 }
 
-// ---- backward of a few rows and outputs, half width: one launch, dz never rounded -----------------------------------------
-// In the kernels above and below dz is rounded to T for its two products, up to half a step of each value: over many values that
-// adds two fifths to the error of the gradients' own rounding, but over few it may double it.  Here every workgroup forms all of
-// dz (rows x N) by itself in fp32 LDS and takes 32 columns of dW and dx.  Bound by latency: 16 rows, 64 -> 20 bf16 6.4 us; one row,
+// ---- backward of a few rows and outputs, half width: one launch ------------------------------------------------------------
+// Every workgroup forms all of dz (rows x N) by itself in fp32 LDS and takes 32 columns of dW and dx.  Bound by latency: 16 rows, 64 -> 20 bf16 6.4 us; one row,
 // 64 -> 150 10.8, where four rows take 15 in the one-pass kernel and its sum over slices; one row, 512 -> 512 43.
 constexpr int kSmallDz = 512, kSmallCols = 32, kSmallWaves = 8;
 constexpr int64_t kSmallWeights = 1 << 18;  // every workgroup reads all of W: up to half a megabyte
@@ -1025,9 +1040,10 @@ __global__ __launch_bounds__(256) void relu_dz_kernel(const T *__restrict__ dy, 
     }
 }
 
-// W [N,K] -> W^T [K,N]: the operand of dx = dz W with its summed axis contiguous (768 x 513 fp16: 5 us).
+// W [N,K] -> W^T [K,N], `parts` times side by side: the operand of dx = dz W with its summed axis contiguous (768 x 513 fp16:
+// 5 us).
 template <typename T>
-__global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w, T *__restrict__ wt, int N, int K) {
+__global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w, T *__restrict__ wt, int N, int K, int parts) {
     __shared__ T t[32][33];
     const int k0 = blockIdx.x * 32, n0 = blockIdx.y * 32;
     const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
@@ -1035,15 +1051,16 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T *__restrict__ w,
         if (n0 + i < N && k0 + c < K) t[i][c] = w[(int64_t)(n0 + i) * K + k0 + c];
     __syncthreads();
     for (int i = r; i < 32; i += 8)
-        if (k0 + i < K && n0 + c < N) wt[(int64_t)(k0 + i) * N + n0 + c] = t[c][i];
+        if (k0 + i < K && n0 + c < N)
+            for (int p = 0; p < parts; ++p) wt[((int64_t)(k0 + i) * parts + p) * N + n0 + c] = t[c][i];
 }
 
 struct DwArgs {
     const void *dz, *x;
     float *part_w, *part_b;  // [slices][N*K], [slices][N]; each may be null
-    void *dw, *db;           // one slice: the outputs themselves, in place of the partial sums
+    void *dw, *db;           // where `direct`: the outputs themselves, in place of the partial sums
     int64_t rows, dzp, xp, slice_rows;
-    int K, N, slices;
+    int K, N, slices, direct;
 };
 
 // dW tile over one slice of the rows: WN x WK waves (four) of 64 columns of dz x 64 columns of x.  Slabs of 64 (fp32: 32)
@@ -1176,11 +1193,11 @@ __global__ __launch_bounds__(256, 2) void linear_dw_kernel(DwArgs a) {
                 for (int j = 0; j < 4; ++j) {
                     const int k = k0 + wk + j * 16 + li;
                     if (k >= a.K) continue;
-                    if (a.slices == 1) ((T *)a.dw)[(int64_t)n * a.K + k] = (T)acc[i][j][q];
+                    if (a.direct) ((T *)a.dw)[(int64_t)n * a.K + k] = (T)acc[i][j][q];
                     else pw[(int64_t)n * a.K + k] = acc[i][j][q];
                 }
             if (want_b && li == 0) {
-                if (a.slices == 1) ((T *)a.db)[n] = (T)accb[i][q];
+                if (a.direct) ((T *)a.db)[n] = (T)accb[i][q];
                 else a.part_b[(int64_t)slice * a.N + n] = accb[i][q];
             }
         }
@@ -1390,14 +1407,14 @@ int launch_dw(const DwArgs &d, const DwShape &p, hipStream_t s) {
 // and rows under way fit 256 registers with something left for the work on them.
 struct BwdRowsPlan {
     int kc, ng, bytes, blocks;  // kc == 0: the layer is too wide
-    bool fine;  // dz as two values, half width: where a gradient has a thousand values or fewer, in which one rounding of dz shows
-                // beside the gradient's own; over more it averages to two fifths (bf16 gelu, with / without: 640 000 rows, 32 -> 32
-                // 46/40 us, 37 560 rows, 8 -> 2 7.8/7.5)
+    bool fine;  // dz as two values (FINE)
 };
-constexpr int64_t kFineValues = 1024;
 
-template <typename T>
-constexpr bool bwd_rows_fine(int kc, int ng) { return sizeof(T) == 2 && (kc == 1 || ng == 2); }
+// gelu and silu in half width: dz is no number of the type.  (none and relu: it is dy's, or zero.)  Rounded to one it would add
+// two fifths to the error of the gradients' own rounding (128 -> 128 bf16: 2.35e-3 against 1.66e-3), so its products take two
+// values of it: 640 000 rows, 128 -> 128 bf16 gelu, forward and backward, 324 us against 266; 64 -> 64 87 against 69 (backward);
+// 100 003 rows, 513 -> 768 fp16 gelu 980 against 640 (backward).
+bool two_values(int act, size_t e) { return e == 2 && (act == FSGS_ACT_GELU || act == FSGS_ACT_SILU); }
 
 template <typename T>
 constexpr bool bwd_rows_fits(int kc, int ng) {
@@ -1406,24 +1423,23 @@ constexpr bool bwd_rows_fits(int kc, int ng) {
 }
 
 template <typename T>
-BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N) {
+BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N, int act) {
     BwdRowsPlan p = {};
     const int row = K * (int)sizeof(T);
     if (row > 512 || N > 256) return p;
     const int kc = row <= 64 ? 1 : row <= 128 ? 2 : row <= 256 ? 4 : 8, ng = (N + 63) / 64 * 2;
     const BwdRowsLds<T> lay(kc, N);
-    p.bytes = lay.bytes;
+    p.fine = two_values(act, sizeof(T));
+    p.bytes = p.fine ? lay.fine_bytes : lay.bytes;
     if (!bwd_rows_fits<T>(kc, ng) || p.bytes > 160 * 1024) return p;
     p.kc = kc, p.ng = ng;
-    p.fine = bwd_rows_fine<T>(kc, ng) && min(rows, (int64_t)N) * K <= kFineValues && lay.fine_bytes <= 160 * 1024;
-    if (p.fine) p.bytes = lay.fine_bytes;
     const int64_t want = (rows + kBwdRows - 1) / kBwdRows;
     p.blocks = (int)(want < 256 ? want : 256);
     return p;
 }
 
-BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N, size_t e) {
-    return e == 4 ? bwd_rows_plan<float>(rows, K, N) : bwd_rows_plan<__bf16>(rows, K, N);
+BwdRowsPlan bwd_rows_plan(int64_t rows, int K, int N, int act, size_t e) {
+    return e == 4 ? bwd_rows_plan<float>(rows, K, N, act) : bwd_rows_plan<__bf16>(rows, K, N, act);
 }
 
 template <typename T, int KC, int NG, bool FINE>
@@ -1437,9 +1453,8 @@ int launch_bwd_rows_as(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s
 template <typename T, int KC, int NG>
 int launch_bwd_rows(const BwdRowsArgs &a, const BwdRowsPlan &p, hipStream_t s) {
     if constexpr (bwd_rows_fits<T>(KC, NG)) {
-        if constexpr (bwd_rows_fine<T>(KC, NG))
-            if (p.fine && (a.act == FSGS_ACT_GELU || a.act == FSGS_ACT_SILU))  // (the others' dz is dy or zero: exact)
-                return launch_bwd_rows_as<T, KC, NG, true>(a, p, s);
+        if constexpr (sizeof(T) == 2)
+            if (p.fine) return launch_bwd_rows_as<T, KC, NG, true>(a, p, s);
         return launch_bwd_rows_as<T, KC, NG, false>(a, p, s);
     } else {
         return FSGS_EINVAL;
@@ -1483,18 +1498,19 @@ int64_t most_sum_rows(int64_t rows, int N) {
 BwdScratch bwd_layout(int64_t rows, int K, int N, size_t e, int act, bool dx, bool dw, bool db) {
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     BwdScratch l;
-    const BwdRowsPlan p = bwd_rows_plan(rows, K, N, e);
+    const BwdRowsPlan p = bwd_rows_plan(rows, K, N, act, e);
     if (p.kc) {
         l.dz = l.wt = l.part_w = 0, l.sums = p.blocks;
         l.part_b = dw ? up((size_t)p.blocks * K * N * 4) : 0;
         l.total = l.part_b + (db ? up((size_t)p.blocks * N * 4) : 0);
         return l;
     }
-    const size_t s = (size_t)dw_shape(rows, K, N, dw).slices;
+    const int cols = two_values(act, e) ? 2 * N : N;  // of dz
+    const size_t s = (size_t)dw_shape(rows, K, cols, dw).slices;
     l.dz = 0;
-    l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * N * e) : 0);
-    l.part_w = l.wt + (dx ? up((size_t)K * N * e) : 0);
-    l.part_b = l.part_w + (dw ? up(s * (size_t)K * N * 4) : 0);
+    l.wt = l.dz + (act != FSGS_ACT_NONE ? up((size_t)rows * cols * e) : 0);
+    l.part_w = l.wt + (dx ? up((size_t)K * cols * e) : 0);
+    l.part_b = l.part_w + (dw ? up(s * (size_t)K * cols * 4) : 0);
     l.sums = act != FSGS_ACT_NONE ? max(most_sum_rows(rows, N), (int64_t)s) : (int64_t)s;
     l.total = l.part_b + (db ? up((size_t)l.sums * (size_t)N * 4) : 0);
     return l;
@@ -1511,7 +1527,7 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
             linear_bwd_small_kernel<T><<<blocks, 64 * kSmallWaves, 0, s>>>(b);
             return check_launch();
         }
-    const BwdRowsPlan p = bwd_rows_plan<T>(a.rows, a.K, a.N);
+    const BwdRowsPlan p = bwd_rows_plan<T>(a.rows, a.K, a.N, a.act);
     if (p.kc) {
         BwdRowsArgs b = {};
         b.x = a.x, b.xp = a.xp, b.w = a.w, b.bias = a.bias, b.dy = a.dy, b.dyp = a.dyp, b.dx = dx;
@@ -1523,6 +1539,8 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         if (rc != FSGS_OK || (!dw && !db)) return rc;
         return launch_reduce<T>(b.part_w, (int64_t)a.N * a.K, dw, b.part_b, a.N, db, p.blocks, s);
     }
+    // dz as two values: [rows, 2N], so that dx sums over twice the columns, against W twice, and dW's second half adds to its first
+    const int parts = two_values(a.act, sizeof(T)) ? 2 : 1, cols = parts * a.N;
     const void *dz = a.dy;
     int64_t dzp = a.dyp;
     float *part_w = dw ? (float *)(scratch + l.part_w) : nullptr, *part_b = db ? (float *)(scratch + l.part_b) : nullptr;
@@ -1540,23 +1558,23 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
     } else if (a.act != FSGS_ACT_NONE) {
         // (the sums of db are taken here, before dz is rounded to T)
         LinArgs z = a;
-        z.y = scratch + l.dz, z.yp = a.N, z.part_b = part_b;
+        z.y = scratch + l.dz, z.yp = cols, z.part_b = part_b, z.lo = cols - a.N;
         const int kind = product_kind<T, kModeDz>(z);
         if (part_b && sum_rows_of(kind, a.rows) > l.sums) return FSGS_ESCRATCH;
         rc = launch_product<T, kModeDz>(z, kind, s);
         if (rc != FSGS_OK) return rc;
-        dz = z.y, dzp = a.N, sum_rows = (int)sum_rows_of(kind, a.rows);
+        dz = z.y, dzp = cols, sum_rows = (int)sum_rows_of(kind, a.rows);
     }
     if (dx) {
         LinArgs g = {};
-        g.x = dz, g.xp = dzp, g.y = dx, g.yp = a.K, g.rows = a.rows, g.K = a.N, g.N = a.K;
+        g.x = dz, g.xp = dzp, g.y = dx, g.yp = a.K, g.rows = a.rows, g.K = cols, g.N = a.K;
         const int kind = product_kind<T, kModeFwd>(g);
         if (kind == kByRows) {
             g.w = a.w;
-            rc = launch_rows<T, kModeFwd>(g, 1, s);
+            rc = launch_rows<T, kModeFwd>(g, a.N, s);
         } else {
             T *wt = (T *)(scratch + l.wt);
-            transpose_kernel<T><<<dim3((a.K + 31) / 32, (a.N + 31) / 32), 256, 0, s>>>((const T *)a.w, wt, a.N, a.K);
+            transpose_kernel<T><<<dim3((a.K + 31) / 32, (a.N + 31) / 32), 256, 0, s>>>((const T *)a.w, wt, a.N, a.K, parts);
             rc = check_launch();
             if (rc != FSGS_OK) return rc;
             g.w = wt;
@@ -1565,11 +1583,11 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         if (rc != FSGS_OK) return rc;
     }
     if (!dw && !db) return FSGS_OK;
-    const DwShape shape = dw_shape(a.rows, a.K, a.N, dw);
-    const int slices = (int)shape.slices;
+    const DwShape shape = dw_shape(a.rows, a.K, cols, dw);
+    const int slices = (int)shape.slices, sums = slices * parts;
     if (dw || !sum_rows) {
         DwArgs d = {};
-        d.dz = dz, d.dzp = dzp, d.x = a.x, d.xp = a.xp, d.rows = a.rows, d.K = a.K, d.N = a.N, d.slices = slices;
+        d.dz = dz, d.dzp = dzp, d.x = a.x, d.xp = a.xp, d.rows = a.rows, d.K = a.K, d.N = cols, d.slices = slices, d.direct = sums == 1;
         d.part_w = part_w, d.part_b = sum_rows ? nullptr : part_b, d.dw = dw, d.db = db;
         d.slice_rows = ((a.rows + slices - 1) / slices + 63) / 64 * 64;
         rc = launch_dw<T>(d, shape, s);
@@ -1581,8 +1599,8 @@ int run_bwd(LinArgs a, const void *y, void *dx, void *dw, void *db, char *scratc
         if (rc != FSGS_OK) return rc;
         db = nullptr;
     }
-    if (slices == 1 || (!dw && !db)) return FSGS_OK;
-    return launch_reduce<T>(part_w, nk, dw, part_b, a.N, db, slices, s);
+    if (sums == 1 || (!dw && !db)) return FSGS_OK;
+    return launch_reduce<T>(part_w, nk, dw, part_b, a.N, db, sums, s);
 }
 
 bool bad_sizes(int64_t rows, int K, int N, int dtype, int act) {
@@ -1614,7 +1632,7 @@ extern "C" int fsgs_linear_fwd(int64_t rows, int in_dim, int out_dim, int dtype,
 extern "C" int fsgs_linear_bwd_uses_output(int64_t rows, int in_dim, int out_dim, int dtype, int act) {
     if (bad_sizes(rows, in_dim, out_dim, dtype, act)) return FSGS_EINVAL;
     const size_t e = dtype == FSGS_F32 ? 4 : 2;
-    return act == FSGS_ACT_RELU && bwd_rows_plan(rows, in_dim, out_dim, e).kc == 0 && !small_bwd(rows, in_dim, out_dim, e);
+    return act == FSGS_ACT_RELU && bwd_rows_plan(rows, in_dim, out_dim, act, e).kc == 0 && !small_bwd(rows, in_dim, out_dim, e);
 }
 
 extern "C" int64_t fsgs_linear_bwd_scratch_bytes(int64_t rows, int in_dim, int out_dim, int dtype, int act, int want_dx,

@@ -1922,9 +1922,9 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     float16) on one device; products in that type, sums in float32, one rounding at the end.  ``act`` is "none", "relu",
     "gelu" (the erf form) or "silu".  Rows of ``x`` and ``residual`` may lie at any pitch (slices of a wider plane are read in
     place).  Differentiable in all four tensors, once; the backward forms the pre-activation again from ``x``.  In the
-    half-width types the gradient of the pre-activation is rounded to that type before its two products (the rounding an
-    unfused layer makes when it stores that gradient), except where that one rounding could be most of the error: 512 values
-    of it and 2^18 weights at most, or 128 inputs and a thousand values of ``x``'s or the weight's gradient at most.  A relu
+    half-width types the gradient of the pre-activation, no number of the type behind gelu and silu, enters its two products as the
+    sum of two values of the type (16 bits in bf16, 22 in fp16 down to an absolute 2^-25), for 512 values of it and 2^18 weights
+    at most in fp32.  A relu
     output that is positive but rounds to zero is -0: a wide relu layer takes its slope from the output's bits."""
     _require_float(x, "x")
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):

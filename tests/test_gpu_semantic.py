@@ -200,7 +200,7 @@ def test_linear_activation_over_its_range(dev, dtype, act):
 
     gelu's tail h = P(t) exp(-z^2/2) is off by its fit, 1.3e-9, and relatively by the exponent's rounding, z^2 / 2 times two
     roundings, and by 32 U32 for P (seven steps, magnitudes 2.7 times the sum), the reciprocal and the exponential; bf16's form by
-    1e-4.  y = max(z, 0) - |z| h; the slope is h - |z| phi, or one minus that.  silu's sigma is off by (2 |z| + 8) U32 of itself.
+    1e-4, fp16's by 5.6e-6 and 32 U32 for |z| <= 6 (Q's terms sum to 44 there: 22 U32 of Q, less of h) and by 2^-26 beyond.  y = max(z, 0) - |z| h; the slope is h - |z| phi, or one minus that.  silu's sigma is off by (2 |z| + 8) U32 of itself.
     The type's rounding comes last; dz enters its product as two values of a half-width type."""
     z = torch.linspace(-14, 14, 100000).to(dtype)
     x = z[:, None].to(dev).requires_grad_(True)
@@ -212,7 +212,10 @@ def test_linear_activation_over_its_range(dev, dtype, act):
         h, phi = 0.5 * torch.erfc(size / math.sqrt(2)), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
         rel = (z * z + 32) * S.U32
         # (the exponential instruction gives zero for what lies below 2^-126, bf16's tail from |z| = 13.1 on: off by that at most)
-        ey = size * (1e-4 * h + 2.0 ** -126 if dtype == torch.bfloat16 else 1.3e-9 + rel * h)
+        ey = size * {torch.float32: 1.3e-9 + rel * h, torch.bfloat16: 1e-4 * h + 2.0 ** -126,
+                     torch.float16: (5.6e-6 + 32 * S.U32) * h}[dtype]
+        if dtype == torch.float16:
+            ey = ey + 2.0 ** -26 * (size > 6)
         es = 1.3e-9 + rel * (h + size * phi) + 2 * S.U32
         low = 0.5 * torch.erfc(-z / math.sqrt(2))  # (1 + erf, as S has it, is 2e-16 off: all of the value at z = -9)
         vy, vs = z * low, low + z * phi
@@ -377,6 +380,58 @@ def test_linear_few_gradient_values(dev, size, dtype, act):
         # (what the second value leaves: half a step of a number that is half a step of dz at most, or a least subnormal)
         e = e + u * u * left[n] + S.TINY[dtype] * (x.abs().sum(0).cpu().double() if n == "dw" else w.abs().sum(0).cpu().double())
         S.check(g[k], (v, e + u * (v.abs() + e) + S.TINY[dtype]), f"{size} {act} {n}")
+
+
+def _check_two_values(size, x, w, b, act, dy, what):
+    """dx, dW and db of a half-width layer whose dz goes into its products as two values of the type: half a step of their own,
+    half a step of half a step of dz, and the fp32 sums."""
+    _, g = _check_layer(x, w, b, None, act, dy, what)
+    want = S.linear(x.float(), w.float(), b.float(), None, act, dy.float())
+    u = S.U[x.dtype]
+    dz = (dy.double() * S.slope(x.double() @ w.double().t() + b.double(), act)).abs().cpu()
+    left = {"dx": dz @ w.cpu().double().abs(), "dw": dz.t() @ x.cpu().double().abs(), "db": 0.0}
+    tiny = {"dw": x.abs().sum(0).cpu().double(), "dx": w.abs().sum(0).cpu().double(), "db": 0.0}
+    for k, n in (("x", "dx"), ("w", "dw"), ("b", "db")):
+        v, e = want[n]
+        # (what the second value leaves: half a step of a number that is half a step of dz at most, or a least subnormal; twice
+        # as many terms, so twice the fp32 sums' part)
+        e = 2 * e + u * u * left[n] + S.TINY[x.dtype] * tiny[n]
+        S.check(g[k], (v, e + u * (v.abs() + e) + S.TINY[x.dtype]), f"{what} {n}")
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("size", [(5000, 64, 128), (3000, 128, 128), (4097, 33, 190), (2000, 16, 224), (600, 100, 64), (130, 128, 65),
+                                  (1000, 7, 129), (2500, 64, 160), (127, 40, 100)], ids=lambda s: "x".join(map(str, s)))
+def test_linear_thin_gradients_keep_dz(dev, size, dtype, act):
+    x, w, b, r, dy = _layer(dev, *size, dtype, res=False, seed=140 + size[0])
+    _check_two_values(size, x, w, b, act, dy, f"{size} {act}")
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("size", DZ[2:] + [(7000, 200, 50), (300, 256, 64), (129, 64, 257), (16, 300, 200), (1, 300, 1000), (513, 130, 33),
+                                           (70000, 32, 256), (20000, 136, 17)], ids=lambda s: "x".join(map(str, s)))
+def test_linear_wide_gradients_keep_dz(dev, size, dtype, act):
+    """... of wider layers: every kernel that forms dz or takes it, one slice of the rows and several."""
+    x, w, b, r, dy = _layer(dev, *size, dtype, res=False, seed=160 + size[0])
+    _check_two_values(size, x, w, b, act, dy, f"{size} {act}")
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("size", [(700, 64, 128), (300, 128, 40), (500, 300, 70)], ids=lambda s: "x".join(map(str, s)))
+def test_linear_largest_fp16_gradients(dev, size, act):
+    """dz beyond fp16's largest number (60 000 times a slope of 1.13): finite gradients stay finite, infinite ones do not."""
+    x, w, b, r, dy = _layer(dev, *size, torch.float16, res=False, seed=150)
+    x, w, b = x * 2.0 ** -9, w * 2.0 ** -4, b * 0 + 1.4  # (z = 1.4: slopes of 1.13 and 1.03)
+    sign = _randn(dev, 1, size[2], seed=151).sign() * torch.where(torch.arange(size[0], device=dev) % 2 == 0, 1.0, -1.0)[:, None]
+    dy = (60000.0 * sign).to(torch.float16)  # (signs alternate down a column: the sums stay in range)
+    _check_two_values(size, x, w, b, act, dy, f"{size} {act}")
+    dy[3, 5] = math.inf
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops.linear_act(*leaves, act), leaves, dy)
+    assert not torch.isfinite(dx[3]).any() and torch.isfinite(dx[:3]).all() and torch.isfinite(dx[4:]).all()
+    assert not torch.isfinite(dw[5]).any() and not torch.isfinite(db[5]) and torch.isfinite(dw[:5]).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)

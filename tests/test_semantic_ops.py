@@ -136,12 +136,14 @@ def test_semantic_head_refuses(kw):
         SemanticHead(**args)
 
 
-def _coefficients(function):
+def _coefficients(function, branch=None):
     import os
     import re
     src = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "linear.hip")).read()
     body = src[src.index(f"float {function}(") :]
     body = body[:body.index("\n}")]
+    if branch is not None:
+        body = body.split("} else {")[branch]
     first, rest = re.search(r"fmaf\(([-\d.e]+)f, [ta], ([-\d.e]+)f\)", body), re.findall(r"fmaf\([pq], [ta], ([-\d.e]+)f\)", body)
     scale = re.search(r"fmaf\(([\d.]+)f, fabsf", body)
     f32 = lambda v: float(torch.tensor(float(v), dtype=torch.float32))  # noqa: E731
@@ -159,13 +161,21 @@ def test_gelu_tails_are_as_close_as_their_comments_say():
     for v in c:
         p = p * t + v
     assert (p * t * e - h).abs().max() < 1.3e-9
-    c, _ = _coefficients("normal_tail_bf16")
-    assert len(c) == 10
-    q = torch.zeros_like(z)
-    for v in c:
-        q = q * z + v
-    rel = (torch.exp2(q) / h - 1).abs()
-    assert rel[z < 1].max() < 5e-6 and rel[z < 2].max() < 3.1e-5 and rel.max() < 1e-4
+    for branch, degree in ((0, 9), (1, 7)):
+        c, _ = _coefficients("normal_tail_half", branch)
+        assert len(c) == degree + 1
+        q = torch.zeros_like(z)
+        for v in c:
+            q = q * z + v
+        rel = (torch.exp2(q) / h - 1).abs()
+        if degree == 9:
+            assert rel[z < 1].max() < 5e-6 and rel[z < 2].max() < 3.1e-5 and rel.max() < 1e-4
+        else:
+            assert rel[z <= 6].max() < 5.6e-6 and (z * torch.exp2(q))[z > 6].max() < 2.0 ** -26
+        far, q = torch.logspace(1.2, 38, 4000, dtype=torch.float64), 0.0
+        for v in c:
+            q = q * far + v
+        assert (q < -120).all()
 
 
 def test_semantic_head_parameters():
