@@ -16,6 +16,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, load, ptr, stream_ptr
@@ -1810,6 +1811,16 @@ def _run_on(dev: torch.device, fn, args, what: str) -> None:
             _run(fn, args, what)
 
 
+def _tracked(*tensors: Optional[Tensor]) -> bool:
+    """Whether a call on these tensors has to go through autograd: one of them records a graph, or carries a forward-mode tangent,
+    which an autograd function refuses where a plain call would lose it."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
     """``t`` [..., width] -> (tensor whose storage the kernels read, elements between two rows).  A tensor whose rows lie at
     one pitch (a slice of a wider plane, an expanded row) is read in place, any other is copied once."""
@@ -1945,8 +1956,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     if act not in ACTIVATIONS:
         raise ValueError(f"act must be one of {tuple(ACTIVATIONS)}, got {act!r}")
     weight, bias = weight.contiguous(), _c(bias)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if _tracked(x, weight, bias, residual):
         return _LinearAct.apply(x, weight, bias, residual, ACTIVATIONS[act])
     return _linear_fwd(x, weight, bias, residual, ACTIVATIONS[act])
 
@@ -2043,4 +2053,4 @@ def topk_distill(logits: Tensor, teacher_idx: Tensor, teacher_logits: Tensor, te
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(REDUCTIONS)}, got {reduction!r}")
     args = logits, teacher_idx, teacher_logits, weight, temperature, REDUCTIONS[reduction]
-    return _TopkDistill.apply(*args) if torch.is_grad_enabled() and logits.requires_grad else _distill_fwd(*args, False)[0]
+    return _TopkDistill.apply(*args) if _tracked(logits, teacher_logits, weight) else _distill_fwd(*args, False)[0]

@@ -859,6 +859,26 @@ def test_distill_offsets_beyond_32_bits(dev):
 
 
 # ---- both together --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(dev, grad):
+    """A tangent is refused, never lost."""
+    from torch.autograd import forward_ad
+    x, w, b, r, _ = _layer(dev, 6, 8, 5, torch.float32)
+    logits, idx, top = _record(dev, 6, 8, 3, torch.float32, ragged=False)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        for i in range(4):
+            args = [x, w, b, "gelu", r]
+            i += i == 3
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError):
+                ops.linear_act(*args)
+        with pytest.raises(NotImplementedError):
+            losses.topk_distill_loss(forward_ad.make_dual(logits, torch.ones_like(logits)), idx, top)
+        with pytest.raises(NotImplementedError):
+            losses.topk_distill_loss(logits, idx, forward_ad.make_dual(top, torch.ones_like(top)))
+        ops.linear_act(x, w, b, "gelu", r), losses.topk_distill_loss(logits, idx, top)
+
+
 def _step(head, feats, idx, top, weight):
     logits = head(feats)
     loss = losses.topk_distill_loss(logits, idx, top, 2.0, weight)

@@ -40,6 +40,19 @@ def test_topk_distill_loss_refuses_what_has_no_gpu_tensor():
         losses.topk_distill_loss(torch.zeros(2, 3), torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2, 1))
 
 
+def test_forward_mode_tangents_go_through_autograd():
+    from torch.autograd import forward_ad
+    t = torch.ones(3)
+    assert not ops._tracked(t, None) and ops._tracked(None, torch.ones(3, requires_grad=True))
+    with torch.no_grad():
+        assert not ops._tracked(torch.ones(3, requires_grad=True))
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(t, t)
+        assert not ops._tracked(t, None) and ops._tracked(t, None, d)
+        with torch.no_grad():
+            assert ops._tracked(d)
+
+
 # The C entries check sizes, codes and pointers before any launch: every call below returns without touching the GPU.
 ONE = C.c_void_p(256)  # (never dereferenced: each of these calls is refused)
 
