@@ -164,9 +164,10 @@ __device__ __forceinline__ int group_column(int t, int r) {
     return sizeof(T) == 2 ? (r >> 2) * 8 + t * 4 + (r & 3) : t * 16 + r;
 }
 
-// The first n (at least one) elements of a chunk.  The two branches end apart (two empty instructions that differ): their stores
-// are the same instructions at other places, and the compiler, left to join them, has given lanes of the one the values of the
-// other.
+// The first n (at least one) elements of a chunk.  The two branches end apart (two empty instructions that differ).  Left to join
+// them, the compiler gave both one last store, `n == 3 ? element 2 : element 3` of an fp32 chunk, and moved element 2 into the
+// register of element 3 for every lane where the branches meet, before the lanes of whole chunks had stored theirs (read in the
+// assembly of the store to LDS: v_mov_b32 v19, v18 behind s_or_b64 exec, then ds_write_b32 of v19 in either branch).
 template <typename T>
 __device__ __forceinline__ void put_chunk(T *to, const Chunk &c, int n, bool stream) {
     if (n >= kChunk<T>) {
