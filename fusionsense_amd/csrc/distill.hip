@@ -408,6 +408,7 @@ __global__ __launch_bounds__(256, 5) void distill_bwd_kernel(DistillArgs a) {
         if (__any(x.far || dead)) put([&](float v) { return dead ? -INFINITY : x.of(v); });
         else put([&](float v) { return fmaf(v, x.scale2, -x.shift); });
         bool again = false;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (another lane may have cleared the word)
         auto mark = [&](int ck) { again |= (atomicOr(&bits[ck >> 5], 1u << (ck & 31)) >> (ck & 31)) & 1u; };
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
