@@ -965,6 +965,49 @@ def test_head_and_loss_captured_and_on_another_stream(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("act", ["gelu", "relu"])
+@pytest.mark.parametrize("R", [5, 700])
+def test_wide_head_and_loss_captured_and_on_two_streams(dev, dtype, act, R):
+    """A head too wide for the one-pass backward, few points and many: a captured step replayed with eager work between, and two
+    steps at once on two streams, give the eager step's bits."""
+    head = SemanticHead(40, 2700, hidden=600, blocks=1, act=act, dtype=dtype, device=dev,
+                        generator=torch.Generator().manual_seed(1))
+
+    def data(seed):
+        feats = _randn(dev, R, 40, seed=seed, dtype=dtype).requires_grad_(True)
+        _, idx, top = _record(dev, R, 2700, 8, torch.float32, torch.float16, seed=seed)
+        return feats, idx, top, torch.rand(R, generator=torch.Generator().manual_seed(seed)).to(dev)
+    sets, want = [data(1), data(2)], []
+    for a in sets:
+        loss, grads = _step(head, *a)
+        want.append([loss.detach().clone()] + [g.clone() for g in grads])
+        del loss, grads
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for _ in range(3):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                loss, grads = _step(head, *sets[i])
+                got[i] = [loss.detach()] + list(grads)
+                del loss, grads
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            assert all(torch.equal(x, y) for x, y in zip(got[i], want[i]))
+    del got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grads = _step(head, *sets[0])
+        out = [loss.detach()] + list(grads)
+    del loss, grads
+    for _ in range(3):
+        for t in out:
+            t.fill_(7.0)
+        graph.replay()
+        (sets[0][0].detach() * 2).sum().item()
+        assert all(torch.equal(x, y) for x, y in zip(out, want[0]))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_head_and_loss_with_saved_tensors_kept_on_the_host(dev, dtype):
     """What the backward needs may come back in other storage and with other strides: the same bits."""
     head = SemanticHead(32, 150, hidden=64, dtype=dtype, device=dev, generator=torch.Generator().manual_seed(0))
