@@ -169,9 +169,9 @@ struct RowExp {
 };
 
 // L lanes per row, the row in their registers (a row that fills a workgroup: step by step, the next step's loads under way).
-// Bound by memory up to some thousand classes: 640 000 x 150 fp32 with K = 16 96 us, 445 MB at 4.6 TB/s; 230 400 x 1203 bf16 with
-// K = 32 147 us, 630 MB at 4.3.  4099 x 32 003 fp16 85 us, 262 MB at 3.1 TB/s: four steps a row beside its joins; more workgroups
-// a CU would spill (5: 120 us, 6: 150).  2 073 600 x 21 bf16 with K = 4 50 us: a lane per row, by its entries' dependent loads.
+// Bound by memory up to some thousand classes: 640 000 x 150 fp32 with K = 16 102 us, 445 MB at 4.4 TB/s; 230 400 x 1203 bf16 with
+// K = 32 155 us, 630 MB at 4.1.  4099 x 32 003 fp16 95 us, 262 MB at 2.8 TB/s: four steps a row beside its joins; more workgroups
+// a CU would spill (5: 120 us, 6: 150).  2 073 600 x 21 bf16 with K = 4 51 us: a lane per row, by its entries' dependent loads.
 template <typename T, int L, int STEPS>
 __global__ __launch_bounds__(256, L == kWideRow ? 4 : 6) void distill_fwd_kernel(DistillArgs a) {
     constexpr int CE = kChunk<T>, ROWS = 256 / L, kHeld = kHeldOf<STEPS>;
@@ -330,7 +330,7 @@ struct BwdLds {
     }
 };
 
-// Bound by memory: 640 000 x 150 fp32 160 us, 845 MB at 5.3 TB/s; 230 400 x 1203 bf16 282 us, 1.19 GB at 4.2 TB/s.
+// Bound by memory: 640 000 x 150 fp32 162 us, 845 MB at 5.2 TB/s; 230 400 x 1203 bf16 297 us, 1.19 GB at 4.0 TB/s.
 // A wave's rows (64 / L of them, neighbours in the gradient) are put together in LDS and leave it as aligned 16-byte
 // streaming stores: rows start at any element, and the line that two stores share would otherwise be written twice.  q of every
 // class goes first, then the teacher's classes once more with their mass taken off.  A class may stand in several entries: its
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(256, 5) void distill_bwd_kernel(DistillArgs a) {
 
 // One row per workgroup, too long for a float per class in LDS: q for every class first, then the teacher's classes once more
 // with their mass taken off.  One bit per class finds a class that stands in several entries.  Bound by memory:
-// 4099 x 32 003 fp16 102 us, 525 MB at 5.1 TB/s.
+// 4099 x 32 003 fp16 103 us, 525 MB at 5.1 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void distill_bwd_wide_kernel(DistillArgs a) {
     constexpr int CE = kChunk<T>, L = kWideRow;

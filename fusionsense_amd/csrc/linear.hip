@@ -475,8 +475,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(LinArgs a) {
 //   kStoreStream  past the caches; rows must start at 64-byte boundaries, which a store instruction then covers whole
 //   kStoreTile    the wave's 16 rows (neighbours in y) are put together in LDS and leave it as aligned streaming stores
 // Bound by memory where the activation is cheap (921 600 rows, 64 -> 64 fp32, silu and a residual: 139 us, 708 MB at 5.1 TB/s;
-// a 4 GiB copy reaches 4.8), by gelu's vector instructions at 640 000 rows, 64 -> 128 bf16 (61 us, 48 without it), and with
-// fp32 class scores (640 000 rows, 32 -> 150: 127 us, 466 MB at 3.7 TB/s) by what overlaps between twelve waves a CU.
+// a 4 GiB copy reaches 4.8), by gelu's vector instructions at 640 000 rows, 64 -> 128 bf16 (60 us, 48 without it), and with
+// fp32 class scores (640 000 rows, 32 -> 150: 130 us, 466 MB at 3.6 TB/s) by what overlaps between twelve waves a CU.
 enum { kStorePlain = 0, kStoreStream = 1, kStoreTile = 2 };
 
 struct RowsArgs {
@@ -646,10 +646,12 @@ __global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(Row
 // operand of dx^T = W^T dz^T, and through LDS it meets x again in dW = dz^T x, whose whole [N,K] lies in the workgroup's
 // registers for the life of the workgroup.  x and dy are read once, dx is written once; W is held once, read along its rows for
 // z and along its columns for dx.
-// 640 000 rows: fp32 32 -> 150 187 us (its three products alone 120 at the rate of a large fp32 product, its bytes 110), bf16
-// 128 -> 128 with gelu 164 us (bytes 98).  Bound by what two waves a SIMD overlap: dW's registers leave no room for more, and
-// the waves meet twice per 128 rows.  (The two layers' training calls went from 0.92 to 0.38 and from 0.71 to 0.36 ms when this
-// kernel took the place of one each for dz, dx and dW.)
+// 640 000 rows: fp32 32 -> 150 201 us (its three products alone 120 at the rate of a large fp32 product, its bytes 110), bf16
+// 128 -> 128 with gelu 257 us (bytes 98; 174 with dz rounded to one value).  Bound by what two waves a SIMD overlap: one workgroup
+// a CU, whose waves meet twice per 128 rows.  LDS holds no second one (126 and 148 KB, of which dz 84 and 74), and a wave takes
+// 230 to 256 registers for the rows of x and dy under way, dz, dx and db (dW's tiles are 12 and 32 of them).  (The two layers'
+// training calls went from 0.92 to 0.38 and, with dz rounded, from 0.71 to 0.36 ms when this kernel took the place of one each
+// for dz, dx and dW.)
 struct BwdRowsArgs {
     const void *x, *w, *bias, *dy;
     void *dx;
@@ -915,8 +917,9 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
 }
 
 // ---- backward of a few rows and outputs, half width: one launch ------------------------------------------------------------
-// Every workgroup forms all of dz (rows x N) by itself in fp32 LDS and takes 32 columns of dW and dx.  Bound by latency: 16 rows, 64 -> 20 bf16 6.4 us; one row,
-// 64 -> 150 10.8, where four rows take 15 in the one-pass kernel and its sum over slices; one row, 512 -> 512 43.
+// Every workgroup forms all of dz (rows x N) by itself in fp32 LDS and takes 32 columns of dW and dx.  Bound by latency: 16 rows, 64 -> 20
+// bf16 gelu 6.5 us; one row, 64 -> 150 11.4, where four rows take 18 in the one-pass kernel and its sum over slices; one row,
+// 512 -> 512 48.
 constexpr int kSmallDz = 512, kSmallCols = 32, kSmallWaves = 8;
 constexpr int64_t kSmallWeights = 1 << 18;  // every workgroup reads all of W: up to half a megabyte
 
@@ -1414,7 +1417,7 @@ struct BwdRowsPlan {
 // gelu and silu in half width: dz is no number of the type.  (none and relu: it is dy's, or zero.)  Rounded to one it would add
 // two fifths to the error of the gradients' own rounding (128 -> 128 bf16: 2.35e-3 against 1.66e-3), so its products take two
 // values of it: 640 000 rows, 128 -> 128 bf16 gelu, forward and backward, 324 us against 266; 64 -> 64 87 against 69 (backward);
-// 100 003 rows, 513 -> 768 fp16 gelu 980 against 640 (backward).
+// 100 003 rows, 513 -> 768 fp16 gelu 980 against 640 (backward: dz 317, dx 258, dW 370).
 bool two_values(int act, size_t e) { return e == 2 && (act == FSGS_ACT_GELU || act == FSGS_ACT_SILU); }
 
 template <typename T>

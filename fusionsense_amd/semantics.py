@@ -4,7 +4,10 @@ The reference's active-touch module names an object's parts, segments views of i
 the high-gradient points (scripts/VLM.py:55-385); its Gaussians carry no labels.  Here every Gaussian carries a feature row
 ``gauss_params["semantics"]`` [N,D]; :func:`fusionsense_amd.fusion.render_fusionsense` composites it to a plane like a colour
 and hands that plane to a :class:`SemanticHead`; :func:`fusionsense_amd.losses.topk_distill_loss` trains both against what was
-kept of a 2-D teacher's scores.  The same head on the feature rows themselves labels the points to touch."""
+kept of a 2-D teacher's scores.  The same head on the feature rows themselves labels the points to touch.
+
+The rows and the head are the caller's to optimize: ``SplatTrainer`` takes the reference's parameters only, so train them on
+Gaussians that are no longer split or culled (each of those leaves N, and with it the rows, behind)."""
 from __future__ import annotations
 
 import math
