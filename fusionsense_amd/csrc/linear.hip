@@ -1215,41 +1215,50 @@ __global__ __launch_bounds__(C * R) void reduce_slices_kernel(const float *__res
                                                               int slices) {
     __shared__ float part[R][C];
     const int c = threadIdx.x % C, r = threadIdx.x / C;
-    const int64_t i = (int64_t)blockIdx.x * C + c;
-    const bool first = i < n1, second = !first && i < n1 + n2;
-    const float *from = first ? p1 + i : p2 + (i - n1);
-    const int64_t pitch = first ? n1 : n2;
-    float s = 0.f;
-    if (first || second) {
-        int t = r;
-        for (; t + 7 * R < slices; t += 8 * R) {
-            float v[8];
+    for (int64_t base = (int64_t)blockIdx.x * C; base < n1 + n2; base += (int64_t)gridDim.x * C) {
+        const int64_t i = base + c;
+        const bool first = i < n1, second = !first && i < n1 + n2;
+        const float *from = first ? p1 + i : p2 + (i - n1);
+        const int64_t pitch = first ? n1 : n2;
+        float s = 0.f;
+        if (first || second) {
+            int t = r;
+            for (; t + 7 * R < slices; t += 8 * R) {
+                float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = from[(t + u * R) * pitch];
+                for (int u = 0; u < 8; ++u) v[u] = from[(t + u * R) * pitch];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) s += v[u];
+                for (int u = 0; u < 8; ++u) s += v[u];
+            }
+            for (; t < slices; t += R) s += from[t * pitch];
         }
-        for (; t < slices; t += R) s += from[t * pitch];
-    }
-    part[r][c] = s;
-    __syncthreads();
-    if (r == 0 && (first || second)) {
-        for (int t = 1; t < R; ++t) s += part[t][c];
-        if (first) out1[i] = (T)s;
-        else out2[i - n1] = (T)s;
+        if constexpr (R > 1) {
+            part[r][c] = s;
+            __syncthreads();
+            if (r == 0)
+                for (int t = 1; t < R; ++t) s += part[t][c];
+            __syncthreads();
+        }
+        if (r == 0 && first) out1[i] = (T)s;
+        if (r == 0 && second) out2[i - n1] = (T)s;
     }
 }
 
+constexpr int kSlicesOfOneThread = 4;
+
 // One or two arrays with the same number of slices.  Few values with many slices (db of a long layer: 1024 x 256) take 64 threads
-// each: 5.9 us.  (16 threads each over 4096 slices, a row per wave of the kernel before it, took 110 us.)
+// each: 5.9 us.  (16 threads each over 4096 slices, a row per wave of the kernel before it, took 110 us.)  A few slices of many
+// values take one thread each (4096 x 4096 bf16, two slices: 41 us, by sixteen threads each 399).
 template <typename T>
 int launch_reduce(const float *p1, int64_t n1, void *out1, const float *p2, int64_t n2, void *out2, int slices, hipStream_t s) {
     if (!out1) p1 = p2, n1 = n2, out1 = out2, n2 = 0;
     if (!out2) n2 = 0;
     const int64_t n = n1 + n2;
     T *const o1 = (T *)out1, *const o2 = (T *)out2;
-    if (slices > 512) reduce_slices_kernel<T, 16, 64><<<(unsigned)((n + 15) / 16), 1024, 0, s>>>(p1, n1, o1, p2, n2, o2, slices);
-    else reduce_slices_kernel<T, 64, 16><<<(unsigned)((n + 63) / 64), 1024, 0, s>>>(p1, n1, o1, p2, n2, o2, slices);
+    auto blocks = [&](int c) { return (unsigned)min((n + c - 1) / c, (int64_t)1 << 20); };  // (a grid holds at most 2^32 threads)
+    if (slices > 512) reduce_slices_kernel<T, 16, 64><<<blocks(16), 1024, 0, s>>>(p1, n1, o1, p2, n2, o2, slices);
+    else if (slices > kSlicesOfOneThread) reduce_slices_kernel<T, 64, 16><<<blocks(64), 1024, 0, s>>>(p1, n1, o1, p2, n2, o2, slices);
+    else reduce_slices_kernel<T, 256, 1><<<blocks(256), 256, 0, s>>>(p1, n1, o1, p2, n2, o2, slices);
     return check_launch();
 }
 

@@ -418,6 +418,26 @@ def test_linear_wide_gradients_keep_dz(dev, size, dtype, act):
     _check_two_values(size, x, w, b, act, dy, f"{size} {act}")
 
 
+def test_linear_gradients_of_very_large_weights(dev):
+    """16 400 x 16 400 weights, more values than a grid has groups of 16 threads for: dx whole, dW and db by blocks of rows."""
+    M, D, dtype = 3, 16400, torch.bfloat16
+    assert D * D * 16 > 2 ** 32
+    g = torch.Generator(device=dev).manual_seed(0)
+    x, b, dy = (torch.randn(s, generator=g, device=dev).to(dtype) for s in ((M, D), (D,), (M, D)))
+    w = torch.randn(D, D, generator=g, device=dev).div_(math.sqrt(D)).to(dtype)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops.linear_act(*leaves, "gelu"), leaves, dy)
+    want, err, mag = 0, 0, 0
+    for n in range(0, D, 1025):
+        wn = w[n:n + 1025].detach()
+        part = S.linear(x, wn, b[n:n + 1025], None, "gelu", dy[:, n:n + 1025])
+        S.check(dw[n:n + 1025], part["dw"], f"dw {n}")
+        S.check(db[n:n + 1025], part["db"], f"db {n}")
+        v, e = part["dx"]  # (with a rounding to the type that only the whole has: the bound is the larger for it)
+        want, err, mag = want + v, err + e, mag + v.abs()
+    S.check(dx, (want, err + 17 * S.U32 * mag + S.U[dtype] * want.abs()), "dx")
+
+
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("size", [(700, 64, 128), (300, 128, 40), (500, 300, 70)], ids=lambda s: "x".join(map(str, s)))
 def test_linear_largest_fp16_gradients(dev, size, act):
