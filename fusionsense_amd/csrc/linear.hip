@@ -42,8 +42,8 @@ __device__ __forceinline__ float normal_tail(float z, float &e) {
 
 // The tail at |z| for the half-width types' forward as one exponential: 2^Q(|z|), Q a polynomial fitted here to log2 of the tail.
 // bf16: degree 9 on [0, 13.2]; relative errors below 5e-6 at |z| < 1, 3.1e-5 < 2, 1e-4 everywhere, a twentieth of an output's
-// half step or less.  fp16: degree 7 on [0, 6], behind which outputs are zero; 5.6e-6, a fortieth.  Both fall on behind
-// their ranges.  (640 000 rows, 64 -> 128: bf16 61 us, fp16 59; by the form above, with its reciprocal, 65 and 72.)
+// half step or less.  fp16: degree 7 on [0, 6], behind which outputs are zero; 5.6e-6 (1e-5 with fp32's roundings, a
+// twenty-fifth).  Both fall on behind their ranges.  (640 000 rows, 64 -> 128: bf16 61 us, fp16 59; by the form above, with its reciprocal, 65 and 72.)
 template <typename T>
 __device__ __forceinline__ float normal_tail_half(float z) {
     const float a = fabsf(z);

@@ -200,8 +200,9 @@ def test_linear_activation_over_its_range(dev, dtype, act):
 
     gelu's tail h = P(t) exp(-z^2/2) is off by its fit, 1.3e-9, and relatively by the exponent's rounding, z^2 / 2 times two
     roundings, and by 32 U32 for P (seven steps, magnitudes 2.7 times the sum), the reciprocal and the exponential; bf16's form by
-    1e-4, fp16's by 5.6e-6 and 32 U32 for |z| <= 6 (Q's terms sum to 44 there: 22 U32 of Q, less of h) and by 2^-26 beyond.  y = max(z, 0) - |z| h; the slope is h - |z| phi, or one minus that.  silu's sigma is off by (2 |z| + 8) U32 of itself.
-    The type's rounding comes last; dz enters its product as two values of a half-width type."""
+    1e-4; fp16's by 5.6e-6 and, for |z| <= 6, by 72 U32 (one rounding a step of Q's evaluation: their magnitudes sum to 100, ln 2
+    of which is h's, and the exponential's two), by 2^-26 beyond.  y = max(z, 0) - |z| h; the slope is h - |z| phi, or one minus
+    that.  silu's sigma is off by (2 |z| + 8) U32 of itself.  The type's rounding comes last; dz enters its product as two values of a half-width type."""
     z = torch.linspace(-14, 14, 100000).to(dtype)
     x = z[:, None].to(dev).requires_grad_(True)
     y = ops.linear_act(x, torch.ones(1, 1, dtype=dtype, device=dev), None, act)
@@ -213,7 +214,7 @@ def test_linear_activation_over_its_range(dev, dtype, act):
         rel = (z * z + 32) * S.U32
         # (the exponential instruction gives zero for what lies below 2^-126, bf16's tail from |z| = 13.1 on: off by that at most)
         ey = size * {torch.float32: 1.3e-9 + rel * h, torch.bfloat16: 1e-4 * h + 2.0 ** -126,
-                     torch.float16: (5.6e-6 + 32 * S.U32) * h}[dtype]
+                     torch.float16: (5.6e-6 + 72 * S.U32) * h}[dtype]
         if dtype == torch.float16:
             ey = ey + 2.0 ** -26 * (size > 6)
         es = 1.3e-9 + rel * (h + size * phi) + 2 * S.U32
@@ -411,7 +412,7 @@ def test_linear_thin_gradients_keep_dz(dev, size, dtype, act):
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("size", DZ[2:] + [(7000, 200, 50), (300, 256, 64), (129, 64, 257), (16, 300, 200), (1, 300, 1000), (513, 130, 33),
-                                           (70000, 32, 256), (20000, 136, 17)], ids=lambda s: "x".join(map(str, s)))
+                                           (70000, 32, 256), (20000, 136, 17), (17000, 136, 1024), (33000, 300, 528)], ids=lambda s: "x".join(map(str, s)))
 def test_linear_wide_gradients_keep_dz(dev, size, dtype, act):
     """... of wider layers: every kernel that forms dz or takes it, one slice of the rows and several."""
     x, w, b, r, dy = _layer(dev, *size, dtype, res=False, seed=160 + size[0])
