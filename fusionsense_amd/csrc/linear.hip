@@ -25,8 +25,8 @@ struct LinArgs {
 };
 
 // The normal distribution's tail h = P(t) exp(-z^2 / 2) at |z|, t = 1 / (1 + c |z|), P a polynomial without a constant term
-// fitted here to erfc over rounded coefficients; P and the exponential apart.  The fit is off by 1.3e-9 of h at most, a fiftieth
-// of half an fp32 step at 1; its evaluation in fp32 adds 1.5e-7, two and a half of those.  The slopes of every type and
+// fitted here to erfc over rounded coefficients; P and the exponential apart.  The fit is off by 1.3e-9 at most (h is a half at
+// zero), a fiftieth of half an fp32 step at 1; its evaluation in fp32 adds 1.5e-7, two and a half of those.  The slopes of every type and
 // fp32's forward use it.
 __device__ __forceinline__ float normal_tail(float z, float &e) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.32f, fabsf(z), 1.f));
@@ -611,7 +611,7 @@ __global__ __launch_bounds__(64 * rows_waves(STORE)) void linear_rows_kernel(Row
             for (int q = 0; q < CPG; ++q) {
                 const int n = column(g, q);
                 if (m < a.rows && n < ncols) {
-                    if constexpr (STORE == kStoreTile) put_chunk((T *)mine + off + li * a.N + n, pack_chunk<T>(z + q * CE), ncols - n, false);
+                    if constexpr (STORE == kStoreTile) put_values<T, MODE>((T *)mine + off + li * a.N + n, z + q * CE, ncols - n, false, 0);
                     else put_values<T, MODE>(y + m * a.yp + n0 + n, z + q * CE, ncols - n, STORE == kStoreStream, a.lo);
                 }
             }
@@ -917,8 +917,8 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void linear_bwd_rows_kernel(BwdR
 }
 
 // ---- backward of a few rows and outputs, half width: one launch ------------------------------------------------------------
-// Every workgroup forms all of dz (rows x N) by itself in fp32 LDS and takes 32 columns of dW and dx.  Bound by latency: 16 rows, 64 -> 20
-// bf16 gelu 6.5 us; one row, 64 -> 150 11.4, where four rows take 18 in the one-pass kernel and its sum over slices; one row,
+// Every workgroup forms all of dz (rows x N) by itself in fp32 LDS and takes 32 columns of dW and dx.  Bound by latency: 16
+// rows, 64 -> 20 bf16 gelu 6.5 us; one row, 64 -> 150 11.4, where four rows take 18 in the one-pass kernel and its sum over slices; one row,
 // 512 -> 512 48.
 constexpr int kSmallDz = 512, kSmallCols = 32, kSmallWaves = 8;
 constexpr int64_t kSmallWeights = 1 << 18;  // every workgroup reads all of W: up to half a megabyte
@@ -1244,11 +1244,12 @@ __global__ __launch_bounds__(C * R) void reduce_slices_kernel(const float *__res
     }
 }
 
-constexpr int kSlicesOfOneThread = 4;
+constexpr int kSlicesOfOneThread = 32;
 
 // One or two arrays with the same number of slices.  Few values with many slices (db of a long layer: 1024 x 256) take 64 threads
-// each: 5.9 us.  (16 threads each over 4096 slices, a row per wave of the kernel before it, took 110 us.)  A few slices of many
-// values take one thread each (4096 x 4096 bf16, two slices: 41 us, by sixteen threads each 399).
+// each: 5.9 us.  (16 threads each over 4096 slices, a row per wave of the kernel before it, took 110 us.)  Few slices take
+// one thread a value (by sixteen: 4096 x 4096 values of two slices 41 us (399), 600 x 600 of 8 to 32 slices 4.8 (13.1), 128 x 128 of
+// as many 3.6 (3.5)).
 template <typename T>
 int launch_reduce(const float *p1, int64_t n1, void *out1, const float *p2, int64_t n2, void *out2, int slices, hipStream_t s) {
     if (!out1) p1 = p2, n1 = n2, out1 = out2, n2 = 0;
